@@ -340,6 +340,118 @@ SC_API int32_t sc_pipeline_plan(const sc_pipeline* p, int32_t offload, const int
 SC_API int32_t sc_pipeline_destroy(sc_pipeline* p);
 
 /*
+ * Operators of a model step on and next to a restored cache.  None has a counterpart in the
+ * reference, whose caches are read by the model's own attention.  They allocate nothing and
+ * compute no gradients.
+ */
+
+/*
+ * Rotary positions of new queries and keys, one launch for both.  For frequency i of a token at
+ * position p, a = p * inv_freq[i]:
+ *   (y1, y2) = factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a)
+ * over pairs (x[i], x[i + R/2]), or (x[2i], x[2i + 1]) with `interleaved`; elements from
+ * R = rotary_dim on are copied.  `inverse` turns by -a and divides by factor.  Angles are kept
+ * as 64-bit fractions of a turn (at most 2^-33 of a turn off for positions below 2^31), products
+ * in fp32, one rounding.
+ *
+ *  q, k       [batch, tokens, heads, head_dim]; strides {batch, token, head, dim}; k may be NULL
+ *  dtype      SC_DTYPE_F16, _BF16 or _F32 of all four tensors
+ *  positions  device int64 (positions_are_64) or int32, strides {batch, token}; NULL: token t is
+ *             at pos_start + t
+ *  inv_freq   host float64 [rotary_dim / 2], radians per position
+ *  q_out may be q and k_out may be k (same strides); head_dim <= 1024, rotary_dim <= 512
+ */
+SC_API int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_heads, int32_t k_heads,
+                             int32_t head_dim, int32_t rotary_dim, int32_t interleaved,
+                             const void* q, const int64_t* q_strides, const void* k,
+                             const int64_t* k_strides, int32_t dtype, const void* positions,
+                             int32_t positions_are_64, const int64_t* pos_strides,
+                             int64_t pos_start, const double* inv_freq, double factor,
+                             int32_t inverse, void* q_out, const int64_t* qo_strides, void* k_out,
+                             const int64_t* ko_strides, void* stream);
+
+/*
+ * Attention of a batch that shares a prefix: each sequence's queries see the whole prefix and,
+ * of the sequence's own cache, the tokens t <= len - n + j (query j of n), so the newest query
+ * sees all of it.  A row that sees nothing gives zeros and a log-sum-exp of -infinity.
+ *
+ *  q, out       [n_tokens, q_heads, head_dim], the sequences' tokens one after another; strides
+ *               {token, head}; unit stride along head_dim in every tensor
+ *  k/v_prefix   [prefix_len, kv_heads, head_dim], strides {token, head}; may be NULL at length 0
+ *  k/v_cache    [batch, cache_len, kv_heads, head_dim], strides {batch, token, head}; with
+ *               page_table a pool [n_pages, page_size, kv_heads, head_dim], strides {page, token,
+ *               head}, and cache_len = page_size * entries of a page-table row; without
+ *               page_table, page_size = cache_len
+ *  cache_lens   device int32 [batch], tokens in use (the queries' own among them); NULL: all
+ *  page_table   device int32, row stride page_table_stride
+ *  cu_q_lens    device int32 [batch + 1], each sequence's first token; NULL: max_q_len each.
+ *               Rows behind the last sequence are left as they were.
+ *  lse          float32 [n_tokens, q_heads], natural logarithm, contiguous; may be NULL
+ *  workspace    of sc_shared_prefix_attention_workspace bytes, 16-byte aligned, for this call
+ *               alone until its work has completed
+ *  status       device word (SC_STATUS_*): a bad page's tokens count as masked, a bad length as 0
+ *  dtype        SC_DTYPE_F16 or _BF16; head_dim a multiple of 8, at most 256; rows start at
+ *               multiples of 16 bytes; out overlaps no input
+ */
+SC_API int32_t sc_shared_prefix_attention_workspace(int64_t n_tokens, int32_t batch, int32_t q_heads,
+                                                    int32_t kv_heads, int32_t head_dim,
+                                                    int64_t max_q_len, int64_t prefix_len,
+                                                    int64_t cache_len, int32_t page_size,
+                                                    int64_t* bytes);
+SC_API int32_t sc_shared_prefix_attention(
+    int64_t n_tokens, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+    int32_t dtype, const void* q, const int64_t* q_strides, int64_t prefix_len, const void* k_prefix,
+    const int64_t* kp_strides, const void* v_prefix, const int64_t* vp_strides, int64_t cache_len,
+    const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,
+    const int32_t* cache_lens, const int32_t* page_table, int64_t page_table_stride, int32_t page_size,
+    int64_t n_pages, const int32_t* cu_q_lens, int64_t max_q_len, double scale, void* out,
+    const int64_t* out_strides, float* lse, void* workspace, int64_t workspace_bytes, int32_t* status,
+    void* stream);
+
+/*
+ * Attention weights added up per cached token:
+ *   out[b, h, t] = scores[b, h, t] + sum over queries j of sequence b and heads g of group h that
+ *                  see t of exp(scale * q[j, g] . k[b, t, h] - lse[j, g])
+ * with the visibility of the attention above (causal = 0: every query sees every token in use).
+ * Tokens not in use keep their score.  No atomics: the same inputs give the same bits.
+ *
+ *  lse     float32, strides {token, head}
+ *  scores, out  float32 [batch, kv_heads, cache_len], strides {batch, head}; out may be scores
+ *  the rest as in sc_shared_prefix_attention (dense caches)
+ */
+SC_API int32_t sc_accumulate_attention_weights(
+    int64_t n_tokens, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+    int32_t dtype, const void* q, const int64_t* q_strides, int64_t cache_len, const void* k_cache,
+    const int64_t* kc_strides, const int32_t* cache_lens, const int32_t* cu_q_lens,
+    int64_t max_q_len, int32_t causal, double scale, const float* lse, const int64_t* lse_strides,
+    const float* scores, const int64_t* scores_strides, float* out, const int64_t* out_strides,
+    int32_t* status, void* stream);
+
+/*
+ * Eviction: per sequence and KV head min(len, budget) tokens stay - the first keep_first, the last
+ * keep_recent and, of the others, those of the highest score (equal scores: the lower index
+ * first; NaN counts as minus infinity) - and move to the front in their order.
+ *
+ *  k/v_cache  [batch, cache_len, n_heads, head_dim] of elem_size-byte elements, strides {batch,
+ *             token, head}; cache_len <= 393216; rows of a multiple of 16 bytes
+ *  scores     float32 [batch, n_heads, cache_len], strides {batch, head}
+ *  k/v_out    [batch, budget, n_heads, head_dim]; scores_out [batch, n_heads, budget].  Rows
+ *             behind the new length are left as they were.
+ *  in_place   an output is its input (same address and strides); otherwise no two overlap
+ *  indices    int32 [batch, n_heads, budget] contiguous: where each kept token was, then -1
+ *  new_lens   int32 [batch]
+ */
+SC_API int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache_len, int32_t head_dim,
+                               int32_t elem_size, int64_t budget, int64_t keep_first,
+                               int64_t keep_recent, const void* k_cache, const int64_t* kc_strides,
+                               const void* v_cache, const int64_t* vc_strides, const float* scores,
+                               const int64_t* scores_strides, const int32_t* cache_lens,
+                               int32_t in_place, void* k_out, const int64_t* ko_strides,
+                               void* v_out, const int64_t* vo_strides, float* scores_out,
+                               const int64_t* so_strides, int32_t* indices, int32_t* new_lens,
+                               int32_t* status, void* stream);
+
+/*
  * Sharing a device buffer between the processes of one machine (CUDA IPC), for the gather of
  * head shards onto one GPU: the owner exports the buffer, each other rank imports it and
  * passes the returned pointer (plus its shard's head offset) as the output of its restore,

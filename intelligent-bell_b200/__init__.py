@@ -10,7 +10,10 @@ the C ABI of ``libspeccache_b200.so`` (declared in ``include/speccache_b200.h``)
 * ``compute_rope_cos_sin_delta`` — shift tables;
 * ``restore_paged`` — ragged, paged gather + restore in one launch;
 * ``restore_layers`` — many layers in one launch;
-* ``cache.KVRestorePipeline`` — pinned-host -> GPU multi-layer restore.
+* ``cache.KVRestorePipeline`` — pinned-host -> GPU multi-layer restore;
+* ``apply_rotary`` — rotary positions of new queries and keys;
+* ``shared_prefix_attention`` — attention of a batch over a restored prefix and its own caches;
+* ``accumulate_attention_weights`` / ``evict_tokens`` — a cache cut to what its queries looked at.
 
 The directory name is not a Python identifier; import it with
 ``importlib.import_module("intelligent-bell_b200")`` (it also registers the alias
@@ -22,6 +25,10 @@ import sys as _sys
 from . import _lib
 from ._build import LIB_PATH, build_library
 from .kernels import (
+    Evicted,
+    RopeScaling,
+    accumulate_attention_weights,
+    apply_rotary,
     compute_rope_cos_sin_delta,
     dequant_and_rope_key,
     dequant_and_rope_key_compiled,
@@ -30,6 +37,7 @@ from .kernels import (
     dequant_value,
     dequant_value_compiled,
     dequant_value_ref,
+    evict_tokens,
     fused_k_dequant_rope_shift_kernel,
     paged_status,
     pytorch_compiled_dequant_rope_shift,
@@ -39,7 +47,9 @@ from .kernels import (
     restore_layers,
     restore_paged,
     rope_shift_keys,
+    rotary_frequencies,
     rotate_half,
+    shared_prefix_attention,
     triton_fused_k_dequant_rope_shift,
     validate_key_inputs,
     validate_value_inputs,
@@ -68,6 +78,10 @@ __all__ = [
     "LIB_PATH",
     "build_library",
     "preload",
+    "Evicted",
+    "RopeScaling",
+    "accumulate_attention_weights",
+    "apply_rotary",
     "compute_rope_cos_sin_delta",
     "dequant_and_rope_key",
     "dequant_and_rope_key_compiled",
@@ -76,6 +90,7 @@ __all__ = [
     "dequant_value",
     "dequant_value_compiled",
     "dequant_value_ref",
+    "evict_tokens",
     "fused_k_dequant_rope_shift_kernel",
     "paged_status",
     "pytorch_compiled_dequant_rope_shift",
@@ -85,7 +100,9 @@ __all__ = [
     "restore_layers",
     "restore_paged",
     "rope_shift_keys",
+    "rotary_frequencies",
     "rotate_half",
+    "shared_prefix_attention",
     "triton_fused_k_dequant_rope_shift",
     "validate_key_inputs",
     "validate_value_inputs",

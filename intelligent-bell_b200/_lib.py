@@ -90,6 +90,30 @@ _SIGNATURES = {
     "sc_pipeline_restore_launches": (_i32, [_vp, _i32, _vp]),
     "sc_pipeline_plan": (_i32, [_vp, _i32, _vp, _i32, _vp, _vp]),
     "sc_pipeline_destroy": (_i32, [_vp]),
+    "sc_rope_apply": (_i32, [_i32, _i64, _i32, _i32, _i32, _i32, _i32,
+                             _vp, _vp, _vp, _vp, _i32,   # q, k, dtype
+                             _vp, _i32, _vp, _i64,       # positions
+                             _vp, _f64, _i32,            # inv_freq, factor, inverse
+                             _vp, _vp, _vp, _vp, _vp]),
+    "sc_shared_prefix_attention_workspace": (_i32, [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64,
+                                                    _i32, _vp]),
+    "sc_shared_prefix_attention": (_i32, [_i64, _i32, _i32, _i32, _i32, _i32,
+                                          _vp, _vp,                      # q
+                                          _i64, _vp, _vp, _vp, _vp,      # prefix
+                                          _i64, _vp, _vp, _vp, _vp,      # own caches
+                                          _vp, _vp, _i64, _i32, _i64,    # lengths, pages
+                                          _vp, _i64, _f64,               # cu_q_lens, scale
+                                          _vp, _vp, _vp, _vp, _i64, _vp, _vp]),
+    "sc_accumulate_attention_weights": (_i32, [_i64, _i32, _i32, _i32, _i32, _i32,
+                                               _vp, _vp, _i64, _vp, _vp,  # q, cache
+                                               _vp, _vp, _i64, _i32, _f64,
+                                               _vp, _vp, _vp, _vp, _vp, _vp,  # lse, scores, out
+                                               _vp, _vp]),
+    "sc_evict_tokens": (_i32, [_i32, _i32, _i64, _i32, _i32, _i64, _i64, _i64,
+                               _vp, _vp, _vp, _vp, _vp, _vp,   # caches, scores
+                               _vp, _i32,
+                               _vp, _vp, _vp, _vp, _vp, _vp,   # outputs
+                               _vp, _vp, _vp, _vp]),
     "sc_ipc_export": (_i32, [_vp, _vp, _vp]),
     "sc_ipc_import": (_i32, [_vp, _i64, _vp, _vp]),
     "sc_ipc_close": (_i32, [_vp]),

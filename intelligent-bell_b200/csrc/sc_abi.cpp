@@ -76,6 +76,10 @@ int32_t sc_preload_kernels(void) {
     if (e == cudaSuccess) e = sc::preload_paged_kernels();
     if (e == cudaSuccess) e = sc::preload_quantize_kernels(true);
     if (e == cudaSuccess) e = sc::preload_shift_kernels();
+    if (e == cudaSuccess) e = sc::preload_rotary_kernels();
+    if (e == cudaSuccess) e = sc::preload_attention_kernels();
+    if (e == cudaSuccess) e = sc::preload_weights_kernels();
+    if (e == cudaSuccess) e = sc::preload_evict_kernels();
     if (e != cudaSuccess) return sc::cuda_error(e, "loading the kernels");
     return sc::ok();
 }

@@ -1,0 +1,654 @@
+// sc_attention.cu — attention of a batch that shares a long prefix.
+//
+// Mathematics.  A query row (token j of sequence b, head h) sees the P prefix tokens and the
+// tokens t <= len_b - n_b + j of its own cache:
+//   o = sum_t e^{s_t - m} v_t / sum_t e^{s_t - m},  s_t = scale q . k_t,  m = max_t s_t.
+// The sums are split over token ranges ("parts"); a part keeps (m, l, o) not normalised and
+// parts join by rescaling to the common maximum.  All rows of all sequences read the prefix
+// together: rows of one KV head are packed (token, head of the group) over the whole batch, so a
+// prefix token is loaded once for 16 or 32 rows instead of once per sequence.
+//
+// attend_rows: 16 * MT rows of one KV head against one part.  The four warps take turns at tiles
+// of TK tokens; each keeps its own ring of tiles in shared memory (cp.async, 16 bytes a lane),
+// its own softmax state and its own 16-bit-input, fp32-accumulating matrix products, and the
+// four states are joined at the end of the part.  Rows of a tile are stored with their 16-byte
+// chunks permuted by the row number, so ldmatrix reads without bank conflicts.
+// join_parts: one warp a row adds the parts up.
+#include <math.h>
+
+#include "sc_attention.cuh"
+
+namespace sc {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kPartTokens = 64;    // parts are multiples of this many tokens
+constexpr int kMaxPagesPerPart = 2048;
+
+// Byte offset of 16-byte chunk c of row r in a tile of DP-element rows.
+template <int DP>
+__device__ __forceinline__ uint32_t chunk_at(int r, int c) {
+    return static_cast<uint32_t>(r) * (DP * 2) + static_cast<uint32_t>((c ^ (r & 7)) * 16);
+}
+
+template <int DP, int MT, int TK, int NST>
+struct RowsShape {
+    static constexpr int kRing = kWarps * NST * 2 * TK * DP * 2;  // bytes of the warps' rings
+    static constexpr int kSmem = 16 * MT * DP * 2 + kRing;
+};
+
+template <typename T, int DP, int MT, int TK, int NST>
+__global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ AttnParams p) {
+    constexpr int MR = 16 * MT;
+    constexpr int CPR = DP / 8;            // chunks a row
+    constexpr int RPI = 32 / CPR;          // rows a warp-wide copy covers
+    constexpr int KT = TK * DP * 2;        // bytes of a K (or V) tile
+    static_assert(kWarps * MR * DP * 4 <= RowsShape<DP, MT, TK, NST>::kRing, "join buffer");
+    extern __shared__ __align__(128) unsigned char smem[];
+    __shared__ int32_t s_page[kMaxPagesPerPart];
+    __shared__ float s_m[kWarps][MR], s_l[kWarps][MR];
+    __shared__ int s_bad;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    unsigned char* s_q = smem;
+    unsigned char* s_ring = smem + MR * DP * 2;
+
+    // Which rows and tokens: own caches first (they are the longer wait), then the prefix.
+    int u = blockIdx.x;
+    const int n_cache_units = p.n_cp * p.tiles_c * p.Hkv * p.B;
+    const bool is_prefix = u >= n_cache_units;
+    int b = 0, part;
+    if (is_prefix) u -= n_cache_units;
+    const int tiles = is_prefix ? p.tiles_p : p.tiles_c;
+    const int rt = u % tiles;
+    u /= tiles;
+    const int h = u % p.Hkv;
+    u /= p.Hkv;
+    int tok0, n_tok;
+    if (is_prefix) {
+        part = u;
+        tok0 = 0;
+        n_tok = used_tokens(p);
+    } else {
+        part = u % p.n_cp;
+        b = u / p.n_cp;
+        sequence_tokens(p, b, tok0, n_tok);
+    }
+    const int rows = n_tok * p.G;
+    const int r0 = rt * MR;
+    if (r0 >= rows) return;
+    const int n_rows = min(MR, rows - r0);
+
+    int t0, t1, see = 0;  // see: own cache tokens the first token of the sequence sees, minus one
+    if (is_prefix) {
+        t0 = part * p.chunk_p;
+        t1 = min(p.P, t0 + p.chunk_p);
+    } else {
+        const int len = cache_length(p, b);
+        const int blocks = (len + kPartTokens - 1) / kPartTokens;
+        const int chunk = (blocks + p.n_cp - 1) / p.n_cp * kPartTokens;
+        see = len - n_tok;
+        const int j_last = static_cast<int>(fdiv(r0 + n_rows - 1, p.div_G));
+        t0 = part * chunk;
+        t1 = min(min(len, t0 + chunk), see + j_last + 1);
+        part += p.n_pp;
+    }
+    const int64_t part_row = static_cast<int64_t>(part) * p.N * p.Hq;
+    if (t0 >= t1) {
+        for (int r = threadIdx.x; r < n_rows; r += kThreads) {
+            const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+            const int g = r0 + r - j * p.G;
+            p.part_ml[part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + g] =
+                make_float2(kNegInf, 0.f);
+        }
+        return;
+    }
+
+    // Queries of the tile, zeros behind the last row and behind D.
+    for (int i = threadIdx.x; i < MR * CPR; i += kThreads) {
+        const int r = i / CPR, c = i - r * CPR;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && c * 8 < p.D) {
+            const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+            const int g = r0 + r - j * p.G;
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (tok0 + j) * p.q_t +
+                                                (h * p.G + g) * p.q_h + c * 8);
+        }
+        *reinterpret_cast<uint4*>(s_q + chunk_at<DP>(r, c)) = v;
+    }
+    if (p.D < DP) {  // columns that no copy writes
+        for (int i = threadIdx.x; i < RowsShape<DP, MT, TK, NST>::kRing / 16; i += kThreads)
+            reinterpret_cast<uint4*>(s_ring)[i] = make_uint4(0, 0, 0, 0);
+    }
+    const bool paged = !is_prefix && p.page_table != nullptr;
+    int first_page = 0;
+    if (threadIdx.x == 0) s_bad = 0;
+    __syncthreads();
+    if (paged) {
+        first_page = static_cast<int>(fdiv(t0, p.div_page));
+        const int last = static_cast<int>(fdiv(t1 - 1, p.div_page));
+        for (int i = threadIdx.x; i <= last - first_page; i += kThreads) {
+            int id = p.page_table[b * p.pt_b + first_page + i];
+            if (id < 0 || id >= p.n_pages) {
+                id = -1;
+                s_bad = 1;
+                if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
+            }
+            s_page[i] = id;
+        }
+        __syncthreads();
+    }
+    const bool bad = s_bad != 0;
+
+    const T* kbase;
+    const T* vbase;
+    int64_t k_t, v_t, k_b = 0, v_b = 0;
+    if (is_prefix) {
+        kbase = static_cast<const T*>(p.kp) + h * p.kp_h;
+        vbase = static_cast<const T*>(p.vp) + h * p.vp_h;
+        k_t = p.kp_t, v_t = p.vp_t;
+    } else {
+        kbase = static_cast<const T*>(p.kc) + h * p.kc_h;
+        vbase = static_cast<const T*>(p.vc) + h * p.vc_h;
+        k_t = p.kc_t, v_t = p.vc_t, k_b = p.kc_b, v_b = p.vc_b;
+        if (!paged) kbase += b * k_b, vbase += b * v_b;
+    }
+
+    const uint32_t ring = smem_addr(s_ring) + warp * NST * 2 * KT;
+    const int n_tiles = (t1 - t0 + TK - 1) / TK;
+    const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
+
+    auto issue = [&](int i) {
+        if (i < my_tiles) {
+            const uint32_t dst = ring + (i % NST) * 2 * KT;
+            const int tt = t0 + (warp + i * kWarps) * TK;
+            const int c = lane % CPR;
+            if (c * 8 < p.D) {
+#pragma unroll
+                for (int it = 0; it < TK / RPI; ++it) {
+                    const int r = it * RPI + lane / CPR;
+                    const int t = tt + r;
+                    bool valid = t < t1;
+                    int64_t ko = 0, vo = 0;
+                    if (valid) {
+                        if (paged) {
+                            const int pg = static_cast<int>(fdiv(t, p.div_page));
+                            const int id = s_page[pg - first_page];
+                            const int in = t - pg * p.page;
+                            valid = id >= 0;
+                            if (valid) {
+                                ko = id * k_b + in * k_t;
+                                vo = id * v_b + in * v_t;
+                            }
+                        } else {
+                            ko = t * k_t;
+                            vo = t * v_t;
+                        }
+                    }
+                    cp_async16(dst + chunk_at<DP>(r, c), kbase + ko + c * 8, valid);
+                    cp_async16(dst + KT + chunk_at<DP>(r, c), vbase + vo + c * 8, valid);
+                }
+            }
+        }
+        cp_async_commit();
+    };
+
+    float o[MT][DP / 8][4];
+    float m[MT][2], l[MT][2];
+    int lim[MT][2];  // tokens below it are seen
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            m[mt][e] = kNegInf;
+            l[mt][e] = 0.f;
+            const int r = mt * 16 + e * 8 + (lane >> 2);
+            const int j = static_cast<int>(fdiv(min(r0 + r, rows - 1), p.div_G));
+            lim[mt][e] = is_prefix ? t1 : min(t1, see + j + 1);
+        }
+#pragma unroll
+        for (int n = 0; n < DP / 8; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+    }
+    // Tiles that end below it are seen whole by every row.
+    const int whole = bad ? -1 : is_prefix ? t1 : min(t1, see + static_cast<int>(fdiv(r0, p.div_G)) + 1);
+
+    for (int i = 0; i < NST - 1; ++i) issue(i);
+    const uint32_t q_addr = smem_addr(s_q);
+    for (int i = 0; i < my_tiles; ++i) {
+        cp_async_wait<NST - 2>();
+        __syncwarp();
+        issue(i + NST - 1);
+        const uint32_t kt = ring + (i % NST) * 2 * KT, vt = kt + KT;
+        const int tt = t0 + (warp + i * kWarps) * TK;
+
+        float s[MT][TK / 8][4];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+#pragma unroll
+        for (int kk = 0; kk < DP / 16; ++kk) {
+            uint32_t a[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+                ldmatrix4(a[mt], q_addr + chunk_at<DP>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+#pragma unroll
+            for (int n = 0; n < TK / 16; ++n) {
+                uint32_t kb[4];
+                ldmatrix4(kb, kt + chunk_at<DP>(n * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                                kk * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816<T>(s[mt][2 * n], a[mt], kb[0], kb[1]);
+                    mma16816<T>(s[mt][2 * n + 1], a[mt], kb[2], kb[3]);
+                }
+            }
+        }
+        const bool mask = tt + TK > whole;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float mx[2] = {m[mt][0], m[mt][1]};
+#pragma unroll
+            for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = s[mt][n][e] * p.scale_log2;
+                    if (mask) {
+                        const int t = tt + n * 8 + (lane & 3) * 2 + (e & 1);
+                        bool seen = t < lim[mt][e >> 1];
+                        if (bad && seen)
+                            seen = s_page[static_cast<int>(fdiv(t, p.div_page)) - first_page] >= 0;
+                        if (!seen) x = kNegInf;
+                    }
+                    s[mt][n][e] = x;
+                    mx[e >> 1] = fmaxf(mx[e >> 1], x);
+                }
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+            }
+            if (__any_sync(0xffffffffu, mx[0] > m[mt][0] || mx[1] > m[mt][1])) {
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const float f = mx[e] == kNegInf ? 1.f : exp2_fast(m[mt][e] - mx[e]);
+                    m[mt][e] = mx[e];
+                    l[mt][e] *= f;
+#pragma unroll
+                    for (int n = 0; n < DP / 8; ++n) {
+                        o[mt][n][2 * e] *= f;
+                        o[mt][n][2 * e + 1] *= f;
+                    }
+                }
+            }
+            const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+#pragma unroll
+            for (int n = 0; n < TK / 8; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float w = exp2_fast(s[mt][n][e] - base[e >> 1]);
+                    s[mt][n][e] = w;
+                    l[mt][e >> 1] += w;
+                }
+        }
+        // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
+        // rounding error goes in as a second product, since this kernel waits for memory and
+        // the products are free.
+#pragma unroll
+        for (int kk = 0; kk < TK / 16; ++kk) {
+            uint32_t hi[MT][4], lo[MT][4];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float x = s[mt][2 * kk + (e >> 1)][2 * (e & 1)];
+                    const float y = s[mt][2 * kk + (e >> 1)][2 * (e & 1) + 1];
+                    hi[mt][e] = pack2<T>(x, y);
+                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                        const float2 r = unpack2<T>(hi[mt][e]);
+                        lo[mt][e] = pack2<T>(x - r.x, y - r.y);
+                    }
+                }
+#pragma unroll
+            for (int n = 0; n < DP / 16; ++n) {
+                uint32_t vb[4];
+                ldmatrix4_t(vb, vt + chunk_at<DP>(kk * 16 + (lane & 7) + (((lane >> 3) & 1) << 3),
+                                                  n * 2 + (lane >> 4)));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    mma16816<T>(o[mt][2 * n], hi[mt], vb[0], vb[1]);
+                    mma16816<T>(o[mt][2 * n + 1], hi[mt], vb[2], vb[3]);
+                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                        mma16816<T>(o[mt][2 * n], lo[mt], vb[0], vb[1]);
+                        mma16816<T>(o[mt][2 * n + 1], lo[mt], vb[2], vb[3]);
+                    }
+                }
+            }
+        }
+    }
+
+    // Join the four warps' states.
+    cp_async_wait<0>();
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
+            l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
+            if ((lane & 3) == 0) {
+                s_m[warp][mt * 16 + e * 8 + (lane >> 2)] = m[mt][e];
+                s_l[warp][mt * 16 + e * 8 + (lane >> 2)] = l[mt][e];
+            }
+        }
+    __syncthreads();
+    float* s_o = reinterpret_cast<float*>(s_ring);  // [warp][MR][DP]
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            const int r = mt * 16 + e * 8 + (lane >> 2);
+            float all = s_m[0][r];
+#pragma unroll
+            for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_m[w][r]);
+            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - all);
+#pragma unroll
+            for (int n = 0; n < DP / 8; ++n)
+                *reinterpret_cast<float2*>(s_o + (warp * MR + r) * DP + n * 8 + (lane & 3) * 2) =
+                    make_float2(o[mt][n][2 * e] * f, o[mt][n][2 * e + 1] * f);
+        }
+    __syncthreads();
+    const int cpr = p.D / 4;
+    for (int i = threadIdx.x; i < n_rows * cpr; i += kThreads) {
+        const int r = i / cpr, c = (i - r * cpr) * 4;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+            const float4 v = *reinterpret_cast<const float4*>(s_o + (w * MR + r) * DP + c);
+            acc.x += v.x, acc.y += v.y, acc.z += v.z, acc.w += v.w;
+        }
+        const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+        const int64_t at = part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
+        *reinterpret_cast<float4*>(p.part_o + at * p.D + c) = acc;
+    }
+    for (int r = threadIdx.x; r < n_rows; r += kThreads) {
+        float all = s_m[0][r], sum = 0.f;
+#pragma unroll
+        for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_m[w][r]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+            sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - all));
+        const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+        p.part_ml[part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G] =
+            make_float2(all, sum);
+    }
+}
+
+// One warp a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over the parts, in order.
+template <typename T>
+__global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ AttnParams p) {
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int64_t all_rows = static_cast<int64_t>(p.N) * p.Hq;
+    if (row >= static_cast<int64_t>(used_tokens(p)) * p.Hq) return;
+    const int parts = p.n_pp + p.n_cp;
+    float m = kNegInf;
+    for (int i = lane; i < parts; i += 32) m = fmaxf(m, p.part_ml[i * all_rows + row].x);
+#pragma unroll
+    for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
+    float sum = 0.f;
+    const int d0 = lane * 4, d1 = 128 + lane * 4;
+    for (int i = 0; i < parts; ++i) {
+        const float2 ml = p.part_ml[i * all_rows + row];
+        if (ml.x == kNegInf && ml.y == 0.f) continue;  // nothing seen in this part
+        const float w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
+        sum += w * ml.y;
+        const float* src = p.part_o + (i * all_rows + row) * p.D;
+        if (d0 < p.D) {
+            const float4 v = *reinterpret_cast<const float4*>(src + d0);
+            a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w;
+        }
+        if (d1 < p.D) {
+            const float4 v = *reinterpret_cast<const float4*>(src + d1);
+            b.x += w * v.x, b.y += w * v.y, b.z += w * v.z, b.w += w * v.w;
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
+    const int64_t tok = row / p.Hq, head = row - tok * p.Hq;
+    T* dst = static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h;
+    if (d0 < p.D)
+        st_v2(dst + d0, make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)));
+    if (d1 < p.D)
+        st_v2(dst + d1, make_uint2(pack2<T>(b.x * inv, b.y * inv), pack2<T>(b.z * inv, b.w * inv)));
+    if (p.lse && lane == 0)
+        p.lse[row] = sum == 0.f ? kNegInf : (m + log2f(sum)) * 0.6931471805599453f;
+}
+
+struct Variant {
+    int dp, mt;
+};
+
+Variant pick_variant(int32_t D, int64_t rows) {
+    const int dp = D <= 64 ? 64 : D <= 128 ? 128 : 256;
+    return {dp, dp < 256 && rows > 16 ? 2 : 1};
+}
+
+template <typename T, int DP, int MT>
+cudaError_t launch_rows(const AttnParams& p, int64_t units, cudaStream_t s, bool load_only) {
+    constexpr int TK = 16, NST = DP == 64 ? 4 : 3;
+    constexpr int bytes = RowsShape<DP, MT, TK, NST>::kSmem;
+    auto kernel = attend_rows<T, DP, MT, TK, NST>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != cudaSuccess || load_only) return e;
+    kernel<<<static_cast<unsigned>(units), kThreads, bytes, s>>>(p);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_rows_dp(const AttnParams& p, Variant v, int64_t units, cudaStream_t s) {
+    if (v.dp == 64)
+        return v.mt == 1 ? launch_rows<T, 64, 1>(p, units, s, false)
+                         : launch_rows<T, 64, 2>(p, units, s, false);
+    if (v.dp == 128)
+        return v.mt == 1 ? launch_rows<T, 128, 1>(p, units, s, false)
+                         : launch_rows<T, 128, 2>(p, units, s, false);
+    return launch_rows<T, 256, 1>(p, units, s, false);
+}
+
+template <typename T>
+cudaError_t preload_attention_type() {
+    AttnParams p{};
+    cudaError_t e = launch_rows<T, 64, 1>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_rows<T, 64, 2>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_rows<T, 128, 1>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_rows<T, 128, 2>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_rows<T, 256, 1>(p, 0, nullptr, true);
+    cudaFuncAttributes attr;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, join_parts<T>);
+    return e;
+}
+
+// How the tokens are split.  Two blocks fit an SM; four rounds of equal parts keep the last
+// round's idle share small without making the parts' join expensive.
+struct Split {
+    int32_t tiles_p, tiles_c, chunk_p, n_pp, n_cp;
+    Variant v;
+};
+
+int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t nq, int32_t P,
+                   int32_t cap, int32_t page, Split* out) {
+    const int64_t G = Hq / Hkv;
+    const int64_t rows_p = N * G, rows_c = cap ? nq * G : 0;
+    Split s{};
+    s.v = pick_variant(D, rows_p > rows_c ? rows_p : rows_c);
+    const int64_t mr = 16 * s.v.mt;
+    s.tiles_p = static_cast<int32_t>((rows_p + mr - 1) / mr);
+    s.tiles_c = static_cast<int32_t>((rows_c + mr - 1) / mr);
+    const double work = static_cast<double>(P) * Hkv * s.tiles_p +
+                        static_cast<double>(cap) * Hkv * B * s.tiles_c;
+    double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
+    const double longest = P > cap ? P : cap;
+    const double most_parts = 64;
+    if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;
+    if (chunk < kPartTokens) chunk = kPartTokens;
+    s.chunk_p = static_cast<int32_t>(chunk > 0x40000000 ? 0x40000000 : chunk);
+    s.n_pp = P ? (P - 1) / s.chunk_p + 1 : 0;
+    s.n_cp = cap ? (cap - 1) / s.chunk_p + 1 : 0;
+    // A part's page ids are held in shared memory.
+    if (cap && page < cap) {
+        const int64_t room = static_cast<int64_t>(kMaxPagesPerPart - 1) * page / kPartTokens * kPartTokens;
+        const int64_t blocks = (static_cast<int64_t>(cap) + kPartTokens - 1) / kPartTokens;
+        const int64_t need = (blocks * kPartTokens + room - 1) / room;
+        if (need > s.n_cp) s.n_cp = static_cast<int32_t>(need);
+    }
+    const int64_t units = static_cast<int64_t>(s.n_pp) * s.tiles_p * Hkv +
+                          size_product(size_product(s.n_cp, s.tiles_c, Hkv), B);
+    if (units >= (int64_t(1) << 31))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "%lld blocks in one call; split it", (long long)units);
+    *out = s;
+    return SC_OK;
+}
+
+int32_t check_sizes(int64_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int64_t nq, int64_t P,
+                    int64_t cap) {
+    if (N < 0 || B < 0 || Hq < 0 || Hkv < 0 || nq < 0 || P < 0 || cap < 0)
+        return set_error(SC_ERR_INVALID_ARGUMENT, "negative size");
+    if (Hkv == 0 ? Hq != 0 : Hq % Hkv != 0)
+        return set_error(SC_ERR_INVALID_ARGUMENT, "%d query heads are no multiple of %d KV heads", Hq, Hkv);
+    if (D <= 0 || D % 8 != 0 || D > 256)
+        return set_error(SC_ERR_UNSUPPORTED, "head_dim %d: a multiple of 8, at most 256", D);
+    if (size_product(N, Hq) >= (int64_t(1) << 31) || P >= (int64_t(1) << 30) || cap >= (int64_t(1) << 30) ||
+        B >= (1 << 24) || size_product(nq, Hq) >= (int64_t(1) << 31))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "too many rows or tokens in one call; split it");
+    return SC_OK;
+}
+
+int64_t workspace_floats(const Split& s, int64_t N, int32_t Hq, int32_t D) {
+    return size_product(static_cast<int64_t>(s.n_pp) + s.n_cp, N * Hq, D + 2);
+}
+
+}  // namespace
+
+cudaError_t preload_attention_kernels() {
+    cudaError_t e = preload_attention_type<__half>();
+    if (e == cudaSuccess) e = preload_attention_type<__nv_bfloat16>();
+    return e;
+}
+
+}  // namespace sc
+
+using namespace sc;
+
+extern "C" int32_t sc_shared_prefix_attention_workspace(int64_t n_tokens, int32_t batch,
+                                                        int32_t q_heads, int32_t kv_heads,
+                                                        int32_t head_dim, int64_t max_q_len,
+                                                        int64_t prefix_len, int64_t cache_len,
+                                                        int32_t page_size, int64_t* bytes) {
+    if (!bytes) return set_error(SC_ERR_INVALID_ARGUMENT, "null pointer argument");
+    *bytes = 0;
+    const int64_t cap = batch ? cache_len : 0;
+    int32_t rc = check_sizes(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, prefix_len, cap);
+    if (rc != SC_OK) return rc;
+    if (cap && page_size <= 0) return set_error(SC_ERR_INVALID_ARGUMENT, "page_size %d", page_size);
+    if (n_tokens == 0 || q_heads == 0) return ok();
+    Split s;
+    rc = plan_split(static_cast<int32_t>(n_tokens), batch, q_heads, kv_heads, head_dim,
+                    static_cast<int32_t>(max_q_len), static_cast<int32_t>(prefix_len),
+                    static_cast<int32_t>(cap), page_size, &s);
+    if (rc != SC_OK) return rc;
+    *bytes = size_product(workspace_floats(s, n_tokens, q_heads, head_dim), 4);
+    return ok();
+}
+
+extern "C" int32_t sc_shared_prefix_attention(
+    int64_t n_tokens, int32_t batch, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+    int32_t dtype, const void* q, const int64_t* q_strides, int64_t prefix_len, const void* k_prefix,
+    const int64_t* kp_strides, const void* v_prefix, const int64_t* vp_strides, int64_t cache_len,
+    const void* k_cache, const int64_t* kc_strides, const void* v_cache, const int64_t* vc_strides,
+    const int32_t* cache_lens, const int32_t* page_table, int64_t page_table_stride, int32_t page_size,
+    int64_t n_pages, const int32_t* cu_q_lens, int64_t max_q_len, double scale, void* out,
+    const int64_t* out_strides, float* lse, void* workspace, int64_t workspace_bytes, int32_t* status,
+    void* stream) {
+    const int64_t cap = batch ? cache_len : 0;
+    int32_t rc = check_sizes(n_tokens, batch, q_heads, kv_heads, head_dim, max_q_len, prefix_len, cap);
+    if (rc != SC_OK) return rc;
+    if (dtype != SC_DTYPE_F16 && dtype != SC_DTYPE_BF16)
+        return set_error(SC_ERR_INVALID_DTYPE, "dtype code %d: float16 or bfloat16", dtype);
+    if (!isfinite(scale)) return set_error(SC_ERR_INVALID_ARGUMENT, "scale must be finite, got %g", scale);
+    if (n_tokens == 0 || q_heads == 0) return ok();
+    if (!cu_q_lens && batch && n_tokens != max_q_len * batch)
+        return set_error(SC_ERR_INVALID_ARGUMENT, "%lld tokens are not %d sequences of %lld",
+                         (long long)n_tokens, batch, (long long)max_q_len);
+    if (cap && page_size <= 0) return set_error(SC_ERR_INVALID_ARGUMENT, "page_size %d", page_size);
+    if (!q || !q_strides || !out || !out_strides || (prefix_len && (!k_prefix || !v_prefix ||
+        !kp_strides || !vp_strides)) || (cap && (!k_cache || !v_cache || !kc_strides || !vc_strides)) ||
+        (cu_q_lens && batch == 0))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "null pointer argument");
+    auto aligned = [&](const void* ptr, const int64_t* st, int n) {
+        bool ok = reinterpret_cast<uintptr_t>(ptr) % 16 == 0;
+        for (int i = 0; i < n; ++i) ok = ok && st[i] % 8 == 0;
+        return ok;
+    };
+    if (!aligned(q, q_strides, 2) || !aligned(out, out_strides, 2) ||
+        (prefix_len && (!aligned(k_prefix, kp_strides, 2) || !aligned(v_prefix, vp_strides, 2))) ||
+        (cap && (!aligned(k_cache, kc_strides, 3) || !aligned(v_cache, vc_strides, 3))))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "rows must start at multiples of 16 bytes");
+
+    Split s;
+    rc = plan_split(static_cast<int32_t>(n_tokens), batch, q_heads, kv_heads, head_dim,
+                    static_cast<int32_t>(max_q_len), static_cast<int32_t>(prefix_len),
+                    static_cast<int32_t>(cap), page_size, &s);
+    if (rc != SC_OK) return rc;
+    const int64_t need = size_product(workspace_floats(s, n_tokens, q_heads, head_dim), 4);
+    if (workspace_bytes < need || (need && !workspace) || reinterpret_cast<uintptr_t>(workspace) % 16)
+        return set_error(SC_ERR_INVALID_ARGUMENT, "workspace of %lld bytes (16-byte aligned) needed, got %lld",
+                         (long long)need, (long long)workspace_bytes);
+
+    AttnParams p{};
+    p.q = q, p.q_t = q_strides[0], p.q_h = q_strides[1];
+    p.kp = k_prefix, p.vp = v_prefix;
+    if (prefix_len)
+        p.kp_t = kp_strides[0], p.kp_h = kp_strides[1], p.vp_t = vp_strides[0], p.vp_h = vp_strides[1];
+    p.kc = k_cache, p.vc = v_cache;
+    if (cap) {
+        p.kc_b = kc_strides[0], p.kc_t = kc_strides[1], p.kc_h = kc_strides[2];
+        p.vc_b = vc_strides[0], p.vc_t = vc_strides[1], p.vc_h = vc_strides[2];
+    }
+    p.page_table = cap ? page_table : nullptr, p.pt_b = page_table_stride, p.n_pages = n_pages;
+    p.cache_lens = cache_lens, p.cu_q = cu_q_lens;
+    p.N = static_cast<int32_t>(n_tokens), p.B = batch, p.Hq = q_heads, p.Hkv = kv_heads;
+    p.G = q_heads / kv_heads, p.D = head_dim, p.nq = static_cast<int32_t>(max_q_len);
+    p.P = static_cast<int32_t>(prefix_len), p.cap = static_cast<int32_t>(cap);
+    p.page = page_size > 0 ? page_size : 1;
+    p.div_G = make_fastdiv(static_cast<uint32_t>(p.G));
+    p.div_page = make_fastdiv(static_cast<uint32_t>(p.page));
+    p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
+    p.n_pp = s.n_pp, p.n_cp = s.n_cp, p.chunk_p = s.chunk_p, p.tiles_p = s.tiles_p, p.tiles_c = s.tiles_c;
+    const int64_t rows = n_tokens * q_heads;
+    p.part_o = static_cast<float*>(workspace);
+    p.part_ml = reinterpret_cast<float2*>(p.part_o + (s.n_pp + s.n_cp) * rows * head_dim);
+    p.out = out, p.o_t = out_strides[0], p.o_h = out_strides[1];
+    p.lse = lse, p.status = status;
+
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const int64_t units = static_cast<int64_t>(s.n_pp) * s.tiles_p * kv_heads +
+                          static_cast<int64_t>(s.n_cp) * s.tiles_c * kv_heads * batch;
+    cudaError_t e = cudaSuccess;
+    if (units)
+        e = dtype == SC_DTYPE_F16 ? launch_rows_dp<__half>(p, s.v, units, st)
+                                  : launch_rows_dp<__nv_bfloat16>(p, s.v, units, st);
+    if (e != cudaSuccess) return cuda_error(e, "attention launch");
+    const unsigned blocks = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
+    if (dtype == SC_DTYPE_F16)
+        join_parts<__half><<<blocks, kThreads, 0, st>>>(p);
+    else
+        join_parts<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_error(e, "attention join launch");
+    return ok();
+}

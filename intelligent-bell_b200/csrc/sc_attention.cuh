@@ -1,0 +1,146 @@
+// sc_attention.cuh — shared by the attention kernels: what a call holds, and the warp-level
+// matrix, copy and exponential instructions they use.
+#pragma once
+
+#include "sc_common.cuh"
+
+namespace sc {
+
+// One call of the shared-prefix attention.  Tokens of q are packed over the sequences; rows of
+// one KV head are (token, head of its group) pairs, token-major.  Strides count elements.
+struct AttnParams {
+    const void* q;
+    int64_t q_t, q_h;
+    const void* kp;  // prefix keys and values [P, Hkv, D]
+    const void* vp;
+    int64_t kp_t, kp_h, vp_t, vp_h;
+    const void* kc;  // own caches [B, cap, Hkv, D], or a pool [n_pages, page, Hkv, D]
+    const void* vc;
+    int64_t kc_b, kc_t, kc_h, vc_b, vc_t, vc_h;
+    const int32_t* page_table;  // null: dense caches
+    int64_t pt_b;
+    int64_t n_pages;
+    const int32_t* cache_lens;  // null: every cache is full
+    const int32_t* cu_q;        // [B + 1] first token of each sequence; null: nq each
+    int32_t N, B, Hq, Hkv, G, D;
+    int32_t nq;       // tokens a sequence, at most
+    int32_t P, cap;   // prefix tokens; own cache tokens a sequence, at most
+    int32_t page;     // tokens a page (dense: cap)
+    FastDiv div_G, div_page;
+    float scale_log2;  // scale * log2(e)
+    int32_t n_pp, n_cp;  // parts of the prefix and of each own cache
+    int32_t chunk_p;     // prefix tokens a part
+    int32_t tiles_p, tiles_c;  // row tiles of the prefix, and at most of a sequence
+    float* part_o;   // [n_pp + n_cp][N * Hq][D], not normalised
+    float2* part_ml; // [n_pp + n_cp][N * Hq]: row maximum (log2 units) and sum
+    void* out;
+    int64_t o_t, o_h;
+    float* lse;  // [N, Hq], or null
+    int32_t* status;
+};
+
+constexpr float kNegInf = -__builtin_huge_valf();
+
+// Tokens of sequence b: its first one and how many.  Device-given starts are bounded by N.
+__device__ __forceinline__ void sequence_tokens(const AttnParams& p, int b, int& tok0, int& n) {
+    if (p.cu_q == nullptr) {
+        tok0 = b * p.nq;
+        n = p.nq;
+        return;
+    }
+    const int a = p.cu_q[b], e = p.cu_q[b + 1];
+    if (a < 0 || e < a || e > p.N || e - a > p.nq) {
+        if (threadIdx.x == 0 && p.status) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
+        tok0 = 0;
+        n = 0;
+        return;
+    }
+    tok0 = a;
+    n = e - a;
+}
+
+// Tokens that belong to sequences (rows behind the last one are left alone).
+__device__ __forceinline__ int used_tokens(const AttnParams& p) {
+    if (p.cu_q == nullptr) return p.N;
+    const int e = p.cu_q[p.B];
+    return e < 0 ? 0 : min(e, p.N);
+}
+
+__device__ __forceinline__ int cache_length(const AttnParams& p, int b) {
+    if (p.cache_lens == nullptr) return p.cap;
+    const int len = p.cache_lens[b];
+    if (len < 0 || len > p.cap) {
+        if (threadIdx.x == 0 && p.status) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
+        return 0;
+    }
+    return len;
+}
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+
+// 16 bytes global -> shared; zeros instead when !valid (the source is then not read).
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n)
+                 : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+
+// c[16 x 8] += a[16 x 16] b[16 x 8], fp32 accumulation.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (std::is_same<T, __half>::value) {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    } else {
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
+            "{%8,%9}, {%0,%1,%2,%3};"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+}
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(bit_cast_u32<__half2>(w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+}  // namespace sc

@@ -112,5 +112,9 @@ cudaError_t preload_paged_kernels();
 cudaError_t preload_quantize_kernels(bool f32_scales);  // fp16-scale kernels, + fp32 if asked
 cudaError_t preload_dense_kernels();
 cudaError_t preload_shift_kernels();
+cudaError_t preload_rotary_kernels();
+cudaError_t preload_attention_kernels();
+cudaError_t preload_weights_kernels();
+cudaError_t preload_evict_kernels();
 
 }  // namespace sc

@@ -6,6 +6,8 @@ Every name here runs the CUDA library and there is no CPU path: the reference's 
 the arithmetic of the function they replace (fp16 or fp32 intermediate of ``q*s``).
 """
 
+from .attention import accumulate_attention_weights, shared_prefix_attention
+from .evict import Evicted, evict_tokens
 from .paged import paged_status, restore_paged
 from .quantize import quantize_kv_int8, quantize_symmetric_int8
 from .restore import (
@@ -22,6 +24,7 @@ from .restore import (
     restore_layers,
     triton_fused_k_dequant_rope_shift,
 )
+from .rotary import RopeScaling, apply_rotary, rotary_frequencies
 from .shift import rope_shift_keys
 from .validation import rotate_half, validate_key_inputs, validate_value_inputs
 
@@ -59,6 +62,10 @@ class _FusedKernelHandle:
 fused_k_dequant_rope_shift_kernel = _FusedKernelHandle()
 
 __all__ = [
+    "Evicted",
+    "RopeScaling",
+    "accumulate_attention_weights",
+    "apply_rotary",
     "compute_rope_cos_sin_delta",
     "dequant_and_rope_key",
     "dequant_and_rope_key_compiled",
@@ -67,6 +74,7 @@ __all__ = [
     "dequant_value",
     "dequant_value_compiled",
     "dequant_value_ref",
+    "evict_tokens",
     "fused_k_dequant_rope_shift_kernel",
     "paged_status",
     "pytorch_compiled_dequant_rope_shift",
@@ -76,7 +84,9 @@ __all__ = [
     "restore_layers",
     "restore_paged",
     "rope_shift_keys",
+    "rotary_frequencies",
     "rotate_half",
+    "shared_prefix_attention",
     "triton_fused_k_dequant_rope_shift",
     "validate_key_inputs",
     "validate_value_inputs",

@@ -1,0 +1,239 @@
+"""Rotary positions of new queries and keys.
+
+The restore path turns cached keys by a relative shift (:func:`rope_shift_keys` and the fused
+restore); this module turns a step's own queries and keys by their absolute positions before
+the keys join the cache, in one launch of ``sc_rope_apply`` for both.  The half layout (the
+pairing of the restore path) and the interleaved one, a rotary part smaller than the head, and
+the usual ways to scale the frequencies for contexts longer than the trained ones.
+"""
+
+from __future__ import annotations
+
+import math
+from dataclasses import dataclass
+
+import numpy as np
+import torch
+
+from .. import _lib
+from .restore import DEFAULT_THETA
+from .staging import step_arguments
+from .validation import require_apart, require_cuda, require_no_grad, same_view
+
+_DTYPES = (torch.float16, torch.bfloat16, torch.float32)
+_KINDS = ("linear", "ntk", "bands", "yarn")
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the rotary frequencies ``f_i = theta^(-2i/R)`` are scaled for long contexts.
+
+    ``kind``:
+
+    * ``"linear"``: every frequency divided by ``factor`` (position interpolation);
+    * ``"ntk"``: ``theta`` multiplied by ``factor^(R / (R - 2))``, which slows the lowest
+      frequency by ``factor`` and leaves the highest;
+    * ``"bands"``: by the turns a frequency makes over ``original_length`` positions: divided by
+      ``factor`` below ``low_freq_factor`` turns, kept above ``high_freq_factor``, a linear
+      blend between;
+    * ``"yarn"``: divided by ``factor`` or kept by a linear ramp over the frequency's index,
+      between the (rounded out) indices that make ``beta_fast`` and ``beta_slow`` turns over
+      ``original_length`` positions; cosines and sines are multiplied by
+      ``0.1 ln(factor) + 1``.
+
+    ``attention_factor`` replaces the factor of the cosines and sines (1 but for ``"yarn"``).
+    """
+
+    kind: str
+    factor: float
+    original_length: int = 0
+    low_freq_factor: float = 1.0
+    high_freq_factor: float = 4.0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attention_factor: float | None = None
+
+    def __post_init__(self) -> None:
+        if self.kind not in _KINDS:
+            raise ValueError(f"scaling kind must be one of {_KINDS}, got {self.kind!r}")
+        if not (math.isfinite(self.factor) and self.factor > 0):
+            raise ValueError(f"factor must be positive and finite, got {self.factor}")
+        if self.kind in ("bands", "yarn") and self.original_length <= 0:
+            raise ValueError(f"{self.kind!r} scaling needs original_length")
+        if self.kind == "bands" and not self.high_freq_factor > self.low_freq_factor:
+            raise ValueError("high_freq_factor must be above low_freq_factor")
+        if self.kind == "yarn" and not self.beta_fast > self.beta_slow > 0:
+            raise ValueError("beta_fast must be above beta_slow, both positive")
+        if self.attention_factor is not None and not (
+                math.isfinite(self.attention_factor) and self.attention_factor > 0):
+            raise ValueError(f"attention_factor must be positive and finite, got {self.attention_factor}")
+
+
+def rotary_frequencies(rotary_dim: int, theta: float = DEFAULT_THETA,
+                       scaling: RopeScaling | None = None) -> tuple[np.ndarray, float]:
+    """float64 ``[rotary_dim / 2]`` frequencies in radians per position, and the factor of the
+    cosines and sines."""
+    if rotary_dim < 0 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be even, got {rotary_dim}")
+    if not (math.isfinite(theta) and theta > 0):
+        raise ValueError(f"theta must be positive and finite, got {theta}")
+    theta = float(theta)
+    i = np.arange(rotary_dim // 2, dtype=np.float64)
+    s = scaling
+    if s is not None and s.kind == "ntk" and rotary_dim > 2:
+        theta *= s.factor ** (rotary_dim / (rotary_dim - 2))
+    f = theta ** (-2.0 * i / rotary_dim) if rotary_dim else i
+    mult = 1.0
+    if s is not None:
+        if s.kind == "linear":
+            f = f / s.factor
+        elif s.kind == "bands":
+            turns = s.original_length * f / (2 * math.pi)
+            keep = np.clip((turns - s.low_freq_factor) / (s.high_freq_factor - s.low_freq_factor), 0.0, 1.0)
+            f = (1.0 - keep) * (f / s.factor) + keep * f
+        elif s.kind == "yarn":
+            if theta <= 1.0:
+                raise ValueError(f"yarn scaling needs theta above 1, got {theta}")
+
+            def index(turns: float) -> float:
+                return rotary_dim * math.log(s.original_length / (turns * 2 * math.pi)) / (2 * math.log(theta))
+
+            lo = max(math.floor(index(s.beta_fast)), 0)
+            hi = min(math.ceil(index(s.beta_slow)), rotary_dim - 1)
+            slow = np.clip((i - lo) / max(hi - lo, 0.001), 0.0, 1.0)
+            f = slow * (f / s.factor) + (1.0 - slow) * f
+            mult = 0.1 * math.log(s.factor) + 1.0 if s.factor > 1 else 1.0
+        if s.attention_factor is not None:
+            mult = s.attention_factor
+    return np.ascontiguousarray(f), mult
+
+
+_FREQUENCIES: dict[tuple, tuple[np.ndarray, int, float]] = {}
+
+
+def _frequencies(rotary_dim: int, theta: float, scaling: RopeScaling | None):
+    """(table, its address, factor), one table per (rotary_dim, theta, scaling)."""
+    key = (rotary_dim, theta, scaling)
+    hit = _FREQUENCIES.get(key)
+    if hit is None:
+        f, mult = rotary_frequencies(rotary_dim, theta, scaling)
+        hit = _FREQUENCIES[key] = (f, f.ctypes.data, mult)
+    return hit
+
+
+def _layout(name: str, x: torch.Tensor) -> tuple[int, int, int, int, tuple[int, int, int, int]]:
+    """(batch, tokens, heads, head_dim, strides in that order) of a 3-D or 4-D tensor."""
+    if x.ndim == 3:
+        s = x.stride()
+        return 1, x.shape[0], x.shape[1], x.shape[2], (0, s[0], s[1], s[2])
+    if x.ndim == 4:
+        s = x.stride()
+        return x.shape[0], x.shape[2], x.shape[1], x.shape[3], (s[0], s[2], s[1], s[3])
+    raise ValueError(f"{name} must be [T, H, D] or [B, H, T, D], got {tuple(x.shape)}")
+
+
+def apply_rotary(
+    q: torch.Tensor,
+    k: torch.Tensor | None,
+    positions,
+    *,
+    theta: float = DEFAULT_THETA,
+    rotary_dim: int | None = None,
+    interleaved: bool = False,
+    scaling: RopeScaling | None = None,
+    inverse: bool = False,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+):
+    """Turn queries and keys by their positions.
+
+    Args:
+        q: float16, bfloat16 or float32 ``[T, Hq, D]``, or ``[B, Hq, T, D]`` in the model layout.
+        k: keys of the same layout and dtype with their own head count, or None.
+        positions: integers ``[T]`` (or ``[B, T]`` with the model layout) on the device or the
+            host, or one int: the first token's position, the others follow it.
+        rotary_dim: how many leading elements of a head are turned (default: all).
+        interleaved: pairs are neighbours (2i, 2i + 1) instead of (i, i + rotary_dim / 2).
+        scaling: a :class:`RopeScaling`; None: unscaled.
+        inverse: undo the rotation (and the scaling's factor) instead.
+        q_out, k_out: outputs of the inputs' shape and dtype, any strides (a cache's next slots,
+            or the input itself); new contiguous tensors by default.
+
+    Angles are kept to 2^-33 of a turn at any position below 2^31; products are in float32 and
+    rounded once.  Returns ``q_out``, or ``(q_out, k_out)`` when keys are given.
+    """
+    require_cuda(q)
+    if q.dtype not in _DTYPES:
+        raise TypeError(f"q must be float16, bfloat16 or float32, got {q.dtype}")
+    require_no_grad("apply_rotary", q, k, q_out, k_out)
+    dev = q.device
+    b, t, hq, d, qs = _layout("q", q)
+    hk, ks = 0, None
+    if k is not None:
+        kb, kt, hk, kd, ks = _layout("k", k)
+        if (kb, kt, kd, k.ndim) != (b, t, d, q.ndim):
+            raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+        if k.dtype != q.dtype:
+            raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
+        if k.device != dev:
+            raise ValueError(f"k is on {k.device}, q on {dev}")
+    elif k_out is not None:
+        raise ValueError("k_out given without k")
+    rd = d if rotary_dim is None else int(rotary_dim)
+    if rd < 0 or rd % 2 or rd > d:
+        raise ValueError(f"rotary_dim must be even and at most head_dim {d}, got {rd}")
+    outs = []
+    for name, x, out, other in (("q_out", q, q_out, k), ("k_out", k, k_out, q)):
+        if x is None:
+            outs.append(None)
+            continue
+        if out is None:
+            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+        else:
+            if out.shape != x.shape or out.device != dev:
+                raise ValueError(f"{name} must have shape {tuple(x.shape)} on {dev}, "
+                                 f"got {tuple(out.shape)} on {out.device}")
+            if out.dtype != x.dtype:
+                raise TypeError(f"{name} must be {x.dtype}, got {out.dtype}")
+            if same_view(out, x):
+                require_apart(name, out)
+            else:
+                require_apart(name, out, x, other)
+        outs.append(out)
+    qo, ko = outs
+    if q_out is not None and k_out is not None and not (same_view(qo, q) and same_view(ko, k)):
+        require_apart("k_out", ko, qo)
+
+    start, pos_ptr, pos64, ps = 0, None, 0, (0, 0)
+    if isinstance(positions, int):
+        start = positions
+    else:
+        if not isinstance(positions, torch.Tensor):
+            positions = torch.as_tensor(positions)
+        if positions.dtype not in (torch.int32, torch.int64):
+            raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
+        if positions.shape != (t,) and positions.shape != (b, t):
+            raise ValueError(f"positions must be [{t}] or [{b}, {t}], got {tuple(positions.shape)}")
+        if positions.device != dev:
+            (positions,) = step_arguments("apply_rotary", [positions.contiguous()], dev)
+        pos64 = 1 if positions.dtype == torch.int64 else 0
+        s = positions.stride()
+        ps = (0, s[0]) if len(s) == 1 else (s[0], s[1])
+        pos_ptr = positions.data_ptr()
+    if b * t == 0 or d == 0:
+        return qo if k is None else (qo, ko)
+    _, freq_ptr, mult = _frequencies(rd, float(theta), scaling)
+    _, _, _, _, qos = _layout("q_out", qo)
+    kos = _layout("k_out", ko)[4] if ko is not None else None
+    lib = _lib.load()
+    st = _lib.stride_buffer()
+    with _lib.on_device(dev):
+        rc = lib.sc_rope_apply(
+            b, t, hq, hk, d, rd, 1 if interleaved else 0,
+            q.data_ptr(), st.put(qs), _lib.ptr(k), st.put(ks) if ks else None,
+            _lib.DTYPE_CODE[q.dtype], pos_ptr, pos64, st.put(ps), start,
+            freq_ptr, mult, 1 if inverse else 0,
+            qo.data_ptr(), st.put(qos), _lib.ptr(ko), st.put(kos) if kos else None,
+            _lib.stream_handle(dev))
+    _lib.check(rc, "apply_rotary")
+    return qo if k is None else (qo, ko)

@@ -55,3 +55,15 @@ def to_device(tensors: list[torch.Tensor], device: torch.device) -> list[torch.T
         out[i] = dev_buf[off:off + n].view(t.dtype).view(t.shape)
         off += span
     return out
+
+
+def step_arguments(what: str, tensors: list[torch.Tensor], device: torch.device) -> list[torch.Tensor]:
+    """:func:`to_device` for the operators of a model step, which may be captured into a graph.
+
+    A captured copy would read the staging buffer again at every replay, after it has gone to
+    another call; host arguments are refused there.
+    """
+    if torch.cuda.is_current_stream_capturing() and any(t.device != device for t in tensors):
+        raise RuntimeError(f"{what}: host arguments cannot be captured into a CUDA graph; "
+                           f"pass tensors on {device}")
+    return to_device(tensors, device)

@@ -107,3 +107,40 @@ def rotate_half(x: torch.Tensor) -> torch.Tensor:
     """
     d_half = x.shape[-1] // 2
     return torch.cat((-x[..., d_half:], x[..., :d_half]), dim=-1)
+
+
+def require_no_grad(what: str, *tensors: torch.Tensor | None) -> None:
+    """The operators of this package compute no gradients; say so instead of dropping them."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() "
+                                   "or on detached tensors")
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    """Half-open byte range that ``t`` reaches."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    lo = t.data_ptr()
+    return lo, lo + (last + 1) * t.element_size()
+
+
+def require_apart(name: str, out: torch.Tensor, *others: torch.Tensor | None) -> None:
+    """``out`` names each of its elements once and reaches into none of ``others``."""
+    for n, s in zip(out.shape, out.stride()):
+        if s == 0 and n > 1:
+            raise ValueError(f"{name} must not be an expanded tensor (strides {tuple(out.stride())})")
+    lo, hi = _extent(out)
+    for t in others:
+        if t is None or t.device != out.device:
+            continue
+        a, b = _extent(t)
+        if lo < b and a < hi:
+            raise ValueError(f"{name} must not overlap an input or another output")
+
+
+def same_view(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors of one shape are the same elements in the same order."""
+    return a.data_ptr() == b.data_ptr() and a.stride() == b.stride() and a.dtype == b.dtype
