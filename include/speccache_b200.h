@@ -77,6 +77,7 @@ typedef enum sc_dtype {
 #define SC_STATUS_BAD_PAGE_ID 0x1    /* page-table entry outside [0, n_pool_pages)          */
 #define SC_STATUS_BAD_SEQ_LEN 0x2    /* seq_len < 0 or > max_pages * page_size              */
 #define SC_STATUS_BAD_OUT_OFFSET 0x4 /* offset not a multiple of 16 or rows beyond out_numel */
+#define SC_STATUS_WAIT_LIMIT 0x8     /* a bounded wait inside an attention kernel ran out     */
 
 /* Message for the last failing call on this host thread ("" if none). */
 SC_API const char* sc_last_error(void);

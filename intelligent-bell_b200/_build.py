@@ -12,6 +12,8 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 REPO_DIR = os.path.dirname(PKG_DIR)
@@ -53,7 +55,7 @@ def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool =
     target = out_path or LIB_PATH
     if out_path is None and not force and not _stale():
         return LIB_PATH
-    cmd = [
+    flags = [
         _nvcc(),
         "-O3",
         "-std=c++17",
@@ -61,22 +63,27 @@ def build_library(force: bool = False, verbose: bool = False, ptxas_info: bool =
         "-lineinfo",
         "-Xcompiler",
         "-fPIC,-O3,-fvisibility=hidden",
-        "-shared",
         f"-I{INCLUDE}",
         *[f"-D{k}={v}" for k, v in (defines or {}).items()],
-        "-o",
-        target + ".tmp",
-        *sources(),
     ]
-    if ptxas_info:
-        cmd.insert(1, "-Xptxas=-v")
-    if verbose:
-        print(" ".join(cmd), file=sys.stderr)
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr}")
-    if verbose or ptxas_info:
-        print(proc.stderr, file=sys.stderr)
+
+    def run(cmd: list[str]) -> None:
+        if verbose:
+            print(" ".join(cmd), file=sys.stderr)
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"nvcc failed ({proc.returncode}):\n{proc.stderr}")
+        if verbose or ptxas_info:
+            print(proc.stderr, file=sys.stderr)
+
+    # One compiler per source, side by side, then one link.
+    with tempfile.TemporaryDirectory() as tmp:
+        objects = [os.path.join(tmp, os.path.basename(src) + ".o") for src in sources()]
+        compile_flags = flags + (["-Xptxas=-v"] if ptxas_info else [])
+        with ThreadPoolExecutor(max_workers=os.cpu_count()) as pool:
+            list(pool.map(lambda so: run([*compile_flags, "-c", so[0], "-o", so[1]]),
+                          zip(sources(), objects)))
+        run([*flags, "-shared", "-o", target + ".tmp", *objects])
     os.replace(target + ".tmp", target)
     return target
 

@@ -37,6 +37,7 @@ SC_FLAG_FORCE_GENERIC = 0x2
 SC_STATUS_BAD_PAGE_ID = 0x1
 SC_STATUS_BAD_SEQ_LEN = 0x2
 SC_STATUS_BAD_OUT_OFFSET = 0x4
+SC_STATUS_WAIT_LIMIT = 0x8
 
 SC_PIPE_NUMA_LOCAL = 0x1
 SC_PIPE_WRITE_COMBINED = 0x2

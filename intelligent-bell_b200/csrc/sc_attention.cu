@@ -473,43 +473,88 @@ cudaError_t preload_attention_type() {
     return e;
 }
 
-// How the tokens are split.  Two blocks fit an SM; four rounds of equal parts keep the last
-// round's idle share small without making the parts' join expensive.
+// How the rows and tokens are split over kernels and parts.
 struct Split {
-    int32_t tiles_p, tiles_c, chunk_p, n_pp, n_cp;
     Variant v;
+    bool tile_p;   // the prefix by attend_tiles
+    bool fused;    // prefix and own caches together by attend_tiles, a sequence's rows at a time
+    bool direct;   // one part, written as the output
+    int32_t tiles_p, tiles_c;  // row tiles (of the kernel that takes them)
+    int32_t chunk_p, n_pp, n_cp;
+    int64_t units_tile, units_rows;
 };
+
+constexpr int kTileRows = 256, kTileTokens = 128;
+constexpr int kMinTileRows = 64;   // fewer rows: the copies bound both kernels
+constexpr int kMinFusedRows = 96;  // fewer rows a sequence: packing the batch's rows wins
+
+// Parts of the token axis for attend_tiles: the number that ends soonest, in units of one step
+// (256 rows x 128 tokens, about 1.3 us), counting whole waves of 148 blocks, a block's start and
+// end (2.5 steps), and the parts' way through memory.
+int32_t plan_parts(double blocks, int64_t steps, double rows, int32_t D) {
+    int32_t best = 1;
+    double best_cost = 0.;
+    for (int32_t n = 1; n <= 64 && (n == 1 || n * 2 <= steps); ++n) {
+        const double waves = ceil(blocks * n / 148.0);
+        double cost = waves * (static_cast<double>((steps + n - 1) / n) + 2.5) * 1.3;
+        if (n > 1) cost += 2.0 + n * rows * D * 8.0 / 5e6;
+        if (n == 1 || cost < best_cost) best = n, best_cost = cost;
+    }
+    return best;
+}
 
 int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t nq, int32_t P,
                    int32_t cap, int32_t page, Split* out) {
     const int64_t G = Hq / Hkv;
     const int64_t rows_p = N * G, rows_c = cap ? nq * G : 0;
     Split s{};
-    s.v = pick_variant(D, rows_p > rows_c ? rows_p : rows_c);
-    const int64_t mr = 16 * s.v.mt;
-    s.tiles_p = static_cast<int32_t>((rows_p + mr - 1) / mr);
-    s.tiles_c = static_cast<int32_t>((rows_c + mr - 1) / mr);
-    const double work = static_cast<double>(P) * Hkv * s.tiles_p +
-                        static_cast<double>(cap) * Hkv * B * s.tiles_c;
-    double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
-    const double longest = P > cap ? P : cap;
-    const double most_parts = 64;
-    if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;
-    if (chunk < kPartTokens) chunk = kPartTokens;
-    s.chunk_p = static_cast<int32_t>(chunk > 0x40000000 ? 0x40000000 : chunk);
-    s.n_pp = P ? (P - 1) / s.chunk_p + 1 : 0;
-    s.n_cp = cap ? (cap - 1) / s.chunk_p + 1 : 0;
-    // A part's page ids are held in shared memory.
-    if (cap && page < cap) {
-        const int64_t room = static_cast<int64_t>(kMaxPagesPerPart - 1) * page / kPartTokens * kPartTokens;
-        const int64_t blocks = (static_cast<int64_t>(cap) + kPartTokens - 1) / kPartTokens;
-        const int64_t need = (blocks * kPartTokens + room - 1) / room;
-        if (need > s.n_cp) s.n_cp = static_cast<int32_t>(need);
+    s.fused = D <= 128 && cap && rows_c >= kMinFusedRows;
+    s.tile_p = !s.fused && D <= 128 && P && rows_p >= kMinTileRows;
+    const double rows = static_cast<double>(N) * Hq;
+    if (s.fused) {
+        s.tiles_c = static_cast<int32_t>((rows_c + kTileRows - 1) / kTileRows);
+        const double most = static_cast<double>(rows_p) / kTileRows + B;  // ragged: fewer than B * tiles_c
+        const double all = static_cast<double>(B) * s.tiles_c;
+        const int64_t steps = (P + kTileTokens - 1) / kTileTokens + (cap + kTileTokens - 1) / kTileTokens;
+        s.n_pp = plan_parts((most < all ? most : all) * Hkv, steps, rows, D);
+        s.direct = s.n_pp == 1;
+        s.units_tile = size_product(size_product(s.n_pp, s.tiles_c, Hkv), B);
+    } else {
+        if (s.tile_p) {
+            s.tiles_p = static_cast<int32_t>((rows_p + kTileRows - 1) / kTileRows);
+            s.n_pp = plan_parts(static_cast<double>(s.tiles_p) * Hkv, (P + kTileTokens - 1) / kTileTokens,
+                                rows, D);
+            s.direct = s.n_pp == 1 && !cap;
+            s.units_tile = size_product(s.n_pp, s.tiles_p, Hkv);
+        }
+        // attend_rows: two blocks fit an SM; two rounds of equal parts.
+        s.v = pick_variant(D, s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c);
+        const int64_t mr = 16 * s.v.mt;
+        const int32_t P_rows = s.tile_p ? 0 : P;
+        if (!s.tile_p) s.tiles_p = static_cast<int32_t>((rows_p + mr - 1) / mr);
+        s.tiles_c = static_cast<int32_t>((rows_c + mr - 1) / mr);
+        const double work = static_cast<double>(P_rows) * Hkv * s.tiles_p +
+                            static_cast<double>(cap) * Hkv * B * s.tiles_c;
+        double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
+        const double longest = P_rows > cap ? P_rows : cap;
+        const double most_parts = 64;
+        if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;
+        if (chunk < kPartTokens) chunk = kPartTokens;
+        s.chunk_p = static_cast<int32_t>(chunk > 0x40000000 ? 0x40000000 : chunk);
+        if (!s.tile_p) s.n_pp = P ? (P - 1) / s.chunk_p + 1 : 0;
+        s.n_cp = cap ? (cap - 1) / s.chunk_p + 1 : 0;
+        // A part's page ids are held in shared memory.
+        if (cap && page < cap) {
+            const int64_t room = static_cast<int64_t>(kMaxPagesPerPart - 1) * page / kPartTokens * kPartTokens;
+            const int64_t blocks = (static_cast<int64_t>(cap) + kPartTokens - 1) / kPartTokens;
+            const int64_t need = (blocks * kPartTokens + room - 1) / room;
+            if (need > s.n_cp) s.n_cp = static_cast<int32_t>(need);
+        }
+        s.units_rows = (s.tile_p ? 0 : size_product(s.n_pp, s.tiles_p, Hkv)) +
+                       size_product(size_product(s.n_cp, s.tiles_c, Hkv), B);
     }
-    const int64_t units = static_cast<int64_t>(s.n_pp) * s.tiles_p * Hkv +
-                          size_product(size_product(s.n_cp, s.tiles_c, Hkv), B);
-    if (units >= (int64_t(1) << 31))
-        return set_error(SC_ERR_INVALID_ARGUMENT, "%lld blocks in one call; split it", (long long)units);
+    if (s.units_rows >= (int64_t(1) << 31) || s.units_tile >= (int64_t(1) << 31))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "too many blocks in one call; split it");
     *out = s;
     return SC_OK;
 }
@@ -529,7 +574,7 @@ int32_t check_sizes(int64_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, in
 }
 
 int64_t workspace_floats(const Split& s, int64_t N, int32_t Hq, int32_t D) {
-    return size_product(static_cast<int64_t>(s.n_pp) + s.n_cp, N * Hq, D + 2);
+    return s.direct ? 0 : size_product(static_cast<int64_t>(s.n_pp) + s.n_cp, N * Hq, D + 2);
 }
 
 }  // namespace
@@ -537,6 +582,7 @@ int64_t workspace_floats(const Split& s, int64_t N, int32_t Hq, int32_t D) {
 cudaError_t preload_attention_kernels() {
     cudaError_t e = preload_attention_type<__half>();
     if (e == cudaSuccess) e = preload_attention_type<__nv_bfloat16>();
+    if (e == cudaSuccess) e = preload_attention_tile_kernels();
     return e;
 }
 
@@ -636,15 +682,21 @@ extern "C" int32_t sc_shared_prefix_attention(
     p.lse = lse, p.status = status;
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const int64_t units = static_cast<int64_t>(s.n_pp) * s.tiles_p * kv_heads +
-                          static_cast<int64_t>(s.n_cp) * s.tiles_c * kv_heads * batch;
     cudaError_t e = cudaSuccess;
-    if (units)
-        e = dtype == SC_DTYPE_F16 ? launch_rows_dp<__half>(p, s.v, units, st)
-                                  : launch_rows_dp<__nv_bfloat16>(p, s.v, units, st);
-    if (e != cudaSuccess) return cuda_error(e, "attention launch");
+    const bool half = dtype == SC_DTYPE_F16;
+    if (s.units_tile) {
+        e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, s.direct,
+                                   s.units_tile, st);
+        if (e != cudaSuccess) return cuda_error(e, "attention tiles launch");
+    }
+    if (s.units_rows) {
+        e = half ? launch_rows_dp<__half>(p, s.v, s.units_rows, st)
+                 : launch_rows_dp<__nv_bfloat16>(p, s.v, s.units_rows, st);
+        if (e != cudaSuccess) return cuda_error(e, "attention launch");
+    }
+    if (s.direct) return ok();
     const unsigned blocks = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    if (dtype == SC_DTYPE_F16)
+    if (half)
         join_parts<__half><<<blocks, kThreads, 0, st>>>(p);
     else
         join_parts<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);

@@ -1,0 +1,606 @@
+// sc_attention_tile.cu — the shared-prefix attention for many rows of one KV head at once, on the
+// 5th-generation tensor cores.
+//
+// A block takes 256 rows (two tiles of 128 (token, head) rows of one KV head) against a run of
+// tokens in tiles of 128: prefix tokens, then tokens of the sequence's own cache.  Per tile pair,
+//   S = Q K^T         128 x 128 x D, fp32 accumulators in tensor memory,
+//   P = 2^(s - m)     one thread a row: no shuffles; written over S as 16 bits,
+//   O += P V          A operand from tensor memory, fp32 accumulators in tensor memory.
+// Two row tiles take turns: while the tensor cores work on one, eight warps turn the other's
+// scores into weights.  The running maximum that scales O is only raised when a score passes it
+// by 2^8, so O is rarely rescaled (weights up to 2^8 and their fp32 sums lose nothing).
+//
+// Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies (cp.async, any
+// strides, pages and odd ends; 16-byte chunks placed in the 128-byte swizzle that the matrix
+// descriptors name), warp 11 issues the products.  Tensor memory: S0, S1 (128 columns each), O0,
+// O1 (D columns each).  Every wait has a limit; a wait that runs out sets a status bit and the
+// block leaves.
+#include <math.h>
+
+#include "sc_attention.cuh"
+
+namespace sc {
+namespace {
+
+constexpr int kTThreads = 384;
+constexpr int kLoadWarps = 3;
+constexpr int kRowTile = 128;
+constexpr int kTokTile = 128;
+constexpr int kWaitLimit = 1 << 18;  // tries of at most about 2 us each
+constexpr float kRaise = 8.f;  // log2: how far a score may pass the maximum in use
+
+template <int DP>
+struct TileShape {
+    static constexpr int kTile = 128 * DP * 2;  // bytes of 128 rows
+    static constexpr int kStages = DP == 128 ? 5 : 8;
+    static constexpr int kSmem = (2 + kStages) * kTile + 1024;  // + alignment
+};
+
+struct TileParams {
+    AttnParams a;
+    int32_t per_seq;   // rows are those of one sequence, and its own cache follows the prefix
+    int32_t tiles;     // 256-row tiles, at most
+    int32_t splits;    // parts of the token axis
+    int32_t direct;    // one part: write the output itself
+};
+
+// ---- barriers ----
+__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+__device__ __forceinline__ void bar_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n"
+        " selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    for (int i = 0; i < kWaitLimit; ++i) {
+        if (bar_try(bar, parity)) return true;
+        if (*gave_up) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+
+// ---- tensor core and tensor memory ----
+__device__ __forceinline__ void tc_fence_before() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_fence_after() {
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+}
+__device__ __forceinline__ void tc_commit(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    const uint32_t acc = add;
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
+    const uint32_t acc = add;
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// 32 columns of the warp's 32 lanes.
+__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
+          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+}
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+        "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() {
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() {
+    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+
+// Shared-memory matrix descriptors of a 128-row tile stored as panels of 64 columns: 128-byte
+// rows, 8 rows a 1024-byte swizzle atom.  Rows as the M or N dimension, columns contracted: atoms
+// follow one another every 1024 bytes (stride offset).  Columns as the N dimension, rows
+// contracted: panels follow every 16 KiB (leading offset), groups of 8 rows every 1024 bytes.
+__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead, uint32_t stride) {
+    return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
+           (static_cast<uint64_t>(stride >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
+}
+
+// Byte offset of 16-byte chunk c (of a 128-row tile's row r).
+__device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
+    return static_cast<uint32_t>((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_constant__ TileParams tp) {
+    using Shape = TileShape<DP>;
+    constexpr int TILE = Shape::kTile, NST = Shape::kStages;
+    constexpr int CPR = DP / 8;
+    const AttnParams& p = tp.a;
+    extern __shared__ unsigned char smem_raw[];
+    __shared__ __align__(8) uint64_t s_bars[2 * NST + 8];
+    __shared__ uint32_t s_tmem;
+    __shared__ int s_gave_up;
+    __shared__ int s_any_bad;
+    __shared__ unsigned char s_ok[4][kTokTile];
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    int u = blockIdx.x;
+    const int split = u % tp.splits;
+    u /= tp.splits;
+    const int rt = u % tp.tiles;
+    u /= tp.tiles;
+    const int h = u % p.Hkv, b = u / p.Hkv;
+    int tok0 = 0, n_tok, len = 0;
+    if (tp.per_seq) {
+        sequence_tokens(p, b, tok0, n_tok);
+        len = p.cap ? cache_length(p, b) : 0;
+    } else {
+        n_tok = used_tokens(p);
+    }
+    const int rows = n_tok * p.G;
+    const int r0 = rt * 2 * kRowTile;
+    if (r0 >= rows) return;
+    const int n_rows = min(2 * kRowTile, rows - r0);
+    const int n_q = n_rows > kRowTile ? 2 : 1;
+
+    // Token tiles: the prefix's, then the own cache's that the last row sees.
+    const int see = len - n_tok;
+    const int vis = max(0, min(len, see + static_cast<int>(fdiv(r0 + n_rows - 1, p.div_G)) + 1));
+    const int tiles_p = (p.P + kTokTile - 1) / kTokTile;
+    const int tiles_all = tiles_p + (vis + kTokTile - 1) / kTokTile;
+    const int per = (tiles_all + tp.splits - 1) / tp.splits;
+    const int first = split * per;
+    const int n_tiles = max(0, min(per, tiles_all - first));
+    const int64_t part_row = static_cast<int64_t>(split) * p.N * p.Hq;
+
+    if (n_tiles == 0) {
+        if (tp.direct) {
+            for (int i = threadIdx.x; i < n_rows * (p.D / 8); i += kTThreads) {
+                const int r = i / (p.D / 8), c = i - r * (p.D / 8);
+                const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+                T* dst = static_cast<T*>(p.out) + (tok0 + j) * p.o_t +
+                         (h * p.G + r0 + r - j * p.G) * p.o_h + c * 8;
+                *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
+            }
+        }
+        for (int r = threadIdx.x; r < n_rows; r += kTThreads) {
+            const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+            const int64_t row = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
+            if (!tp.direct)
+                p.part_ml[part_row + row] = make_float2(kNegInf, 0.f);
+            else if (p.lse)
+                p.lse[row] = kNegInf;
+        }
+        return;
+    }
+
+    const uint32_t s_base = (smem_addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t s_q = s_base, s_ring = s_base + 2 * TILE;
+    const uint32_t bars = smem_addr(s_bars);
+    const uint32_t q_full = bars;
+    auto full = [&](int s) { return bars + 8u * (1 + s); };
+    auto empty = [&](int s) { return bars + 8u * (1 + NST + s); };
+    auto s_full = [&](int q) { return bars + 8u * (1 + 2 * NST + q); };
+    auto p_full = [&](int q) { return bars + 8u * (3 + 2 * NST + q); };
+    auto o_full = [&](int q) { return bars + 8u * (5 + 2 * NST + q); };
+    const uint32_t drained = bars + 8u * (7 + 2 * NST);
+    volatile int* gave_up = &s_gave_up;
+
+    if (threadIdx.x == 0) {
+        bar_init(q_full, kLoadWarps);
+        bar_init(drained, 1);
+        for (int s = 0; s < NST; ++s) {
+            bar_init(full(s), kLoadWarps);
+            bar_init(empty(s), 1);
+        }
+        for (int q = 0; q < 2; ++q) {
+            bar_init(s_full(q), 1);
+            bar_init(p_full(q), 4);
+            bar_init(o_full(q), 1);
+        }
+        s_gave_up = 0;
+        s_any_bad = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 11) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_addr(&s_tmem))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (p.D < DP) {  // columns that no copy writes
+        for (int i = threadIdx.x; i < (2 + NST) * TILE / 16; i += kTThreads)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s_base + 16u * i), "r"(0)
+                         : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = s_tmem;
+    constexpr uint32_t kO = 256;  // first column of O0
+
+    if (warp >= 8 && warp < 8 + kLoadWarps) {
+        // ---- copies ----
+        const int lw = warp - 8;
+        // Chunks of eight columns: a warp-wide copy covers 4 rows x 8 chunks of one panel.
+        const int sub = lane >> 3, c8 = lane & 7;
+        auto done = [&](uint32_t bar) {
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) bar_arrive(bar);
+        };
+        for (int q = 0; q < n_q; ++q)
+            for (int g = lw; g < 32; g += kLoadWarps) {
+                const int r = g * 4 + sub;
+                const int row = r0 + q * kRowTile + r;
+                const bool in = q * kRowTile + r < n_rows;
+                const int j = static_cast<int>(fdiv(in ? row : 0, p.div_G));
+                const T* src = static_cast<const T*>(p.q) + (tok0 + (in ? j : 0)) * p.q_t +
+                               (h * p.G + (in ? row - j * p.G : 0)) * p.q_h;
+#pragma unroll
+                for (int pn = 0; pn < CPR / 8; ++pn) {
+                    const int c = pn * 8 + c8;
+                    if (c * 8 < p.D) cp_async16(s_q + q * TILE + tile_chunk(r, c), src + c * 8, in);
+                }
+            }
+        cp_async_commit();
+        const bool paged = p.page_table != nullptr;
+        const int n_loads = 2 * n_tiles;
+        constexpr int LAG = 2;  // copies in flight behind the newest
+        bool alive = true;
+        for (int i = 0; i < n_loads + LAG; ++i) {
+            if (i < n_loads && alive) {
+                const int s = i % NST;
+                if (i >= NST) {
+                    alive = bar_wait(empty(s), ((i / NST) - 1) & 1, gave_up);
+                    alive = __all_sync(0xffffffffu, alive);
+                }
+                if (alive) {
+                    const int tile = first + (i >> 1);
+                    const bool is_v = i & 1;
+                    const bool pre = tile < tiles_p;
+                    const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
+                    const int t1 = pre ? p.P : vis;
+                    const uint32_t dst = s_ring + s * TILE;
+                    const T* base;
+                    int64_t st_t, st_b = 0;
+                    if (pre) {
+                        base = static_cast<const T*>(is_v ? p.vp : p.kp) + h * (is_v ? p.vp_h : p.kp_h);
+                        st_t = is_v ? p.vp_t : p.kp_t;
+                    } else {
+                        base = static_cast<const T*>(is_v ? p.vc : p.kc) + h * (is_v ? p.vc_h : p.kc_h);
+                        st_t = is_v ? p.vc_t : p.kc_t;
+                        st_b = is_v ? p.vc_b : p.kc_b;
+                        if (!paged) base += b * st_b;
+                    }
+#pragma unroll
+                    for (int gi = 0; gi < (32 + kLoadWarps - 1) / kLoadWarps; ++gi) {
+                        const int g = lw + gi * kLoadWarps;
+                        if (g < 32) {
+                            const int r = g * 4 + sub, t = t0 + r;
+                            bool in = t < t1;
+                            int64_t off = 0;
+                            if (in) {
+                                if (!pre && paged) {
+                                    const int pg = static_cast<int>(fdiv(t, p.div_page));
+                                    const int id = p.page_table[b * p.pt_b + pg];
+                                    in = id >= 0 && id < p.n_pages;
+                                    if (in) off = id * st_b + (t - pg * p.page) * st_t;
+                                    if (!is_v && c8 == 0) {
+                                        s_ok[(i >> 1) & 3][r] = in;
+                                        if (!in) {
+                                            s_any_bad = 1;
+                                            if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
+                                        }
+                                    }
+                                } else {
+                                    off = t * st_t;
+                                    if (!is_v && c8 == 0 && !pre) s_ok[(i >> 1) & 3][r] = 1;
+                                }
+                            }
+#pragma unroll
+                            for (int pn = 0; pn < CPR / 8; ++pn) {
+                                const int c = pn * 8 + c8;
+                                if (c * 8 < p.D)
+                                    cp_async16(dst + tile_chunk(r, c), base + off + c * 8, in);
+                            }
+                        }
+                    }
+                }
+            }
+            cp_async_commit();
+            if (i == 0) {
+                cp_async_wait<1>();
+                done(q_full);
+            }
+            if (i >= LAG) {
+                cp_async_wait<LAG>();
+                if (alive) done(full((i - LAG) % NST));
+            }
+        }
+        cp_async_wait<0>();
+    } else if (warp == 11) {
+        // ---- products ----
+        if (lane == 0) {
+            constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+            constexpr uint32_t id_common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
+            constexpr uint32_t id_qk = id_common | ((128u >> 3) << 17);
+            constexpr uint32_t id_pv = id_common | ((static_cast<uint32_t>(DP) >> 3) << 17) | (1u << 16);
+            auto qk = [&](int q, int stage) {
+                const uint32_t qa = s_q + q * TILE, ka = s_ring + stage * TILE;
+#pragma unroll
+                for (int kk = 0; kk < DP / 16; ++kk) {
+                    const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
+                    mma_ss(tmem + q * 128, desc(qa + off, 16, 1024), desc(ka + off, 16, 1024), id_qk, kk > 0);
+                }
+            };
+            auto pv = [&](int q, int stage, bool add) {
+                const uint32_t va = s_ring + stage * TILE;
+#pragma unroll
+                for (int kk = 0; kk < kTokTile / 16; ++kk)
+                    mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, desc(va + kk * 2048, 16384, 1024),
+                           id_pv, add || kk > 0);
+            };
+            bool alive = bar_wait(q_full, 0, gave_up) && bar_wait(full(0), 0, gave_up);
+            if (alive) {
+                for (int q = 0; q < n_q; ++q) {
+                    qk(q, 0);
+                    tc_commit(s_full(q));
+                }
+                tc_commit(empty(0));
+            }
+            for (int i = 0; i < n_tiles && alive; ++i) {
+                const int vl = 2 * i + 1, kl = 2 * i + 2;  // loads V_i, K_{i+1}
+                alive = bar_wait(full(vl % NST), (vl / NST) & 1, gave_up);
+                if (alive && i + 1 < n_tiles) alive = bar_wait(full(kl % NST), (kl / NST) & 1, gave_up);
+                for (int q = 0; q < n_q && alive; ++q) {
+                    alive = bar_wait(p_full(q), i & 1, gave_up);
+                    if (!alive) break;
+                    tc_fence_after();
+                    pv(q, vl % NST, i > 0);
+                    tc_commit(o_full(q));
+                    if (i + 1 < n_tiles) {
+                        // The weights that this product reads lie where the next scores go.
+                        alive = bar_wait(o_full(q), i & 1, gave_up);
+                        if (!alive) break;
+                        qk(q, kl % NST);
+                        tc_commit(s_full(q));
+                    }
+                }
+                if (alive) {
+                    tc_commit(empty(vl % NST));
+                    if (i + 1 < n_tiles) tc_commit(empty(kl % NST));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        // ---- softmax: one thread a row ----
+        const int q = warp >> 2;
+        const int r = q * kRowTile + (warp & 3) * 32 + lane;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        const uint32_t s_at = tmem + q * 128 + lanes, o_at = tmem + kO + q * DP + lanes;
+        const bool any = q * kRowTile + (warp & 3) * 32 < n_rows;  // a row of this warp counts
+        if (q < n_q) {
+            const int row = min(r0 + r, rows - 1);
+            const int j = static_cast<int>(fdiv(row, p.div_G));
+            const int own_limit = min(vis, see + j + 1);
+            float m = kNegInf, l = 0.f;  // m: the maximum in use
+            bool alive = true;
+            for (int i = 0; i < n_tiles; ++i) {
+                alive = bar_wait(s_full(q), i & 1, gave_up);
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+                tc_fence_after();
+                if (any) {
+                    const int tile = first + i;
+                    const bool pre = tile < tiles_p;
+                    const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
+                    const int seen = (pre ? p.P : own_limit) - t0;  // columns below it count
+                    uint32_t x[128];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, x + c * 32);
+                    tmem_wait_ld();
+                    const bool bad = !pre && *reinterpret_cast<volatile int*>(&s_any_bad) != 0;
+                    if (__any_sync(0xffffffffu, seen < kTokTile) || bad) {
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) {
+                            bool on = c < seen;
+                            if (bad && on) on = s_ok[i & 3][c] != 0;
+                            if (!on) x[c] = __float_as_uint(kNegInf);
+                        }
+                    }
+                    float top = kNegInf;
+                    const float sc = p.scale_log2;
+                    if (sc >= 0.f) {
+                        float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]));
+                        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * sc;
+                    }
+                    if (!(sc > 0.f)) {  // scaled first: a mask must stay minus infinity
+                        top = kNegInf;
+#pragma unroll
+                        for (int c = 0; c < 128; ++c) {
+                            const float v = __uint_as_float(x[c]);
+                            const float w = v == kNegInf ? kNegInf : v * sc;
+                            x[c] = __float_as_uint(w);
+                            top = fmaxf(top, w);
+                        }
+                    }
+                    const float mul = sc > 0.f ? sc : 1.f;
+                    if (__any_sync(0xffffffffu, top > m + kRaise || (m == kNegInf && top > m))) {
+                        const bool raise = top > m + kRaise || (m == kNegInf && top > m);
+                        const float f = raise ? exp2_fast(m - top) : 1.f;
+                        if (raise) m = top;
+                        l *= f;
+                        if (i > 0) {
+                            alive = bar_wait(o_full(q), (i - 1) & 1, gave_up);
+                            alive = __all_sync(0xffffffffu, alive);
+                            if (!alive) break;
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < DP / 32; ++c) {
+                                uint32_t o[32];
+                                tmem_ld32(o_at + c * 32, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                                tmem_st32(o_at + c * 32, o);
+                            }
+                        }
+                    }
+                    const float base = m == kNegInf ? 0.f : m;
+                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    uint32_t w[64];
+#pragma unroll
+                    for (int c = 0; c < 64; ++c) {
+                        const float e0 = exp2_fast(fmaf(__uint_as_float(x[2 * c]), mul, -base));
+                        const float e1 = exp2_fast(fmaf(__uint_as_float(x[2 * c + 1]), mul, -base));
+                        sum[(2 * c) & 3] += e0;
+                        sum[(2 * c + 1) & 3] += e1;
+                        w[c] = pack2<T>(e0, e1);  // 16-bit weights, as the product takes them
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_st32(s_at, w);
+                    tmem_st32(s_at + 32, w + 32);
+                    tmem_wait_st();
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) bar_arrive(p_full(q));
+            }
+            if (alive) {
+                alive = bar_wait(o_full(q), (n_tiles - 1) & 1, gave_up);
+                alive = __all_sync(0xffffffffu, alive);
+            }
+            if (alive && any) {
+                tc_fence_after();
+                const bool mine = r < n_rows;
+                const int64_t at = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + row - j * p.G;
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                T* dst = static_cast<T*>(p.out) + (tok0 + j) * p.o_t + (h * p.G + row - j * p.G) * p.o_h;
+                float* po = p.part_o + (part_row + at) * p.D;
+#pragma unroll
+                for (int c = 0; c < DP / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld32(o_at + c * 32, o);
+                    tmem_wait_ld();
+                    if (mine) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) {
+                            if (c * 32 + e >= p.D) continue;
+                            if (tp.direct) {
+                                uint32_t v[4];
+#pragma unroll
+                                for (int k = 0; k < 4; ++k)
+                                    v[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv,
+                                                    __uint_as_float(o[e + 2 * k + 1]) * inv);
+                                st_v4(dst + c * 32 + e, make_uint4(v[0], v[1], v[2], v[3]));
+                            } else {
+                                st_v4(po + c * 32 + e, make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
+                                st_v4(po + c * 32 + e + 4, make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]));
+                            }
+                        }
+                    }
+                }
+                if (mine) {
+                    if (!tp.direct)
+                        p.part_ml[part_row + at] = make_float2(m, l);
+                    else if (p.lse)
+                        p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const bool lost = s_gave_up != 0;
+    if (lost) {
+        // Products may still be running: let them end (again with a limit) before the memory goes.
+        __syncthreads();
+        if (threadIdx.x == 11 * 32) {
+            s_gave_up = 0;
+            tc_commit(drained);
+            bar_wait(drained, 0, gave_up);
+            if (p.status) atomicOr(p.status, SC_STATUS_WAIT_LIMIT);
+        }
+        __syncthreads();
+    }
+    if (warp == 11)
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+template <typename T, int DP>
+cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, cudaStream_t s, bool load_only) {
+    auto kernel = attend_tiles<T, DP>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         TileShape<DP>::kSmem);
+    if (e != cudaSuccess || load_only) return e;
+    kernel<<<units, kTThreads, TileShape<DP>::kSmem, s>>>(p);
+    return cudaGetLastError();
+}
+
+}  // namespace
+
+cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
+                                   bool direct, int64_t units, cudaStream_t s) {
+    TileParams p{};
+    p.a = a;
+    p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.direct = direct;
+    const unsigned n = static_cast<unsigned>(units);
+    if (a.D <= 64)
+        return half ? launch_tiles_dp<__half, 64>(p, n, s, false)
+                    : launch_tiles_dp<__nv_bfloat16, 64>(p, n, s, false);
+    return half ? launch_tiles_dp<__half, 128>(p, n, s, false)
+                : launch_tiles_dp<__nv_bfloat16, 128>(p, n, s, false);
+}
+
+cudaError_t preload_attention_tile_kernels() {
+    TileParams p{};
+    cudaError_t e = launch_tiles_dp<__half, 64>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 64>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__half, 128>(p, 0, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 128>(p, 0, nullptr, true);
+    return e;
+}
+
+}  // namespace sc

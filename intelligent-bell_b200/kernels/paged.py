@@ -35,7 +35,8 @@ def paged_status(device: torch.device | str | int | None = None, reset: bool = T
     """Read (and by default clear) the paged kernels' status bits on ``device``.
 
     Synchronises with the device's current stream.  Bits: SC_STATUS_BAD_PAGE_ID (1),
-    SC_STATUS_BAD_SEQ_LEN (2), SC_STATUS_BAD_OUT_OFFSET (4).
+    SC_STATUS_BAD_SEQ_LEN (2), SC_STATUS_BAD_OUT_OFFSET (4), SC_STATUS_WAIT_LIMIT (8, an
+    attention kernel gave up a wait: its outputs are undefined).
     """
     dev = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(
         device if not isinstance(device, int) else f"cuda:{device}")

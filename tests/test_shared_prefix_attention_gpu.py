@@ -100,6 +100,14 @@ SHAPES = [
     ([1, 1], [10, 10], 16, 1, 8, 20, 10, 0),
     ([17, 31], [60, 31], 12, 4, 128, None, 64, 0),  # no prefix
     ([1, 1, 1], [0, 0, 0], 4, 2, 64, 0, 5, 0),      # nothing to see at all
+    # many rows of a KV head: 256-row tiles
+    ([64, 3, 70], [64, 2, 300], 8, 2, 128, 257, 300, 0),
+    ([100, 1, 33], [90, 1, 40], 6, 2, 80, 129, 100, 24),
+    ([65], [65], 4, 1, 96, None, 80, 0),
+    ([128, 128], [128, 140], 2, 1, 64, 128, 140, 7),
+    ([257], [0], 1, 1, 128, 0, 4, 0),               # rows that see nothing
+    ([1] * 40, list(range(40)), 14, 2, 128, 700, 40, 8),
+    ([1] * 70, [3] * 70, 4, 4, 64, 300, 3, 0),
 ]
 
 
@@ -112,15 +120,16 @@ def test_matches_the_oracle(scb, ref, dtype, shape):
     assert scb.paged_status(DEV) == 0
 
 
-@pytest.mark.parametrize("n,hq,hk,d", [(1, 8, 8, 64), (5, 16, 2, 128), (90, 7, 1, 128)])
+@pytest.mark.parametrize("n,hq,hk,d", [(1, 8, 8, 64), (5, 16, 2, 128), (90, 7, 1, 128), (300, 2, 1, 64), (70, 2, 2, 40)])
 def test_prefix_alone(scb, ref, n, hq, hk, d):
     c = Case(12, torch.bfloat16, [n], [0], hq, hk, d, 333, None)
     c.check(ref, *c.run(scb))
 
 
-def test_scales(scb, ref):
+@pytest.mark.parametrize("n", [2, 60])
+def test_scales(scb, ref, n):
     for scale in (0.0, -0.2, 1.0):
-        c = Case(13, torch.float16, [2, 2], [9, 4], 4, 2, 64, 50, 9)
+        c = Case(13, torch.float16, [n, n], [n + 7, n + 2], 4, 2, 64, 50, n + 7)
         c.check(ref, *c.run(scb, scale=scale), scale=scale)
 
 
@@ -167,6 +176,14 @@ def test_nothing_is_read_behind_the_lengths(scb, ref, page, q_len):
     got = c.run(scb)
     assert bits_equal(got[0], want[0]) and bits_equal(got[1], want[1])
     c.check(ref, *got)
+
+
+def test_scores_that_grow_along_the_tokens(scb, ref):
+    """The running maximum is passed again and again, by little and by much."""
+    for n in (1, 50):
+        c = Case(28, torch.bfloat16, [n, n], [n + 30, n], 8, 2, 128, 900, n + 30)
+        c.kp.mul_(torch.linspace(0.1, 6, 900, device=DEV).to(torch.bfloat16)[:, None, None])
+        c.check(ref, *c.run(scb))
 
 
 def test_not_a_number_reaches_its_rows_alone(scb):
@@ -218,6 +235,13 @@ def test_bad_pages_and_lengths_are_reported(scb, ref):
     scb.shared_prefix_attention(c.q, c.kp, c.vp, c.kc, c.vc, c.lens_t(), page_table=c.table, cu_q_lens=cu,
                                 max_q_len=3)
     assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_SEQ_LEN
+    # many rows
+    c = Case(27, torch.float16, [50, 60], [200, 150], 4, 2, 64, 100, 200, 16)
+    c.table[0, 3] = -1
+    c.table[1, 9] = c.kc.shape[0]
+    out, lse = c.run(scb)
+    assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_PAGE_ID
+    c.check(ref, out, lse)
 
 
 def test_strided_queries_and_outputs(scb, ref):
@@ -236,7 +260,7 @@ def test_strided_queries_and_outputs(scb, ref):
 
 
 def test_repeatable_bit_for_bit_and_on_a_side_stream(scb):
-    c = Case(22, torch.bfloat16, [1] * 6, [500, 3, 77, 0, 260, 511], 32, 8, 128, 3000, 512)
+    c = Case(22, torch.bfloat16, [1] * 6, [500, 3, 77, 0, 260, 511], 32, 8, 128, 3001, 512)
     out, lse = c.run(scb)
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
