@@ -55,6 +55,17 @@ int sm_count() {
     return n;
 }
 
+cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 void default_inv_freq(int32_t head_dim, double theta, float* out) {
     for (int i = 0; i < head_dim / 2; ++i) {
         const float expo = (2.0f * static_cast<float>(i)) / static_cast<float>(head_dim);

@@ -443,7 +443,8 @@ cudaError_t launch_rows(const AttnParams& p, int64_t units, cudaStream_t s, bool
     constexpr int TK = 16, NST = DP == 64 ? 4 : 3;
     constexpr int bytes = RowsShape<DP, MT, TK, NST>::kSmem;
     auto kernel = attend_rows<T, DP, MT, TK, NST>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), bytes, done);
     if (e != cudaSuccess || load_only) return e;
     kernel<<<static_cast<unsigned>(units), kThreads, bytes, s>>>(p);
     return cudaGetLastError();

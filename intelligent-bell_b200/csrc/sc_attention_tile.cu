@@ -572,8 +572,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
 template <typename T, int DP>
 cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, cudaStream_t s, bool load_only) {
     auto kernel = attend_tiles<T, DP>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         TileShape<DP>::kSmem);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), TileShape<DP>::kSmem, done);
     if (e != cudaSuccess || load_only) return e;
     kernel<<<units, kTThreads, TileShape<DP>::kSmem, s>>>(p);
     return cudaGetLastError();

@@ -315,11 +315,15 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_in_place(const __grid_
     }
 }
 
+cudaError_t allow_select() {
+    static std::atomic<uint64_t> done{0};
+    return allow_shared_memory(reinterpret_cast<const void*>(select_tokens), kMaxSegment * 4, done);
+}
+
 }  // namespace
 
 cudaError_t preload_evict_kernels() {
-    cudaError_t e = cudaFuncSetAttribute(select_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMaxSegment * 4);
+    cudaError_t e = allow_select();
     cudaFuncAttributes attr;
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, move_rows);
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, move_rows_in_place);
@@ -394,8 +398,7 @@ extern "C" int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache
                                    (rows * ranks * 2 <= 148 && cache_len > static_cast<int64_t>(ranks) * 4096)))
         ranks *= 2;
     sp.segment = static_cast<int32_t>(((cache_len + ranks - 1) / ranks + 31) / 32 * 32);
-    cudaError_t e = cudaFuncSetAttribute(select_tokens, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kMaxSegment * 4);
+    cudaError_t e = allow_select();
     if (e != cudaSuccess) return cuda_error(e, "eviction set-up");
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));

@@ -4,6 +4,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "speccache_b200.h"
 
 namespace sc {
@@ -20,6 +22,10 @@ int32_t ok();
 
 // Map a CUDA error to SC_ERR_CUDA with context.
 int32_t cuda_error(cudaError_t e, const char* what);
+
+// Let `kernel` use `bytes` of dynamic shared memory on the current device; `done` (one per kernel)
+// remembers the devices that have been set, so only a device's first launch pays for the call.
+cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
 // Streaming multiprocessor count of the current device (cached per device).
 int sm_count();

@@ -216,7 +216,8 @@ template <typename T, int DP, int NST>
 cudaError_t launch_weights(const WeightParams& p, int64_t blocks, cudaStream_t s, bool load_only) {
     auto kernel = add_weights<T, DP, NST>;
     constexpr int kMost = kWWarps * NST * kWTile * DP * 2 + (DP == 256 ? 128 : 256) * (DP * 2 + 8);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    static std::atomic<uint64_t> done{0};
+    cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), kMost, done);
     if (e != cudaSuccess || load_only) return e;
     const int bytes = kWWarps * NST * kWTile * DP * 2 + p.row_room * (DP * 2 + 8);
     kernel<<<static_cast<unsigned>(blocks), kWThreads, bytes, s>>>(p);

@@ -22,32 +22,50 @@ from .validation import require_apart, require_cuda, require_no_grad, same_view
 _DTYPES = (torch.float16, torch.bfloat16)
 
 
-def _check_like(name: str, t: torch.Tensor, q: torch.Tensor, shape: tuple) -> None:
-    if tuple(t.shape) != shape:
+def _refuse_rows(name: str, t: torch.Tensor):
+    raise ValueError(f"{name}: head_dim must be contiguous and rows must start at multiples of "
+                     f"16 bytes, got strides {tuple(t.stride())}")
+
+
+def _like(name: str, t: torch.Tensor, shape: tuple, dtype: torch.dtype, dev: torch.device) -> None:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, got {tuple(t.shape)}")
-    if t.dtype != q.dtype:
-        raise TypeError(f"{name} must be {q.dtype} like q, got {t.dtype}")
-    if t.device != q.device:
-        raise ValueError(f"{name} is on {t.device}, q on {q.device}")
-    _check_rows(name, t)
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype} like q, got {t.dtype}")
+    if t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, q on {dev}")
 
 
-def _check_rows(name: str, t: torch.Tensor) -> None:
-    """Unit stride along the head, rows at multiples of 16 bytes."""
-    st = t.stride()
-    n = 16 // t.element_size()
-    if t.numel() and (st[-1] != 1 and t.shape[-1] > 1 or t.data_ptr() % 16 or
-                      any(s % n for s, size in zip(st[:-1], t.shape) if size > 1)):
-        raise ValueError(f"{name}: head_dim must be contiguous and rows must start at multiples of "
-                         f"16 bytes, got strides {tuple(st)}")
+def _rows3(name: str, t: torch.Tensor) -> tuple[int, int]:
+    """Strides of ``[n, H, D]`` rows of 16-bit values (0 where a dimension has one entry), with
+    a unit stride along the head and every row at a multiple of 16 bytes."""
+    n0, n1, n2 = t.shape
+    s0, s1, s2 = t.stride()
+    if n0 < 2:
+        s0 = 0
+    if n1 < 2:
+        s1 = 0
+    if ((s0 | s1) & 7 or s2 != 1 or t.data_ptr() & 15) and t.numel():
+        _refuse_rows(name, t)
+    return s0, s1
 
 
-def _row_strides(t: torch.Tensor) -> tuple[int, ...]:
-    """Strides of all dimensions but the last; 0 where a dimension has one entry."""
-    return tuple(s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]))
+def _rows4(name: str, t: torch.Tensor, mask: int = 7) -> tuple[int, int, int]:
+    """:func:`_rows3` of ``[B, n, H, D]``; ``mask``: elements of 16 bytes, less one."""
+    nb, n0, n1, n2 = t.shape
+    sb, s0, s1, s2 = t.stride()
+    if nb < 2:
+        sb = 0
+    if n0 < 2:
+        s0 = 0
+    if n1 < 2:
+        s1 = 0
+    if ((sb | s0 | s1) & mask or s2 != 1 or t.data_ptr() & 15) and t.numel():
+        _refuse_rows(name, t)
+    return sb, s0, s1
 
 
-def _check_queries(what: str, q: torch.Tensor, kv_heads: int) -> tuple[int, int, int]:
+def _check_queries(q: torch.Tensor, kv_heads: int) -> tuple[int, int, int]:
     if q.ndim != 3:
         raise ValueError(f"q must be [tokens, heads, head_dim], got {tuple(q.shape)}")
     if q.dtype not in _DTYPES:
@@ -57,11 +75,10 @@ def _check_queries(what: str, q: torch.Tensor, kv_heads: int) -> tuple[int, int,
         raise ValueError(f"head_dim must be a multiple of 8 and at most 256, got {d}")
     if kv_heads == 0 or hq % kv_heads:
         raise ValueError(f"{hq} query heads are no multiple of {kv_heads} KV heads")
-    _check_rows("q", q)
     return n, hq, d
 
 
-def _sequence_starts(what: str, n: int, batch: int, q_lens, cu_q_lens, max_q_len):
+def _sequence_starts(n: int, batch: int, q_lens, cu_q_lens, max_q_len):
     """(starts or None, tokens a sequence at most) from whichever the caller gave."""
     if q_lens is not None and cu_q_lens is not None:
         raise ValueError("give q_lens or cu_q_lens, not both")
@@ -96,8 +113,9 @@ def _sequence_starts(what: str, n: int, batch: int, q_lens, cu_q_lens, max_q_len
 
 def _lengths(name: str, lens, batch: int, most: int):
     """int32 [batch] lengths; host values are checked here, device values by the kernel."""
-    if lens is None:
-        return None
+    if lens is None or (isinstance(lens, torch.Tensor) and lens.is_cuda and lens.dtype == torch.int32 and
+                        lens.shape == (batch,) and lens.stride(0) == 1):
+        return lens
     if not isinstance(lens, torch.Tensor):
         lens = torch.as_tensor(lens)
     if lens.dtype not in (torch.int32, torch.int64):
@@ -111,7 +129,10 @@ def _lengths(name: str, lens, batch: int, most: int):
 
 def _on_device(what: str, tensors: list, device: torch.device) -> list:
     """Device versions of the given (or None) small arguments."""
-    if all(t is None or t.device == device for t in tensors):
+    for t in tensors:
+        if t is not None and t.device != device:
+            break
+    else:
         return tensors
     there = [t for t in tensors if t is not None]
     moved = iter(step_arguments(what, there, device))
@@ -165,19 +186,25 @@ def shared_prefix_attention(
     if ref.ndim < 2:
         raise ValueError(f"keys must be [.., Hkv, D], got {tuple(ref.shape)}")
     hk = ref.shape[-2]
-    n, hq, d = _check_queries("shared_prefix_attention", q, hk)
-    p_len = 0
+    n, hq, d = _check_queries(q, hk)
+    dtype = q.dtype
+    st = _lib.stride_buffer()
+    qs = st.put(_rows3("q", q))
+    p_len, kps, vps = 0, None, None
     if k_prefix is not None:
         p_len = k_prefix.shape[0]
-        _check_like("k_prefix", k_prefix, q, (p_len, hk, d))
-        _check_like("v_prefix", v_prefix, q, (p_len, hk, d))
-    batch, cap, page, n_pages, table, lens = 0, 0, 1, 0, None, None
+        shape = (p_len, hk, d)
+        _like("k_prefix", k_prefix, shape, dtype, dev)
+        _like("v_prefix", v_prefix, shape, dtype, dev)
+        kps, vps = st.put(_rows3("k_prefix", k_prefix)), st.put(_rows3("v_prefix", v_prefix))
+    batch, cap, page, n_pages, table, lens, kcs, vcs = 0, 0, 1, 0, None, None, None, None
     if k_cache is not None:
         if k_cache.ndim != 4:
             raise ValueError(f"caches must be [B, S, Hkv, D], got {tuple(k_cache.shape)}")
         shape = (k_cache.shape[0], k_cache.shape[1], hk, d)
-        _check_like("k_cache", k_cache, q, shape)
-        _check_like("v_cache", v_cache, q, shape)
+        _like("k_cache", k_cache, shape, dtype, dev)
+        _like("v_cache", v_cache, shape, dtype, dev)
+        kcs, vcs = st.put(_rows4("k_cache", k_cache)), st.put(_rows4("v_cache", v_cache))
         if page_table is not None:
             table = page_table if isinstance(page_table, torch.Tensor) else torch.as_tensor(page_table)
             if table.ndim != 2:
@@ -198,12 +225,13 @@ def shared_prefix_attention(
     if batch or q_lens is not None or cu_q_lens is not None:
         if batch == 0 and k_cache is None:
             raise ValueError("q_lens belong to caches, none given")
-        cu, nq = _sequence_starts("shared_prefix_attention", n, batch, q_lens, cu_q_lens, max_q_len)
+        cu, nq = _sequence_starts(n, batch, q_lens, cu_q_lens, max_q_len)
     if out is None:
-        out = torch.empty((n, hq, d), dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     else:
-        _check_like("out", out, q, (n, hq, d))
+        _like("out", out, (n, hq, d), dtype, dev)
         require_apart("out", out, q, k_prefix, v_prefix, k_cache, v_cache)
+    os = st.put(_rows3("out", out))
     lse = torch.empty((n, hq), dtype=torch.float32, device=dev)
     if n == 0 or hq == 0:
         return out, lse
@@ -217,19 +245,17 @@ def shared_prefix_attention(
     with _lib.on_device(dev):
         rc = lib.sc_shared_prefix_attention_workspace(n, batch, hq, hk, d, nq, p_len, cap, page,
                                                       ctypes.addressof(size))
-        _lib.check(rc, "shared_prefix_attention")
-        work = torch.empty(size.value, dtype=torch.uint8, device=dev)
-        st = _lib.stride_buffer()
+        if rc:
+            _lib.check(rc, "shared_prefix_attention")
+        need = size.value
+        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         rc = lib.sc_shared_prefix_attention(
-            n, batch, hq, hk, d, _lib.DTYPE_CODE[q.dtype],
-            q.data_ptr(), st.put(_row_strides(q)),
-            p_len, _lib.ptr(k_prefix), st.put(_row_strides(k_prefix)) if p_len else None,
-            _lib.ptr(v_prefix), st.put(_row_strides(v_prefix)) if p_len else None,
-            cap, _lib.ptr(k_cache), st.put(_row_strides(k_cache)) if cap else None,
-            _lib.ptr(v_cache), st.put(_row_strides(v_cache)) if cap else None,
-            _lib.ptr(lens), _lib.ptr(table), table.stride(0) if table is not None else 0, page, n_pages,
-            _lib.ptr(cu), nq, scale, out.data_ptr(), st.put(_row_strides(out)), lse.data_ptr(),
-            work.data_ptr(), size.value, _status_word(dev).data_ptr(), _lib.stream_handle(dev))
+            n, batch, hq, hk, d, _lib.DTYPE_CODE[dtype], q.data_ptr(), qs,
+            p_len, _lib.ptr(k_prefix), kps, _lib.ptr(v_prefix), vps,
+            cap, _lib.ptr(k_cache), kcs, _lib.ptr(v_cache), vcs, _lib.ptr(lens),
+            _lib.ptr(table), table.stride(0) if table is not None else 0, page, n_pages,
+            _lib.ptr(cu), nq, scale, out.data_ptr(), os, lse.data_ptr(),
+            _lib.ptr(work), need, _status_word(dev).data_ptr(), _lib.stream_handle(dev))
     _lib.check(rc, "shared_prefix_attention")
     return out, lse
 
@@ -270,15 +296,16 @@ def accumulate_attention_weights(
     if k_cache.ndim != 4:
         raise ValueError(f"k_cache must be [B, S, Hkv, D], got {tuple(k_cache.shape)}")
     batch, s, hk, _ = k_cache.shape
-    n, hq, d = _check_queries("accumulate_attention_weights", q, hk)
-    _check_like("k_cache", k_cache, q, (batch, s, hk, d))
+    n, hq, d = _check_queries(q, hk)
+    _like("k_cache", k_cache, (batch, s, hk, d), q.dtype, dev)
+    qs, ks = _rows3("q", q), _rows4("k_cache", k_cache)
     if out is None:
         out = scores
     for name, t, shape in (("lse", lse, (n, hq)), ("scores", scores, (batch, hk, s)),
                            ("out", out, (batch, hk, s))):
         if t.dtype != torch.float32:
             raise TypeError(f"{name} must be float32, got {t.dtype}")
-        if tuple(t.shape) != shape or t.device != dev:
+        if t.shape != shape or t.device != dev:
             raise ValueError(f"{name} must be {list(shape)} on {dev}, got {tuple(t.shape)} on {t.device}")
     for name, t in (("scores", scores), ("out", out)):
         if t.stride(2) != 1 and s > 1:
@@ -288,7 +315,7 @@ def accumulate_attention_weights(
     else:
         require_apart("out", out, q, k_cache, lse, scores)
     lens = _lengths("cache_lens", cache_lens, batch, s)
-    cu, nq = _sequence_starts("accumulate_attention_weights", n, batch, q_lens, cu_q_lens, max_q_len)
+    cu, nq = _sequence_starts(n, batch, q_lens, cu_q_lens, max_q_len)
     if out.numel() == 0:
         return out
     lens, cu = _on_device("accumulate_attention_weights", [lens, cu], dev)
@@ -300,8 +327,8 @@ def accumulate_attention_weights(
     st = _lib.stride_buffer()
     with _lib.on_device(dev):
         rc = lib.sc_accumulate_attention_weights(
-            n, batch, hq, hk, d, _lib.DTYPE_CODE[q.dtype], q.data_ptr(), st.put(_row_strides(q)),
-            s, k_cache.data_ptr(), st.put(_row_strides(k_cache)), _lib.ptr(lens), _lib.ptr(cu), nq,
+            n, batch, hq, hk, d, _lib.DTYPE_CODE[q.dtype], q.data_ptr(), st.put(qs),
+            s, k_cache.data_ptr(), st.put(ks), _lib.ptr(lens), _lib.ptr(cu), nq,
             1 if causal else 0, scale, lse.data_ptr(), st.put(lse.stride()),
             scores.data_ptr(), st.put(scores.stride()[:2]), out.data_ptr(), st.put(out.stride()[:2]),
             _status_word(dev).data_ptr(), _lib.stream_handle(dev))

@@ -7,7 +7,7 @@ from typing import NamedTuple
 import torch
 
 from .. import _lib
-from .attention import _check_rows, _lengths, _on_device, _row_strides
+from .attention import _lengths, _on_device, _rows4
 from .paged import _status_word
 from .validation import require_apart, require_cuda, require_no_grad, same_view
 
@@ -75,10 +75,11 @@ def evict_tokens(
         raise TypeError(f"v_cache must be {k_cache.dtype} like k_cache, got {v_cache.dtype}")
     if scores.dtype != torch.float32:
         raise TypeError(f"scores must be float32, got {scores.dtype}")
-    if tuple(scores.shape) != (b, h, s) or scores.device != dev:
+    if scores.shape != (b, h, s) or scores.device != dev:
         raise ValueError(f"scores must be {[b, h, s]} on {dev}, got {tuple(scores.shape)} on {scores.device}")
-    _check_rows("k_cache", k_cache)
-    _check_rows("v_cache", v_cache)
+    mask = 16 // k_cache.element_size() - 1
+    st = _lib.stride_buffer()
+    ks, vs = st.put(_rows4("k_cache", k_cache, mask)), st.put(_rows4("v_cache", v_cache, mask))
     lens = _lengths("cache_lens", cache_lens, b, s)
     fresh = torch.empty if lens is None and s >= budget else torch.zeros
     in_place = False
@@ -94,12 +95,10 @@ def evict_tokens(
             outs.append(out)
             continue
         want = (b, h, budget) if name == "scores_out" else (b, budget, h, d)
-        if tuple(out.shape) != want or out.device != dev:
+        if out.shape != want or out.device != dev:
             raise ValueError(f"{name} must be {list(want)} on {dev}, got {tuple(out.shape)} on {out.device}")
         if out.dtype != src.dtype:
             raise TypeError(f"{name} must be {src.dtype}, got {out.dtype}")
-        if name != "scores_out":
-            _check_rows(name, out)
         if budget and same_view(out, src):
             if budget > s:
                 raise ValueError(f"{name} in place cannot hold more than its {s} tokens")
@@ -118,15 +117,14 @@ def evict_tokens(
         return Evicted(*outs, indices, new_lens)
     (lens,) = _on_device("evict_tokens", [lens], dev)
     ko, vo, so = outs
+    kos, vos = st.put(_rows4("k_out", ko, mask)), st.put(_rows4("v_out", vo, mask))
     lib = _lib.load()
-    st = _lib.stride_buffer()
     with _lib.on_device(dev):
         rc = lib.sc_evict_tokens(
             b, h, s, d, k_cache.element_size(), budget, keep_first, keep_recent,
-            k_cache.data_ptr(), st.put(_row_strides(k_cache)),
-            v_cache.data_ptr(), st.put(_row_strides(v_cache)),
+            k_cache.data_ptr(), ks, v_cache.data_ptr(), vs,
             scores.data_ptr(), st.put(scores.stride()[:2]), _lib.ptr(lens), 1 if in_place else 0,
-            ko.data_ptr(), st.put(_row_strides(ko)), vo.data_ptr(), st.put(_row_strides(vo)),
+            ko.data_ptr(), kos, vo.data_ptr(), vos,
             so.data_ptr(), st.put(so.stride()[:2]), indices.data_ptr(), new_lens.data_ptr(),
             _status_word(dev).data_ptr(), _lib.stream_handle(dev))
     _lib.check(rc, "evict_tokens")

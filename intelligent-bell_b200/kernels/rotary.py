@@ -188,7 +188,7 @@ def apply_rotary(
             outs.append(None)
             continue
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=dev)
+            out = torch.empty_like(x, memory_format=torch.contiguous_format)
         else:
             if out.shape != x.shape or out.device != dev:
                 raise ValueError(f"{name} must have shape {tuple(x.shape)} on {dev}, "

@@ -120,24 +120,27 @@ def require_no_grad(what: str, *tensors: torch.Tensor | None) -> None:
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
     """Half-open byte range that ``t`` reaches."""
-    if t.numel() == 0:
-        return 0, 0
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    last = 0
+    for n, s in zip(t.shape, t.stride()):
+        if n == 0:
+            return 0, 0
+        last += (n - 1) * s
     lo = t.data_ptr()
     return lo, lo + (last + 1) * t.element_size()
 
 
 def require_apart(name: str, out: torch.Tensor, *others: torch.Tensor | None) -> None:
     """``out`` names each of its elements once and reaches into none of ``others``."""
-    for n, s in zip(out.shape, out.stride()):
-        if s == 0 and n > 1:
-            raise ValueError(f"{name} must not be an expanded tensor (strides {tuple(out.stride())})")
+    if 0 in out.stride():
+        for n, s in zip(out.shape, out.stride()):
+            if s == 0 and n > 1:
+                raise ValueError(f"{name} must not be an expanded tensor (strides {tuple(out.stride())})")
     lo, hi = _extent(out)
     for t in others:
-        if t is None or t.device != out.device:
+        if t is None:
             continue
         a, b = _extent(t)
-        if lo < b and a < hi:
+        if lo < b and a < hi and t.device == out.device:
             raise ValueError(f"{name} must not overlap an input or another output")
 
 
