@@ -10,11 +10,15 @@
 // scores into weights.  The running maximum that scales O is only raised when a score passes it
 // by 2^8, so O is rarely rescaled (weights up to 2^8 and their fp32 sums lose nothing).
 //
-// Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies (cp.async, any
-// strides, pages and odd ends; 16-byte chunks placed in the 128-byte swizzle that the matrix
-// descriptors name), warp 11 issues the products.  Tensor memory: S0, S1 (128 columns each), O0,
-// O1 (D columns each).  Every wait has a limit; a wait that runs out sets a status bit and the
-// block leaves.
+// Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies, warp 11 issues
+// the products.  Tiles come by TMA (4-D tensor maps of prefix, caches or page pool; a page's piece
+// is a box of gcd(page, 128) rows) in the 128-byte swizzle that the matrix descriptors name; what
+// a map cannot say (pages of fewer than 8 rows' alignment, expanded strides) and the last values
+// of a cache, whose rows behind its length must read as zero, by cp.async in the same order.
+// (All tiles by cp.async from these three warps: 4.3 us a step, their address arithmetic the
+// bound.)  Tensor memory: S0, S1 (128 columns each), O0, O1 (D columns each).  Every wait has a
+// limit; a wait that runs out sets a status bit and the block leaves.
+#include <cuda.h>
 #include <math.h>
 
 #include "sc_attention.cuh"
@@ -42,6 +46,9 @@ struct TileParams {
     int32_t tiles;     // 256-row tiles, at most
     int32_t splits;    // parts of the token axis
     int32_t direct;    // one part: write the output itself
+    int32_t tma_p, tma_c;  // whether the maps below are in use
+    int32_t box_c;         // rows of a box of the own caches
+    CUtensorMap kp, vp, kc, vc;
 };
 
 // ---- barriers ----
@@ -68,6 +75,21 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     }
     *gave_up = 1;
     return false;
+}
+
+__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
+                 : "memory");
+}
+
+// One box: columns from x, rows from t of head h of sequence (or page) b.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int t,
+                                         int h, int b) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
+        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
+        "l"(map), "r"(bar), "r"(x), "r"(t), "r"(h), "r"(b)
+        : "memory");
 }
 
 // ---- tensor core and tensor memory ----
@@ -123,6 +145,19 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float y;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
+    return y;
 }
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -223,7 +258,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     volatile int* gave_up = &s_gave_up;
 
     if (threadIdx.x == 0) {
-        bar_init(q_full, kLoadWarps);
+        bar_init(q_full, kTThreads / 32);
         bar_init(drained, 1);
         for (int s = 0; s < NST; ++s) {
             bar_init(full(s), kLoadWarps);
@@ -249,113 +284,135 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s_base + 16u * i), "r"(0)
                          : "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
     }
+    // Chunks of eight columns: a warp-wide copy covers 4 rows x 8 chunks of one panel.
+    const int sub = lane >> 3, c8 = lane & 7;
+    for (int g = warp; g < n_q * 32; g += kTThreads / 32) {
+        const int r = g * 4 + sub;
+        const bool in = r < n_rows;
+        const int row = in ? r0 + r : r0;
+        const int j = static_cast<int>(fdiv(row, p.div_G));
+        const T* src = static_cast<const T*>(p.q) + (tok0 + j) * p.q_t + (h * p.G + row - j * p.G) * p.q_h;
+        const uint32_t dst = s_q + (r >> 7) * TILE;
+#pragma unroll
+        for (int pn = 0; pn < CPR / 8; ++pn) {
+            const int c = pn * 8 + c8;
+            if (c * 8 < p.D) cp_async16(dst + tile_chunk(r & 127, c), src + c * 8, in);
+        }
+    }
+    cp_async_commit();
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
+    auto copies_done = [&](uint32_t bar) {
+        cp_async_wait<0>();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) bar_arrive(bar);
+    };
+    if (warp < 8 || warp == 11) copies_done(q_full);
     constexpr uint32_t kO = 256;  // first column of O0
 
     if (warp >= 8 && warp < 8 + kLoadWarps) {
         // ---- copies ----
         const int lw = warp - 8;
-        // Chunks of eight columns: a warp-wide copy covers 4 rows x 8 chunks of one panel.
-        const int sub = lane >> 3, c8 = lane & 7;
-        auto done = [&](uint32_t bar) {
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) bar_arrive(bar);
-        };
-        for (int q = 0; q < n_q; ++q)
+        const bool paged = p.page_table != nullptr;
+        const int n_loads = 2 * n_tiles;
+        bool alive = true;
+        for (int i = 0; i < n_loads && alive; ++i) {
+            if (i == 1) copies_done(q_full);  // the first tile is on its way
+            const int s = i % NST;
+            if (i >= NST) {
+                alive = bar_wait(empty(s), ((i / NST) - 1) & 1, gave_up);
+                alive = __all_sync(0xffffffffu, alive);
+                if (!alive) break;
+            }
+            const int tile = first + (i >> 1);
+            const bool is_v = i & 1;
+            const bool pre = tile < tiles_p;
+            const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
+            const uint32_t dst = s_ring + s * TILE;
+            if (pre ? tp.tma_p : tp.tma_c && (!is_v || t0 + kTokTile <= len)) {
+                if (lw == 0) {
+                    if (lane == 0) bar_expect(full(s), TILE);
+                    __syncwarp();
+                    const CUtensorMap* map = pre ? (is_v ? &tp.vp : &tp.kp) : (is_v ? &tp.vc : &tp.kc);
+                    if (pre || !paged) {
+                        if (lane < CPR / 8) tma_load(dst + lane * 16384, map, full(s), lane * 64, t0, h, pre ? 0 : b);
+                    } else {
+                        // One lane a box; a page that is not there lies outside the map: zeros.
+                        const int box = tp.box_c, n_box = kTokTile / box;
+                        const int bx = lane % n_box, t = t0 + bx * box;
+                        int id = static_cast<int>(p.n_pages), in = 0;
+                        bool ok = true;
+                        if (t < vis) {
+                            const int pg = static_cast<int>(fdiv(t, p.div_page));
+                            in = t - pg * p.page;
+                            id = p.page_table[b * p.pt_b + pg];
+                            ok = id >= 0 && id < p.n_pages;
+                            if (!ok) id = static_cast<int>(p.n_pages);
+                        }
+                        if (!is_v) {
+                            const int local = (i >> 1) & 3;
+                            for (int e = lane / n_box; e < box; e += 32 / n_box) s_ok[local][bx * box + e] = ok;
+                            if (!ok) {
+                                s_any_bad = 1;
+                                if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
+                            }
+                            __syncwarp();
+                        }
+                        for (int pn = lane / n_box; pn < CPR / 8; pn += 32 / n_box)
+                            tma_load(dst + pn * 16384 + bx * box * 128, map, full(s), pn * 64, in, h, id);
+                    }
+                } else if (lane == 0) {
+                    bar_arrive(full(s));
+                }
+                continue;
+            }
+            const T* base;
+            int64_t st_t, st_b = 0;
+            if (pre) {
+                base = static_cast<const T*>(is_v ? p.vp : p.kp) + h * (is_v ? p.vp_h : p.kp_h);
+                st_t = is_v ? p.vp_t : p.kp_t;
+            } else {
+                base = static_cast<const T*>(is_v ? p.vc : p.kc) + h * (is_v ? p.vc_h : p.kc_h);
+                st_t = is_v ? p.vc_t : p.kc_t;
+                st_b = is_v ? p.vc_b : p.kc_b;
+                if (!paged) base += b * st_b;
+            }
+            const int t1 = pre ? p.P : vis;
             for (int g = lw; g < 32; g += kLoadWarps) {
-                const int r = g * 4 + sub;
-                const int row = r0 + q * kRowTile + r;
-                const bool in = q * kRowTile + r < n_rows;
-                const int j = static_cast<int>(fdiv(in ? row : 0, p.div_G));
-                const T* src = static_cast<const T*>(p.q) + (tok0 + (in ? j : 0)) * p.q_t +
-                               (h * p.G + (in ? row - j * p.G : 0)) * p.q_h;
+                const int r = g * 4 + sub, t = t0 + r;
+                bool in = t < t1;
+                int64_t off = 0;
+                if (in) {
+                    if (!pre && paged) {
+                        const int pg = static_cast<int>(fdiv(t, p.div_page));
+                        const int id = p.page_table[b * p.pt_b + pg];
+                        in = id >= 0 && id < p.n_pages;
+                        if (in) off = id * st_b + (t - pg * p.page) * st_t;
+                        if (!is_v && c8 == 0) {
+                            s_ok[(i >> 1) & 3][r] = in;
+                            if (!in) {
+                                s_any_bad = 1;
+                                if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
+                            }
+                        }
+                    } else {
+                        off = t * st_t;
+                    }
+                }
 #pragma unroll
                 for (int pn = 0; pn < CPR / 8; ++pn) {
                     const int c = pn * 8 + c8;
-                    if (c * 8 < p.D) cp_async16(s_q + q * TILE + tile_chunk(r, c), src + c * 8, in);
-                }
-            }
-        cp_async_commit();
-        const bool paged = p.page_table != nullptr;
-        const int n_loads = 2 * n_tiles;
-        constexpr int LAG = 2;  // copies in flight behind the newest
-        bool alive = true;
-        for (int i = 0; i < n_loads + LAG; ++i) {
-            if (i < n_loads && alive) {
-                const int s = i % NST;
-                if (i >= NST) {
-                    alive = bar_wait(empty(s), ((i / NST) - 1) & 1, gave_up);
-                    alive = __all_sync(0xffffffffu, alive);
-                }
-                if (alive) {
-                    const int tile = first + (i >> 1);
-                    const bool is_v = i & 1;
-                    const bool pre = tile < tiles_p;
-                    const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
-                    const int t1 = pre ? p.P : vis;
-                    const uint32_t dst = s_ring + s * TILE;
-                    const T* base;
-                    int64_t st_t, st_b = 0;
-                    if (pre) {
-                        base = static_cast<const T*>(is_v ? p.vp : p.kp) + h * (is_v ? p.vp_h : p.kp_h);
-                        st_t = is_v ? p.vp_t : p.kp_t;
-                    } else {
-                        base = static_cast<const T*>(is_v ? p.vc : p.kc) + h * (is_v ? p.vc_h : p.kc_h);
-                        st_t = is_v ? p.vc_t : p.kc_t;
-                        st_b = is_v ? p.vc_b : p.kc_b;
-                        if (!paged) base += b * st_b;
-                    }
-#pragma unroll
-                    for (int gi = 0; gi < (32 + kLoadWarps - 1) / kLoadWarps; ++gi) {
-                        const int g = lw + gi * kLoadWarps;
-                        if (g < 32) {
-                            const int r = g * 4 + sub, t = t0 + r;
-                            bool in = t < t1;
-                            int64_t off = 0;
-                            if (in) {
-                                if (!pre && paged) {
-                                    const int pg = static_cast<int>(fdiv(t, p.div_page));
-                                    const int id = p.page_table[b * p.pt_b + pg];
-                                    in = id >= 0 && id < p.n_pages;
-                                    if (in) off = id * st_b + (t - pg * p.page) * st_t;
-                                    if (!is_v && c8 == 0) {
-                                        s_ok[(i >> 1) & 3][r] = in;
-                                        if (!in) {
-                                            s_any_bad = 1;
-                                            if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
-                                        }
-                                    }
-                                } else {
-                                    off = t * st_t;
-                                    if (!is_v && c8 == 0 && !pre) s_ok[(i >> 1) & 3][r] = 1;
-                                }
-                            }
-#pragma unroll
-                            for (int pn = 0; pn < CPR / 8; ++pn) {
-                                const int c = pn * 8 + c8;
-                                if (c * 8 < p.D)
-                                    cp_async16(dst + tile_chunk(r, c), base + off + c * 8, in);
-                            }
-                        }
-                    }
+                    if (c * 8 < p.D) cp_async16(dst + tile_chunk(r, c), base + off + c * 8, in);
                 }
             }
             cp_async_commit();
-            if (i == 0) {
-                cp_async_wait<1>();
-                done(q_full);
-            }
-            if (i >= LAG) {
-                cp_async_wait<LAG>();
-                if (alive) done(full((i - LAG) % NST));
-            }
+            copies_done(full(s));
         }
-        cp_async_wait<0>();
     } else if (warp == 11) {
         // ---- products ----
         if (lane == 0) {
@@ -434,40 +491,48 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     const bool pre = tile < tiles_p;
                     const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
                     const int seen = (pre ? p.P : own_limit) - t0;  // columns below it count
-                    uint32_t x[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, x + c * 32);
-                    tmem_wait_ld();
                     const bool bad = !pre && *reinterpret_cast<volatile int*>(&s_any_bad) != 0;
-                    if (__any_sync(0xffffffffu, seen < kTokTile) || bad) {
-#pragma unroll
-                        for (int c = 0; c < 128; ++c) {
-                            bool on = c < seen;
-                            if (bad && on) on = s_ok[i & 3][c] != 0;
-                            if (!on) x[c] = __float_as_uint(kNegInf);
-                        }
-                    }
+                    const bool masked = __any_sync(0xffffffffu, seen < kTokTile) || bad;
+                    // A bit a column of chunk c: this row sees it.
+                    auto mask_of = [&](int c) -> uint32_t {
+                        const int n = seen - c * 32;
+                        uint32_t on = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+                        if (bad)
+                            for (int e = 0; e < 32; ++e)
+                                if (!s_ok[i & 3][c * 32 + e]) on &= ~(1u << e);
+                        return on;
+                    };
+                    // The tile's maximum.  Chunks of 32 columns, read a second time below: tensor
+                    // memory has bandwidth to spare, and the short loops stay in the instruction
+                    // cache (all 128 columns unrolled: 4.85 us a step; so: see above).
                     float top = kNegInf;
-                    const float sc = p.scale_log2;
-                    if (sc >= 0.f) {
-                        float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32];
+                        tmem_ld32(s_at + c * 32, x);
+                        tmem_wait_ld();
+                        if (p.scale_log2 <= 0.f) {  // the order turns: scale before the maximum
 #pragma unroll
-                        for (int c = 0; c < 128; ++c) t4[c & 3] = fmaxf(t4[c & 3], __uint_as_float(x[c]));
-                        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * sc;
-                    }
-                    if (!(sc > 0.f)) {  // scaled first: a mask must stay minus infinity
-                        top = kNegInf;
-#pragma unroll
-                        for (int c = 0; c < 128; ++c) {
-                            const float v = __uint_as_float(x[c]);
-                            const float w = v == kNegInf ? kNegInf : v * sc;
-                            x[c] = __float_as_uint(w);
-                            top = fmaxf(top, w);
+                            for (int e = 0; e < 32; ++e)
+                                x[e] = __float_as_uint(__uint_as_float(x[e]) * p.scale_log2);
                         }
+                        if (masked) {
+                            const uint32_t on = mask_of(c);
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!((on >> e) & 1)) x[e] = __float_as_uint(kNegInf);
+                        }
+                        float t2 = kNegInf;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 4) {
+                            top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                            t2 = max3(t2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
+                        }
+                        top = fmaxf(top, t2);
                     }
-                    const float mul = sc > 0.f ? sc : 1.f;
-                    if (__any_sync(0xffffffffu, top > m + kRaise || (m == kNegInf && top > m))) {
-                        const bool raise = top > m + kRaise || (m == kNegInf && top > m);
+                    if (p.scale_log2 > 0.f) top *= p.scale_log2;
+                    const bool raise = top > m + kRaise || (m == kNegInf && top > m);
+                    if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
@@ -476,7 +541,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             alive = __all_sync(0xffffffffu, alive);
                             if (!alive) break;
                             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < DP / 32; ++c) {
                                 uint32_t o[32];
                                 tmem_ld32(o_at + c * 32, o);
@@ -488,19 +553,40 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         }
                     }
                     const float base = m == kNegInf ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
-                    uint32_t w[64];
+                    const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                    float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+#pragma unroll 1
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t x[32], w[16];
+                        tmem_ld32(s_at + c * 32, x);
+                        tmem_wait_ld();
+                        const uint32_t on = masked ? mask_of(c) : 0xffffffffu;
 #pragma unroll
-                    for (int c = 0; c < 64; ++c) {
-                        const float e0 = exp2_fast(fmaf(__uint_as_float(x[2 * c]), mul, -base));
-                        const float e1 = exp2_fast(fmaf(__uint_as_float(x[2 * c + 1]), mul, -base));
-                        sum[(2 * c) & 3] += e0;
-                        sum[(2 * c + 1) & 3] += e1;
-                        w[c] = pack2<T>(e0, e1);  // 16-bit weights, as the product takes them
+                        for (int e = 0; e < 16; ++e) {
+                            float2 v = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                            v = __ffma2_rn(v, mul2, sub2);
+                            v.x = exp2_fast(v.x);
+                            v.y = exp2_fast(v.y);
+                            x[2 * e] = __float_as_uint(v.x);
+                            x[2 * e + 1] = __float_as_uint(v.y);
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                if (!((on >> e) & 1)) x[e] = 0;
+                        }
+#pragma unroll
+                        for (int e = 0; e < 16; ++e) {
+                            const float2 v = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                            if (e & 1)
+                                sum2 = __fadd2_rn(sum2, v);
+                            else
+                                sum = __fadd2_rn(sum, v);
+                            w[e] = pack2<T>(v.x, v.y);  // 16-bit weights, as the product takes them
+                        }
+                        tmem_st16(s_at + c * 16, w);  // over columns already read
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-                    tmem_st32(s_at, w);
-                    tmem_st32(s_at + 32, w + 32);
+                    l += (sum.x + sum.y) + (sum2.x + sum2.y);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -518,7 +604,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 T* dst = static_cast<T*>(p.out) + (tok0 + j) * p.o_t + (h * p.G + row - j * p.G) * p.o_h;
                 float* po = p.part_o + (part_row + at) * p.D;
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < DP / 32; ++c) {
                     uint32_t o[32];
                     tmem_ld32(o_at + c * 32, o);
@@ -579,6 +665,49 @@ cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, cudaStream_t s,
     return cudaGetLastError();
 }
 
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
+                                 CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult found;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
+            found != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            f = nullptr;
+        }
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// A map of [n3][n2][n1][n0] 16-bit elements (strides in elements) in boxes of 64 columns x `rows`.
+// False where a map cannot say it: the kernel then copies without one.
+bool make_map(CUtensorMap* map, bool half, const void* base, const int64_t (&n)[4], const int64_t (&st)[3],
+              int rows) {
+    const EncodeTiled encode = encode_tiled();
+    if (!encode) return false;
+    cuuint64_t dims[4], strides[3];
+    for (int i = 0; i < 4; ++i) {
+        if (n[i] <= 0 || n[i] > 0xffffffffll) return false;
+        dims[i] = static_cast<cuuint64_t>(n[i]);
+    }
+    for (int i = 0; i < 3; ++i) {
+        // a dimension of one entry has no stride of its own
+        const int64_t s = n[i + 1] == 1 ? (n[0] + 7) / 8 * 8 : st[i];
+        if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
+        strides[i] = static_cast<cuuint64_t>(s * 2);
+    }
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, step[4] = {1, 1, 1, 1};
+    return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+                  const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 }  // namespace
 
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
@@ -586,6 +715,21 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
     TileParams p{};
     p.a = a;
     p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.direct = direct;
+    if (a.P) {
+        const int64_t n[4] = {a.D, a.P, a.Hkv, 1};
+        p.tma_p = make_map(&p.kp, half, a.kp, n, {a.kp_t, a.kp_h, 0}, kTokTile) &&
+                  make_map(&p.vp, half, a.vp, n, {a.vp_t, a.vp_h, 0}, kTokTile);
+    }
+    if (per_seq && a.cap) {
+        const bool paged = a.page_table != nullptr;
+        int box = kTokTile;
+        while (paged && a.page % box) box /= 2;
+        p.box_c = box;
+        const int64_t n[4] = {a.D, paged ? a.page : a.cap, a.Hkv, paged ? a.n_pages : a.B};
+        // a box starts at a swizzle atom: 8 rows
+        p.tma_c = box >= 8 && make_map(&p.kc, half, a.kc, n, {a.kc_t, a.kc_h, a.kc_b}, box) &&
+                  make_map(&p.vc, half, a.vc, n, {a.vc_t, a.vc_h, a.vc_b}, box);
+    }
     const unsigned n = static_cast<unsigned>(units);
     if (a.D <= 64)
         return half ? launch_tiles_dp<__half, 64>(p, n, s, false)
