@@ -30,7 +30,7 @@ constexpr int kTThreads = 384;
 constexpr int kLoadWarps = 3;
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
-constexpr int kWaitLimit = 1 << 18;  // tries of at most about 2 us each
+constexpr int kWaitLimit = 1 << 20;  // tries
 constexpr float kRaise = 8.f;  // log2: how far a score may pass the maximum in use
 
 template <int DP>
@@ -61,7 +61,7 @@ __device__ __forceinline__ void bar_arrive(uint32_t bar) {
 __device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
     uint32_t ok;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 2000;\n"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
         " selp.u32 %0, 1, 0, p;\n}"
         : "=r"(ok)
         : "r"(bar), "r"(parity)
@@ -75,6 +75,12 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     }
     *gave_up = 1;
     return false;
+}
+// The same for a whole warp: one lane asks, all get its answer.
+__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = bar_wait(bar, parity, gave_up);
+    return __shfl_sync(0xffffffffu, ok, 0);
 }
 
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
@@ -190,7 +196,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     __shared__ __align__(8) uint64_t s_bars[2 * NST + 8];
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
-    __shared__ int s_any_bad;
+    __shared__ int s_any_bad, s_copy;
     __shared__ unsigned char s_ok[4][kTokTile];
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         bar_init(q_full, kTThreads / 32);
         bar_init(drained, 1);
         for (int s = 0; s < NST; ++s) {
-            bar_init(full(s), kLoadWarps);
+            bar_init(full(s), 1);
             bar_init(empty(s), 1);
         }
         for (int q = 0; q < 2; ++q) {
@@ -321,14 +327,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         const bool paged = p.page_table != nullptr;
         const int n_loads = 2 * n_tiles;
         bool alive = true;
-        for (int i = 0; i < n_loads && alive; ++i) {
+        for (int i = 0; i < n_loads; ++i) {
             if (i == 1) copies_done(q_full);  // the first tile is on its way
             const int s = i % NST;
-            if (i >= NST) {
-                alive = bar_wait(empty(s), ((i / NST) - 1) & 1, gave_up);
-                alive = __all_sync(0xffffffffu, alive);
-                if (!alive) break;
-            }
             const int tile = first + (i >> 1);
             const bool is_v = i & 1;
             const bool pre = tile < tiles_p;
@@ -336,6 +337,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             const uint32_t dst = s_ring + s * TILE;
             if (pre ? tp.tma_p : tp.tma_c && (!is_v || t0 + kTokTile <= len)) {
                 if (lw == 0) {
+                    if (i >= NST) alive = bar_wait_warp(empty(s), ((i / NST) - 1) & 1, gave_up);
+                    if (!alive) continue;
                     if (lane == 0) bar_expect(full(s), TILE);
                     __syncwarp();
                     const CUtensorMap* map = pre ? (is_v ? &tp.vp : &tp.kp) : (is_v ? &tp.vc : &tp.kc);
@@ -366,11 +369,17 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         for (int pn = lane / n_box; pn < CPR / 8; pn += 32 / n_box)
                             tma_load(dst + pn * 16384 + bx * box * 128, map, full(s), pn * 64, in, h, id);
                     }
-                } else if (lane == 0) {
-                    bar_arrive(full(s));
                 }
                 continue;
             }
+            // The first copying warp waits for the stage and tells the other two.
+            if (lw == 0) {
+                if (alive && i >= NST) alive = bar_wait_warp(empty(s), ((i / NST) - 1) & 1, gave_up);
+                if (lane == 0) s_copy = alive;
+            }
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kLoadWarps) : "memory");
+            alive = *reinterpret_cast<volatile int*>(&s_copy) != 0;
+            if (!alive) break;
             const T* base;
             int64_t st_t, st_b = 0;
             if (pre) {
@@ -411,7 +420,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 }
             }
             cp_async_commit();
-            copies_done(full(s));
+            cp_async_wait<0>();
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * kLoadWarps) : "memory");
+            if (lw == 0 && lane == 0) bar_arrive(full(s));
         }
     } else if (warp == 11) {
         // ---- products ----
@@ -420,20 +432,24 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             constexpr uint32_t id_common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
             constexpr uint32_t id_qk = id_common | ((128u >> 3) << 17);
             constexpr uint32_t id_pv = id_common | ((static_cast<uint32_t>(DP) >> 3) << 17) | (1u << 16);
+            // Descriptors of the first step; a step's address is added to the low word.
+            const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_ring, 16, 1024),
+                           v_desc = desc(s_ring, 16384, 1024);
             auto qk = [&](int q, int stage) {
-                const uint32_t qa = s_q + q * TILE, ka = s_ring + stage * TILE;
+                const uint64_t qd = q_desc + static_cast<uint32_t>(q * (TILE / 16));
+                const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (TILE / 16));
 #pragma unroll
                 for (int kk = 0; kk < DP / 16; ++kk) {
-                    const uint32_t off = (kk >> 2) * 16384 + (kk & 3) * 32;
-                    mma_ss(tmem + q * 128, desc(qa + off, 16, 1024), desc(ka + off, 16, 1024), id_qk, kk > 0);
+                    const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
+                    mma_ss(tmem + q * 128, qd + off, kd + off, id_qk, kk > 0);
                 }
             };
             auto pv = [&](int q, int stage, bool add) {
-                const uint32_t va = s_ring + stage * TILE;
+                const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (TILE / 16));
 #pragma unroll
                 for (int kk = 0; kk < kTokTile / 16; ++kk)
-                    mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, desc(va + kk * 2048, 16384, 1024),
-                           id_pv, add || kk > 0);
+                    mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, vd + kk * (2048 / 16), id_pv,
+                           add || kk > 0);
             };
             bool alive = bar_wait(q_full, 0, gave_up) && bar_wait(full(0), 0, gave_up);
             if (alive) {
@@ -446,7 +462,6 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             for (int i = 0; i < n_tiles && alive; ++i) {
                 const int vl = 2 * i + 1, kl = 2 * i + 2;  // loads V_i, K_{i+1}
                 alive = bar_wait(full(vl % NST), (vl / NST) & 1, gave_up);
-                if (alive && i + 1 < n_tiles) alive = bar_wait(full(kl % NST), (kl / NST) & 1, gave_up);
                 for (int q = 0; q < n_q && alive; ++q) {
                     alive = bar_wait(p_full(q), i & 1, gave_up);
                     if (!alive) break;
@@ -456,6 +471,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     if (i + 1 < n_tiles) {
                         // The weights that this product reads lie where the next scores go.
                         alive = bar_wait(o_full(q), i & 1, gave_up);
+                        if (alive && q == 0) alive = bar_wait(full(kl % NST), (kl / NST) & 1, gave_up);
                         if (!alive) break;
                         qk(q, kl % NST);
                         tc_commit(s_full(q));
@@ -482,8 +498,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             float m = kNegInf, l = 0.f;  // m: the maximum in use
             bool alive = true;
             for (int i = 0; i < n_tiles; ++i) {
-                alive = bar_wait(s_full(q), i & 1, gave_up);
-                alive = __all_sync(0xffffffffu, alive);
+                alive = bar_wait_warp(s_full(q), i & 1, gave_up);
                 if (!alive) break;
                 tc_fence_after();
                 if (any) {
@@ -493,52 +508,46 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     const int seen = (pre ? p.P : own_limit) - t0;  // columns below it count
                     const bool bad = !pre && *reinterpret_cast<volatile int*>(&s_any_bad) != 0;
                     const bool masked = __any_sync(0xffffffffu, seen < kTokTile) || bad;
-                    // A bit a column of chunk c: this row sees it.
-                    auto mask_of = [&](int c) -> uint32_t {
-                        const int n = seen - c * 32;
-                        uint32_t on = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-                        if (bad)
-                            for (int e = 0; e < 32; ++e)
-                                if (!s_ok[i & 3][c * 32 + e]) on &= ~(1u << e);
-                        return on;
-                    };
-                    // The tile's maximum.  Chunks of 32 columns, read a second time below: tensor
-                    // memory has bandwidth to spare, and the short loops stay in the instruction
-                    // cache (all 128 columns unrolled: 4.85 us a step; so: see above).
-                    float top = kNegInf;
-#pragma unroll 1
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32];
-                        tmem_ld32(s_at + c * 32, x);
-                        tmem_wait_ld();
-                        if (p.scale_log2 <= 0.f) {  // the order turns: scale before the maximum
+                    uint32_t x[128];
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                x[e] = __float_as_uint(__uint_as_float(x[e]) * p.scale_log2);
-                        }
-                        if (masked) {
-                            const uint32_t on = mask_of(c);
+                    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, x + c * 32);
+                    tmem_wait_ld();
+                    if (p.scale_log2 <= 0.f) {  // the order turns: scale before the maximum
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!((on >> e) & 1)) x[e] = __float_as_uint(kNegInf);
-                        }
-                        float t2 = kNegInf;
-#pragma unroll
-                        for (int e = 0; e < 32; e += 4) {
-                            top = max3(top, __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-                            t2 = max3(t2, __uint_as_float(x[e + 2]), __uint_as_float(x[e + 3]));
-                        }
-                        top = fmaxf(top, t2);
+                        for (int e = 0; e < 128; ++e)
+                            x[e] = __float_as_uint(__uint_as_float(x[e]) * p.scale_log2);
                     }
-                    if (p.scale_log2 > 0.f) top *= p.scale_log2;
+                    if (masked) {
+                        uint32_t on[4];  // a bit a column: this row sees it
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int n = seen - c * 32;
+                            on[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
+                            if (bad)
+                                for (int e = 0; e < 32; ++e)
+                                    if (!s_ok[i & 3][c * 32 + e]) on[c] &= ~(1u << e);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            if (!((on[e >> 5] >> (e & 31)) & 1)) x[e] = __float_as_uint(kNegInf);
+                    }
+                    float top = kNegInf;
+                    {
+                        float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
+#pragma unroll
+                        for (int e = 0; e < 128; e += 2)
+                            t4[(e >> 1) & 3] = max3(t4[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
+                    }
+                    const float mul = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
+                    top *= mul;
                     const bool raise = top > m + kRaise || (m == kNegInf && top > m);
                     if (__any_sync(0xffffffffu, raise)) {
                         const float f = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
                         if (i > 0) {
-                            alive = bar_wait(o_full(q), (i - 1) & 1, gave_up);
-                            alive = __all_sync(0xffffffffu, alive);
+                            alive = bar_wait_warp(o_full(q), (i - 1) & 1, gave_up);
                             if (!alive) break;
                             tc_fence_after();
 #pragma unroll 1
@@ -553,38 +562,25 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         }
                     }
                     const float base = m == kNegInf ? 0.f : m;
-                    const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                    const float2 mul2 = make_float2(mul, mul), sub2 = make_float2(-base, -base);
                     float2 sum = make_float2(0.f, 0.f), sum2 = sum;
-#pragma unroll 1
+#pragma unroll
                     for (int c = 0; c < 4; ++c) {
-                        uint32_t x[32], w[16];
-                        tmem_ld32(s_at + c * 32, x);
-                        tmem_wait_ld();
-                        const uint32_t on = masked ? mask_of(c) : 0xffffffffu;
+                        uint32_t w[16];
 #pragma unroll
                         for (int e = 0; e < 16; ++e) {
-                            float2 v = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
+                            float2 v = make_float2(__uint_as_float(x[c * 32 + 2 * e]),
+                                                   __uint_as_float(x[c * 32 + 2 * e + 1]));
                             v = __ffma2_rn(v, mul2, sub2);
                             v.x = exp2_fast(v.x);
                             v.y = exp2_fast(v.y);
-                            x[2 * e] = __float_as_uint(v.x);
-                            x[2 * e + 1] = __float_as_uint(v.y);
-                        }
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                if (!((on >> e) & 1)) x[e] = 0;
-                        }
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            const float2 v = make_float2(__uint_as_float(x[2 * e]), __uint_as_float(x[2 * e + 1]));
                             if (e & 1)
                                 sum2 = __fadd2_rn(sum2, v);
                             else
                                 sum = __fadd2_rn(sum, v);
                             w[e] = pack2<T>(v.x, v.y);  // 16-bit weights, as the product takes them
                         }
-                        tmem_st16(s_at + c * 16, w);  // over columns already read
+                        tmem_st16(s_at + c * 16, w);
                     }
                     l += (sum.x + sum.y) + (sum2.x + sum2.y);
                     tmem_wait_st();
@@ -594,8 +590,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 if (lane == 0) bar_arrive(p_full(q));
             }
             if (alive) {
-                alive = bar_wait(o_full(q), (n_tiles - 1) & 1, gave_up);
-                alive = __all_sync(0xffffffffu, alive);
+                alive = bar_wait_warp(o_full(q), (n_tiles - 1) & 1, gave_up);
             }
             if (alive && any) {
                 tc_fence_after();
