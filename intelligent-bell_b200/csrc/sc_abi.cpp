@@ -55,15 +55,25 @@ int sm_count() {
     return n;
 }
 
-cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+namespace {
+cudaError_t set_once(const void* kernel, cudaFuncAttribute what, int value, std::atomic<uint64_t>& done) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
     if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    e = cudaFuncSetAttribute(kernel, what, value);
     if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
     return e;
+}
+}  // namespace
+
+cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+    return set_once(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes, done);
+}
+
+cudaError_t allow_clusters(const void* kernel, std::atomic<uint64_t>& done) {
+    return set_once(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1, done);
 }
 
 void default_inv_freq(int32_t head_dim, double theta, float* out) {

@@ -105,18 +105,6 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
         return;
     }
 
-    // Queries of the tile, zeros behind the last row and behind D.
-    for (int i = threadIdx.x; i < MR * CPR; i += kThreads) {
-        const int r = i / CPR, c = i - r * CPR;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (r < n_rows && c * 8 < p.D) {
-            const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
-            const int g = r0 + r - j * p.G;
-            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (tok0 + j) * p.q_t +
-                                                (h * p.G + g) * p.q_h + c * 8);
-        }
-        *reinterpret_cast<uint4*>(s_q + chunk_at<DP>(r, c)) = v;
-    }
     if (p.D < DP) {  // columns that no copy writes
         for (int i = threadIdx.x; i < RowsShape<DP, MT, TK, NST>::kRing / 16; i += kThreads)
             reinterpret_cast<uint4*>(s_ring)[i] = make_uint4(0, 0, 0, 0);
@@ -124,7 +112,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     const bool paged = !is_prefix && p.page_table != nullptr;
     int first_page = 0;
     if (threadIdx.x == 0) s_bad = 0;
-    __syncthreads();
+    if (paged || p.D < DP) __syncthreads();
     if (paged) {
         first_page = static_cast<int>(fdiv(t0, p.div_page));
         const int last = static_cast<int>(fdiv(t1 - 1, p.div_page));
@@ -139,8 +127,6 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
         }
         __syncthreads();
     }
-    const bool bad = s_bad != 0;
-
     const T* kbase;
     const T* vbase;
     int64_t k_t, v_t, k_b = 0, v_b = 0;
@@ -194,6 +180,22 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
         cp_async_commit();
     };
 
+    for (int i = 0; i < NST - 1; ++i) issue(i);
+    // Queries of the tile, zeros behind the last row and behind D.
+    for (int i = threadIdx.x; i < MR * CPR; i += kThreads) {
+        const int r = i / CPR, c = i - r * CPR;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < n_rows && c * 8 < p.D) {
+            const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+            const int g = r0 + r - j * p.G;
+            v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + (tok0 + j) * p.q_t +
+                                                (h * p.G + g) * p.q_h + c * 8);
+        }
+        *reinterpret_cast<uint4*>(s_q + chunk_at<DP>(r, c)) = v;
+    }
+    __syncthreads();
+    const bool bad = s_bad != 0;
+
     float o[MT][DP / 8][4];
     float m[MT][2], l[MT][2];
     int lim[MT][2];  // tokens below it are seen
@@ -215,7 +217,6 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     // Tiles that end below it are seen whole by every row.
     const int whole = bad ? -1 : is_prefix ? t1 : min(t1, see + static_cast<int>(fdiv(r0, p.div_G)) + 1);
 
-    for (int i = 0; i < NST - 1; ++i) issue(i);
     const uint32_t q_addr = smem_addr(s_q);
     for (int i = 0; i < my_tiles; ++i) {
         cp_async_wait<NST - 2>();
@@ -403,21 +404,38 @@ __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ A
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f), b = a;
     float sum = 0.f;
     const int d0 = lane * 4, d1 = 128 + lane * 4;
-    for (int i = 0; i < parts; ++i) {
-        const float2 ml = p.part_ml[i * all_rows + row];
-        if (ml.x == kNegInf && ml.y == 0.f) continue;  // nothing seen in this part
-        const float w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
-        sum += w * ml.y;
-        const float* src = p.part_o + (i * all_rows + row) * p.D;
-        if (d0 < p.D) {
-            const float4 v = *reinterpret_cast<const float4*>(src + d0);
-            a.x += w * v.x, a.y += w * v.y, a.z += w * v.z, a.w += w * v.w;
+    const int64_t step = all_rows * p.D;
+    const float* src = p.part_o + row * p.D;
+    for (int g = 0; g < parts; g += 32) {
+        // A lane a part: its weight; 0 where the part saw nothing (its o was not written).
+        float w = 0.f;
+        if (g + lane < parts) {
+            const float2 ml = p.part_ml[(g + lane) * all_rows + row];
+            w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
+            sum += ml.x == kNegInf && ml.y == 0.f ? 0.f : w * ml.y;
         }
-        if (d1 < p.D) {
-            const float4 v = *reinterpret_cast<const float4*>(src + d1);
-            b.x += w * v.x, b.y += w * v.y, b.z += w * v.z, b.w += w * v.w;
+        const int n = min(32, parts - g);
+        for (int i = 0; i < n; i += 4, src += 4 * step) {
+            float wi[4];
+            float4 v[4], u[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {  // four parts' loads in flight
+                wi[j] = __shfl_sync(0xffffffffu, w, i + j);
+                v[j] = u[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (!(wi[j] == 0.f)) {
+                    if (d0 < p.D) v[j] = *reinterpret_cast<const float4*>(src + j * step + d0);
+                    if (d1 < p.D) u[j] = *reinterpret_cast<const float4*>(src + j * step + d1);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                a.x += wi[j] * v[j].x, a.y += wi[j] * v[j].y, a.z += wi[j] * v[j].z, a.w += wi[j] * v[j].w;
+                b.x += wi[j] * u[j].x, b.y += wi[j] * u[j].y, b.z += wi[j] * u[j].z, b.w += wi[j] * u[j].w;
+            }
         }
     }
+#pragma unroll
+    for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
     const float inv = sum == 0.f ? 0.f : 1.f / sum;  // a row that sees nothing is zero
     const int64_t tok = row / p.Hq, head = row - tok * p.Hq;
     T* dst = static_cast<T*>(p.out) + tok * p.o_t + head * p.o_h;
@@ -475,6 +493,9 @@ cudaError_t preload_attention_type() {
 }
 
 // How the rows and tokens are split over kernels and parts.
+#ifndef SC_ROWS_WAVES
+#define SC_ROWS_WAVES 2
+#endif
 struct Split {
     Variant v;
     bool tile_p;   // the prefix by attend_tiles
@@ -536,7 +557,7 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
         s.tiles_c = static_cast<int32_t>((rows_c + mr - 1) / mr);
         const double work = static_cast<double>(P_rows) * Hkv * s.tiles_p +
                             static_cast<double>(cap) * Hkv * B * s.tiles_c;
-        double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
+        double chunk = ceil(work / (148.0 * 2 * SC_ROWS_WAVES) / kPartTokens) * kPartTokens;
         const double longest = P_rows > cap ? P_rows : cap;
         const double most_parts = 64;
         if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;

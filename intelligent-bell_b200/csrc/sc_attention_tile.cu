@@ -18,10 +18,9 @@
 // (All tiles by cp.async from these three warps: 4.3 us a step, their address arithmetic the
 // bound.)  Tensor memory: S0, S1 (128 columns each), O0, O1 (D columns each).  Every wait has a
 // limit; a wait that runs out sets a status bit and the block leaves.
-#include <cuda.h>
 #include <math.h>
 
-#include "sc_attention.cuh"
+#include "sc_tensor.cuh"
 
 namespace sc {
 namespace {
@@ -30,7 +29,6 @@ constexpr int kTThreads = 384;
 constexpr int kLoadWarps = 3;
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
-constexpr int kWaitLimit = 1 << 20;  // tries
 constexpr float kRaise = 8.f;  // log2: how far a score may pass the maximum in use
 
 template <int DP>
@@ -50,136 +48,6 @@ struct TileParams {
     int32_t box_c;         // rows of a box of the own caches
     CUtensorMap kp, vp, kc, vc;
 };
-
-// ---- barriers ----
-__device__ __forceinline__ void bar_init(uint32_t bar, int count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void bar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool bar_try(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    for (int i = 0; i < kWaitLimit; ++i) {
-        if (bar_try(bar, parity)) return true;
-        if (*gave_up) return false;
-    }
-    *gave_up = 1;
-    return false;
-}
-// The same for a whole warp: one lane asks, all get its answer.
-__device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, volatile int* gave_up) {
-    bool ok = true;
-    if ((threadIdx.x & 31) == 0) ok = bar_wait(bar, parity, gave_up);
-    return __shfl_sync(0xffffffffu, ok, 0);
-}
-
-__device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
-                 : "memory");
-}
-
-// One box: columns from x, rows from t of head h of sequence (or page) b.
-__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, uint32_t bar, int x, int t,
-                                         int h, int b) {
-    asm volatile(
-        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes "
-        "[%0], [%1, {%3, %4, %5, %6}], [%2];" ::"r"(dst),
-        "l"(map), "r"(bar), "r"(x), "r"(t), "r"(h), "r"(b)
-        : "memory");
-}
-
-// ---- tensor core and tensor memory ----
-__device__ __forceinline__ void tc_fence_before() {
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile(
-        "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)
-        : "memory");
-}
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
-    const uint32_t acc = add;
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool add) {
-    const uint32_t acc = add;
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
-        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-
-// 32 columns of the warp's 32 lanes.
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
-          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
-          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]),
-          "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(addr));
-}
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
-        "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
-        "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
-        "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr),
-        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-        "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float y;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
-    return y;
-}
-__device__ __forceinline__ void tmem_wait_ld() {
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_wait_st() {
-    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptors of a 128-row tile stored as panels of 64 columns: 128-byte
-// rows, 8 rows a 1024-byte swizzle atom.  Rows as the M or N dimension, columns contracted: atoms
-// follow one another every 1024 bytes (stride offset).  Columns as the N dimension, rows
-// contracted: panels follow every 16 KiB (leading offset), groups of 8 rows every 1024 bytes.
-__device__ __forceinline__ uint64_t desc(uint32_t addr, uint32_t lead, uint32_t stride) {
-    return static_cast<uint64_t>((addr & 0x3FFFF) >> 4) | (static_cast<uint64_t>(lead >> 4) << 16) |
-           (static_cast<uint64_t>(stride >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
-}
 
 // Byte offset of 16-byte chunk c (of a 128-row tile's row r).
 __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
@@ -660,49 +528,6 @@ cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, cudaStream_t s,
     return cudaGetLastError();
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                 const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
-                                 CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion,
-                                 CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult found;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &found) != cudaSuccess ||
-            found != cudaDriverEntryPointSuccess) {
-            cudaGetLastError();
-            f = nullptr;
-        }
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return fn;
-}
-
-// A map of [n3][n2][n1][n0] 16-bit elements (strides in elements) in boxes of 64 columns x `rows`.
-// False where a map cannot say it: the kernel then copies without one.
-bool make_map(CUtensorMap* map, bool half, const void* base, const int64_t (&n)[4], const int64_t (&st)[3],
-              int rows) {
-    const EncodeTiled encode = encode_tiled();
-    if (!encode) return false;
-    cuuint64_t dims[4], strides[3];
-    for (int i = 0; i < 4; ++i) {
-        if (n[i] <= 0 || n[i] > 0xffffffffll) return false;
-        dims[i] = static_cast<cuuint64_t>(n[i]);
-    }
-    for (int i = 0; i < 3; ++i) {
-        // a dimension of one entry has no stride of its own
-        const int64_t s = n[i + 1] == 1 ? (n[0] + 7) / 8 * 8 : st[i];
-        if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
-        strides[i] = static_cast<cuuint64_t>(s * 2);
-    }
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), 1, 1}, step[4] = {1, 1, 1, 1};
-    return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
-                  const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                  CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 }  // namespace
 
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
@@ -712,8 +537,8 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
     p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.direct = direct;
     if (a.P) {
         const int64_t n[4] = {a.D, a.P, a.Hkv, 1};
-        p.tma_p = make_map(&p.kp, half, a.kp, n, {a.kp_t, a.kp_h, 0}, kTokTile) &&
-                  make_map(&p.vp, half, a.vp, n, {a.vp_t, a.vp_h, 0}, kTokTile);
+        p.tma_p = make_map(&p.kp, half, a.kp, n, {a.kp_t, a.kp_h, 0}, kTokTile, 1) &&
+                  make_map(&p.vp, half, a.vp, n, {a.vp_t, a.vp_h, 0}, kTokTile, 1);
     }
     if (per_seq && a.cap) {
         const bool paged = a.page_table != nullptr;
@@ -722,8 +547,8 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
         p.box_c = box;
         const int64_t n[4] = {a.D, paged ? a.page : a.cap, a.Hkv, paged ? a.n_pages : a.B};
         // a box starts at a swizzle atom: 8 rows
-        p.tma_c = box >= 8 && make_map(&p.kc, half, a.kc, n, {a.kc_t, a.kc_h, a.kc_b}, box) &&
-                  make_map(&p.vc, half, a.vc, n, {a.vc_t, a.vc_h, a.vc_b}, box);
+        p.tma_c = box >= 8 && make_map(&p.kc, half, a.kc, n, {a.kc_t, a.kc_h, a.kc_b}, box, 1) &&
+                  make_map(&p.vc, half, a.vc, n, {a.vc_t, a.vc_h, a.vc_b}, box, 1);
     }
     const unsigned n = static_cast<unsigned>(units);
     if (a.D <= 64)

@@ -5,12 +5,14 @@
 // scores by the lower index (NaN counts as minus infinity).  The kept keys, values and scores
 // move together to the front, in their order.
 //
-// select_tokens: one block, or a cluster of up to 8, holds the scores of a (b, h) as ordered
-// 32-bit keys in shared memory (read from HBM once) and finds the last kept key by three radix
-// passes (11, 11 and 10 bits, from the top) over histograms in shared memory, summed over the
-// cluster through distributed shared memory.  A token's place is then the number of kept tokens
-// before it: (those above the key or forced) + min(equal ones before it, equal ones wanted), so
-// one count per warp and one scan are enough and no order depends on timing.
+// select_tokens: one block, or a cluster of up to 16, holds the scores of a (b, h) as ordered
+// 32-bit keys in registers (read from HBM once, every load in flight at once) and finds the last
+// kept key by three radix passes (11, 11 and 10 bits, from the top) over histograms in shared
+// memory, added up in the first block's through distributed shared memory.  A token's place is then
+// the number of kept tokens before it: (those above the key or forced) + min(equal ones before
+// it, equal ones wanted), so one count per warp and one scan are enough and no order depends on
+// timing.  (Keys in shared memory, 512 threads, clusters of 8: 20 us for 128 rows of 8,192 and 50
+// for 8 rows of 131,072.)
 //
 // move_rows / move_rows_in_place: the kept rows, 16 bytes a lane.  In place, row i comes from
 // row idx[i] >= i, so a block that owns a column slice of a (b, h) moves it front to back: a
@@ -25,11 +27,12 @@ namespace cg = cooperative_groups;
 namespace sc {
 namespace {
 
-constexpr int kSelThreads = 512;
+constexpr int kSelThreads = 1024;
 constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kMaxCluster = 8;
-constexpr int kMaxSegment = 49152;  // keys a block: 192 KiB of shared memory
+constexpr int kMaxCluster = 16;
+constexpr int kMaxKeys = 32;  // a thread
+constexpr int kMaxTokens = 393216;
 
 struct SelectParams {
     const float* scores;
@@ -38,7 +41,6 @@ struct SelectParams {
     int32_t* new_lens;
     int32_t* indices;  // [B, H, budget]
     int32_t B, H, S, budget, first, recent;
-    int32_t segment;   // keys a block of the cluster
     int32_t* status;
 };
 
@@ -59,38 +61,45 @@ __device__ __forceinline__ int evict_length(const int32_t* lens, int b, int S, i
     return len;
 }
 
-// Sum over the block of x, and the sum before this thread (exclusive).  Called by every thread.
-__device__ __forceinline__ int block_scan(int x, int& total, int* s_warp) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int v = x;
+__device__ __forceinline__ int warp_scan(int x, int lane) {  // inclusive
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, v, d);
-        if (lane >= d) v += y;
+        const int y = __shfl_up_sync(0xffffffffu, x, d);
+        if (lane >= d) x += y;
     }
-    __syncthreads();
-    if (lane == 31) s_warp[warp] = v;
-    __syncthreads();
-    int before = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < kSelWarps; ++w) {
-        const int y = s_warp[w];
-        if (w < warp) before += y;
-        all += y;
-    }
-    total = all;
-    return before + v - x;
+    return x;
 }
 
+// The sum of x over the warps before this one (x: one value a warp) and over all.  Called by
+// every thread; s_warp is free again after the next block-wide barrier.
+__device__ __forceinline__ int warps_before(int x, int& total, int* s_warp) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (lane == 0) s_warp[warp] = x;
+    __syncthreads();
+    const int v = warp_scan(s_warp[lane], lane);
+    total = __shfl_sync(0xffffffffu, v, 31);
+    return __shfl_sync(0xffffffffu, v, warp) - x;
+}
+
+// KPT keys a thread: warp w of rank r holds tokens [(r * 32 + w) * 32 KPT, + 32 KPT), key j of lane l
+// being token 32 j + l of them.
+template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_constant__ SelectParams p) {
-    extern __shared__ __align__(16) uint32_t s_keys[];
     __shared__ uint32_t s_hist[kBins];
-    __shared__ int s_warp[kSelWarps];
+    __shared__ int s_warp[3][kSelWarps];
     __shared__ int s_pick[2];    // digit, equal ones still wanted
     __shared__ int s_counts[2];  // this block's kept-for-sure and equal tokens
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank());
     const int ranks = static_cast<int>(cluster.num_blocks());
+    auto sync_all = [&] {
+        if (ranks > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+    };
+    // The cluster's histogram is the first block's.
+    uint32_t* all_hist = cluster.map_shared_rank(s_hist, 0);
     const int row = blockIdx.x / ranks;
     const int b = row / p.H, h = row - b * p.H;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -108,10 +117,17 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
 
     // Free tokens are [lo, hi); budget >= first + recent, so some of them go.
     const int lo = min(p.first, len), hi = max(lo, len - p.recent);
-    const int base = rank * p.segment;
-    const int f0 = max(base, lo) - base, f1 = min(base + p.segment, hi) - base;  // free, local
-    const float* scores = p.scores + b * p.s_b + h * p.s_h + base;
-    for (int i = f0 + threadIdx.x; i < f1; i += kSelThreads) s_keys[i] = order_key(scores[i]);
+    const int t0 = (rank * kSelWarps + warp) * 32 * KPT + lane;
+    const float* scores = p.scores + b * p.s_b + h * p.s_h;
+    float raw[KPT];
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+        const int t = t0 + 32 * j;
+        raw[j] = t >= lo && t < hi ? __ldg(scores + t) : 0.f;
+    }
+    uint32_t keys[KPT];
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) keys[j] = order_key(raw[j]);
 
     int want = n_new - lo - (len - hi);  // free tokens that stay
     uint32_t key = 0;                    // the last kept key's bits found so far
@@ -122,89 +138,96 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
         const int top = shift;
         shift -= bits;
         const uint32_t digits = (1u << bits) - 1u;
-        __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kSelThreads) s_hist[i] = 0;
         __syncthreads();
-        for (int i = f0 + threadIdx.x; i < f1; i += kSelThreads) {
-            const uint32_t x = s_keys[i];
-            if (top == 32 || (x >> top) == above) atomicAdd(&s_hist[(x >> shift) & digits], 1u);
-        }
-        cluster.sync();
-        // Bins in descending order, four a thread, summed over the cluster.
-        int mine[kBins / kSelThreads], sum = 0;
 #pragma unroll
-        for (int j = 0; j < kBins / kSelThreads; ++j) {
-            const int bin = kBins - 1 - (threadIdx.x * (kBins / kSelThreads) + j);
-            int n = 0;
-            for (int r = 0; r < ranks; ++r)
-                n += static_cast<int>(cluster.map_shared_rank(s_hist, r)[bin]);
-            mine[j] = n;
-            sum += n;
+        for (int j = 0; j < KPT; ++j) {
+            const int t = t0 + 32 * j;
+            if (t >= lo && t < hi && (top == 32 || (keys[j] >> top) == above))
+                atomicAdd(&s_hist[(keys[j] >> shift) & digits], 1u);
         }
-        int total;
-        int before = block_scan(sum, total, s_warp);
-        if (want > 0 && before < want && before + sum >= want) {
+        if (ranks > 1) {
+            __syncthreads();
+            uint32_t mine[kBins / kSelThreads];
 #pragma unroll
-            for (int j = 0; j < kBins / kSelThreads; ++j) {
-                if (before < want && before + mine[j] >= want) {
-                    s_pick[0] = kBins - 1 - (threadIdx.x * (kBins / kSelThreads) + j);
-                    s_pick[1] = want - before;
-                }
-                before += mine[j];
+            for (int j = 0; j < kBins / kSelThreads; ++j) mine[j] = s_hist[threadIdx.x + j * kSelThreads];
+            cluster.sync();  // the first block's own counts are complete, too
+            if (rank != 0) {
+#pragma unroll
+                for (int j = 0; j < kBins / kSelThreads; ++j)
+                    if (mine[j]) atomicAdd(&all_hist[threadIdx.x + j * kSelThreads], mine[j]);
             }
         }
-        cluster.sync();  // also: nobody reads this histogram any more
-        if (want > 0) {
-            key |= static_cast<uint32_t>(s_pick[0]) << shift;
-            want = s_pick[1];
+        sync_all();
+        if (rank == 0) {
+            // Bins in descending order, two a thread.
+            static_assert(kBins == 2 * kSelThreads, "two bins a thread");
+            const int bin = kBins - 1 - 2 * threadIdx.x;
+            const int n0 = static_cast<int>(s_hist[bin]), n1 = static_cast<int>(s_hist[bin - 1]);
+            const int upto = warp_scan(n0 + n1, lane);
+            int total;
+            const int before =
+                warps_before(__shfl_sync(0xffffffffu, upto, 31), total, s_warp[0]) + upto - n0 - n1;
+            if (want > 0 && before < want && before + n0 + n1 >= want) {
+                const bool second = before + n0 < want;
+                s_pick[0] = second ? bin - 1 : bin;
+                s_pick[1] = want - before - (second ? n0 : 0);
+            }
         }
+        sync_all();
+        if (want > 0) {
+            const int* pick = cluster.map_shared_rank(s_pick, 0);
+            const int digit = pick[0], left = pick[1];
+            key |= static_cast<uint32_t>(digit) << shift;
+            want = left;
+        }
+        if (ranks > 1) cluster.sync();  // everybody has read the choice and the histogram
     }
     // Free tokens above `key` stay, and the first `want` equal to it (want = 0: none do).
     const int wanted = want;
     const bool none = n_new - lo - (len - hi) <= 0;
 
-    // Each warp owns a run of the segment.
-    const int s0 = base, s1 = min(base + p.segment, len);
-    const int n_seg = max(0, s1 - s0);
-    const int run = ((n_seg + kSelWarps - 1) / kSelWarps + 31) / 32 * 32;
-    const int w0 = warp * run, w1 = min(w0 + run, n_seg);
-    auto kind = [&](int i) -> int {  // 0 goes, 1 stays, 2 equal
-        const int t = base + i;
+    auto kind = [&](int j) -> int {  // 0 goes, 1 stays, 2 equal
+        const int t = t0 + 32 * j;
+        if (t >= len) return 0;
         if (t < lo || t >= hi) return 1;
         if (none) return 0;
-        const uint32_t x = s_keys[i];
-        return x > key ? 1 : x == key ? 2 : 0;
+        return keys[j] > key ? 1 : keys[j] == key ? 2 : 0;
     };
     int stay = 0, equal = 0;
-    for (int i = w0 + lane; i < w0 + run; i += 32) {
-        const int k = i < w1 ? kind(i) : 0;
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+        const int k = kind(j);
         stay += __popc(__ballot_sync(0xffffffffu, k == 1));
         equal += __popc(__ballot_sync(0xffffffffu, k == 2));
     }
     int total_stay, total_equal;
-    const int stay_before = block_scan(lane == 0 ? stay : 0, total_stay, s_warp);
-    const int equal_before = block_scan(lane == 0 ? equal : 0, total_equal, s_warp);
-    if (threadIdx.x == 0) {
-        s_counts[0] = total_stay;
-        s_counts[1] = total_equal;
+    int g = warps_before(stay, total_stay, s_warp[1]), e = warps_before(equal, total_equal, s_warp[2]);
+    if (ranks > 1) {
+        if (threadIdx.x == 0) {
+            s_counts[0] = total_stay;
+            s_counts[1] = total_equal;
+        }
+        cluster.sync();
+        int cg_ = 0, ce = 0;  // a lane a rank before this one
+        if (lane < rank) {
+            const int* c = cluster.map_shared_rank(s_counts, lane);
+            cg_ = c[0], ce = c[1];
+        }
+        g += __reduce_add_sync(0xffffffffu, cg_);
+        e += __reduce_add_sync(0xffffffffu, ce);
     }
-    cluster.sync();
-    int g = __shfl_sync(0xffffffffu, stay_before, 0), e = __shfl_sync(0xffffffffu, equal_before, 0);
-    for (int r = 0; r < rank; ++r) {
-        const int* c = cluster.map_shared_rank(s_counts, r);
-        g += c[0];
-        e += c[1];
-    }
-    for (int i = w0 + lane; i < w0 + run; i += 32) {
-        const int k = i < w1 ? kind(i) : 0;
+#pragma unroll
+    for (int j = 0; j < KPT; ++j) {
+        const int k = kind(j);
         const uint32_t bs = __ballot_sync(0xffffffffu, k == 1), be = __ballot_sync(0xffffffffu, k == 2);
         const uint32_t below = (1u << lane) - 1u;
         const int gb = g + __popc(bs & below), eb = e + __popc(be & below);
-        if (k == 1 || (k == 2 && eb < wanted)) idx[gb + min(eb, wanted)] = base + i;
+        if (k == 1 || (k == 2 && eb < wanted)) idx[gb + min(eb, wanted)] = t0 + 32 * j;
         g += __popc(bs);
         e += __popc(be);
     }
-    cluster.sync();  // no block leaves while another reads its shared memory
+    if (ranks > 1) cluster.sync();  // no block leaves while another reads its shared memory
 }
 
 // ---------------------------------------------------------------------------------------
@@ -315,15 +338,31 @@ __global__ void __launch_bounds__(kMoveThreads) move_rows_in_place(const __grid_
     }
 }
 
-cudaError_t allow_select() {
+template <int KPT>
+cudaError_t launch_select(const SelectParams& p, int ranks, cudaStream_t s, bool load_only) {
     static std::atomic<uint64_t> done{0};
-    return allow_shared_memory(reinterpret_cast<const void*>(select_tokens), kMaxSegment * 4, done);
+    cudaError_t e = allow_clusters(reinterpret_cast<const void*>(select_tokens<KPT>), done);
+    if (e != cudaSuccess || load_only) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(p.B * p.H * ranks));
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = static_cast<unsigned>(ranks);
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, select_tokens<KPT>, p);
 }
 
 }  // namespace
 
 cudaError_t preload_evict_kernels() {
-    cudaError_t e = allow_select();
+    SelectParams p{};
+    cudaError_t e = launch_select<8>(p, 1, nullptr, true);
+    if (e == cudaSuccess) e = launch_select<16>(p, 1, nullptr, true);
+    if (e == cudaSuccess) e = launch_select<kMaxKeys>(p, 1, nullptr, true);
     cudaFuncAttributes attr;
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, move_rows);
     if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, move_rows_in_place);
@@ -358,9 +397,9 @@ extern "C" int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache
                          (long long)keep_first, (long long)keep_recent, (long long)budget);
     if (row_bytes % 16 != 0)
         return set_error(SC_ERR_UNSUPPORTED, "rows of %d bytes: a multiple of 16", row_bytes);
-    if (cache_len > static_cast<int64_t>(kMaxSegment) * kMaxCluster)
+    if (cache_len > kMaxTokens)
         return set_error(SC_ERR_UNSUPPORTED, "caches of %lld tokens: at most %d", (long long)cache_len,
-                         kMaxSegment * kMaxCluster);
+                         kMaxTokens);
     if (budget >= (int64_t(1) << 24) || size_product(budget, row_bytes / 16) >= (int64_t(1) << 31) ||
         size_product(batch, n_heads) > 65535)
         return set_error(SC_ERR_INVALID_ARGUMENT, "too many rows in one call; split it");
@@ -392,26 +431,16 @@ extern "C" int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache
     sp.budget = static_cast<int32_t>(budget);
     sp.first = static_cast<int32_t>(keep_first), sp.recent = static_cast<int32_t>(keep_recent);
     sp.status = status;
-    // A cluster where one block cannot hold the scores, or where there are few long rows.
+    // A cluster where there are fewer rows than SMs, down to 16 keys a thread (8 rows of 131,072:
+    // 26.7 us; 8 keys and twice the blocks 29.0, 32 keys 43.4), or where one block cannot hold a
+    // row's keys.
     int ranks = 1;
-    while (ranks < kMaxCluster && (cache_len > static_cast<int64_t>(ranks) * kMaxSegment ||
-                                   (rows * ranks * 2 <= 148 && cache_len > static_cast<int64_t>(ranks) * 4096)))
+    auto per_thread = [&] { return (cache_len + ranks * kSelThreads - 1) / (ranks * kSelThreads); };
+    while (ranks < kMaxCluster && (per_thread() > kMaxKeys || (rows * ranks * 2 <= 148 && per_thread() > 16)))
         ranks *= 2;
-    sp.segment = static_cast<int32_t>(((cache_len + ranks - 1) / ranks + 31) / 32 * 32);
-    cudaError_t e = allow_select();
-    if (e != cudaSuccess) return cuda_error(e, "eviction set-up");
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(rows * ranks));
-    cfg.blockDim = dim3(kSelThreads);
-    cfg.dynamicSmemBytes = static_cast<size_t>(sp.segment) * 4;
-    cfg.stream = st;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = static_cast<unsigned>(ranks);
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, select_tokens, sp);
+    cudaError_t e = per_thread() <= 8    ? launch_select<8>(sp, ranks, st, false)
+                    : per_thread() <= 16 ? launch_select<16>(sp, ranks, st, false)
+                                         : launch_select<kMaxKeys>(sp, ranks, st, false);
     if (e != cudaSuccess) return cuda_error(e, "eviction select launch");
     if (budget == 0) return ok();
 

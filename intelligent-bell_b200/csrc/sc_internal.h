@@ -27,6 +27,9 @@ int32_t cuda_error(cudaError_t e, const char* what);
 // remembers the devices that have been set, so only a device's first launch pays for the call.
 cudaError_t allow_shared_memory(const void* kernel, int bytes, std::atomic<uint64_t>& done);
 
+// Let `kernel` run in clusters of more than 8 blocks; `done` as above.
+cudaError_t allow_clusters(const void* kernel, std::atomic<uint64_t>& done);
+
 // Streaming multiprocessor count of the current device (cached per device).
 int sm_count();
 

@@ -25,7 +25,7 @@
 namespace sc {
 namespace {
 
-constexpr int kRThreads = 128;
+constexpr int kRThreads = 256;
 constexpr int kMaxRotary = 512;       // frequencies travel as kernel parameters
 constexpr int kMaxTokensPerBlock = 32;
 constexpr int kTableEntries = 2048;   // float2 entries of the block's table
@@ -381,8 +381,10 @@ extern "C" int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_head
         int tokens = room / p.chunk;
         if (tokens > kMaxTokensPerBlock) tokens = kMaxTokensPerBlock;
         if (half && tokens > kTableEntries / half) tokens = kTableEntries / half;
-        p.tokens = tokens < 1 ? 1 : tokens;
         const int64_t all = static_cast<int64_t>(batch) * n_tokens;
+        // few tokens: over as many SMs as there are
+        if (tokens > (all + 147) / 148) tokens = static_cast<int>((all + 147) / 148);
+        p.tokens = tokens < 1 ? 1 : tokens;
         grid = dim3(static_cast<unsigned>((all + p.tokens - 1) / p.tokens), parts);
     } else {
         const int64_t work = rows * ((head_dim + 1) / 2);

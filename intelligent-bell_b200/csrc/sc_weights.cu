@@ -13,7 +13,7 @@
 #include <limits.h>
 #include <math.h>
 
-#include "sc_attention.cuh"
+#include "sc_weights.cuh"
 
 namespace sc {
 namespace {
@@ -23,27 +23,6 @@ constexpr int kWThreads = 32 * kWWarps;
 constexpr int kWTile = 32;                     // tokens a warp's tile
 constexpr int kWBlock = kWTile * kWWarps;      // tokens a block's step
 
-struct WeightParams {
-    const void* q;
-    int64_t q_t, q_h;
-    const void* k;
-    int64_t k_b, k_t, k_h;
-    const float* lse;  // [N, Hq]
-    int64_t lse_t, lse_h;
-    const float* scores;
-    int64_t s_b, s_h;
-    float* out;
-    int64_t o_b, o_h;
-    const int32_t* cache_lens;
-    const int32_t* cu_q;
-    int32_t N, B, Hq, Hkv, G, D, nq, S;
-    int32_t causal;
-    int32_t parts, chunk;  // blocks a (b, h), tokens a block
-    int32_t row_room;      // queries that fit in shared memory (a multiple of 16)
-    FastDiv div_G;
-    float scale_log2;
-    int32_t* status;
-};
 
 template <int DP>
 __device__ __forceinline__ uint32_t w_chunk_at(int r, int c) {
@@ -245,6 +224,7 @@ cudaError_t preload_weights_type() {
 cudaError_t preload_weights_kernels() {
     cudaError_t e = preload_weights_type<__half>();
     if (e == cudaSuccess) e = preload_weights_type<__nv_bfloat16>();
+    if (e == cudaSuccess) e = preload_weight_tile_kernels();
     return e;
 }
 
@@ -303,21 +283,25 @@ extern "C" int32_t sc_accumulate_attention_weights(
     p.div_G = make_fastdiv(static_cast<uint32_t>(p.G));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
     p.status = status;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    bool taken = false;
+    cudaError_t e = launch_weight_tiles(p, dtype == SC_DTYPE_F16, s, &taken);
+    if (e != cudaSuccess) return cuda_error(e, "attention weights launch");
+    if (taken) return ok();
     const int64_t most = size_product(p.nq, p.G);
     const int room = head_dim > 128 ? 128 : 256;
     p.row_room = most >= room ? room : most < 16 ? 16 : static_cast<int32_t>((most + 15) / 16 * 16);
     // Two blocks an SM; two rounds of them.
     const double total = static_cast<double>(batch) * kv_heads * cache_len;
-    double chunk = ceil(total / (148.0 * 2 * 2) / kWBlock) * kWBlock;
+    double chunk = ceil(total / (148.0 * 2 * 4) / kWBlock) * kWBlock;
     if (chunk > cache_len) chunk = ceil(static_cast<double>(cache_len) / kWBlock) * kWBlock;
     p.chunk = static_cast<int32_t>(chunk);
     p.parts = static_cast<int32_t>((cache_len + p.chunk - 1) / p.chunk);
     const int64_t blocks = size_product(p.parts, batch, kv_heads);
     if (blocks >= (int64_t(1) << 31))
         return set_error(SC_ERR_INVALID_ARGUMENT, "%lld blocks in one call; split it", (long long)blocks);
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = dtype == SC_DTYPE_F16 ? launch_weights_dp<__half>(p, blocks, s)
-                                                : launch_weights_dp<__nv_bfloat16>(p, blocks, s);
+    e = dtype == SC_DTYPE_F16 ? launch_weights_dp<__half>(p, blocks, s)
+                              : launch_weights_dp<__nv_bfloat16>(p, blocks, s);
     if (e != cudaSuccess) return cuda_error(e, "attention weights launch");
     return ok();
 }

@@ -378,7 +378,8 @@ def _check_weights(ref, c, lse, scores, out, causal=True):
 @pytest.mark.parametrize("q_lens,lens,hq,hk,d,cap", [
     ([1], [1], 1, 1, 64, 1), ([1, 1, 1], [0, 140, 33], 8, 2, 128, 150), ([1] * 4, [7, 64, 129, 2], 28, 4, 128, 130),
     ([5, 5], [3, 80], 6, 2, 80, 80), ([20, 1, 33], [60, 9, 33], 8, 1, 64, 70), ([3], [50], 10, 2, 256, 61),
-    ([70, 70], [90, 200], 8, 2, 128, 200)])
+    ([70, 70], [90, 200], 8, 2, 128, 200), ([1] * 9, [1000, 0, 256, 257, 5, 300, 128, 129, 700], 14, 2, 128, 1000),
+    ([150, 3], [1200, 700], 12, 4, 64, 1200), ([300], [290], 5, 1, 128, 310), ([40], [900], 7, 1, 40, 1000)])
 def test_weights_match_the_oracle(scb, ref, dtype, q_lens, lens, hq, hk, d, cap):
     c, lse, scores = _weights_case(scb, 31, dtype, q_lens, lens, hq, hk, d, cap)
     out = torch.full_like(scores, -1.0)
@@ -389,6 +390,18 @@ def test_weights_match_the_oracle(scb, ref, dtype, q_lens, lens, hq, hk, d, cap)
     mine = scores.clone()
     assert scb.accumulate_attention_weights(c.q, c.kc, lse, mine, c.lens, q_lens=c.q_lens) is mine
     assert bits_equal(mine, out)
+
+
+def test_weights_of_pages_apart_and_expanded_heads(scb, ref):
+    """Layouts that tensor maps cannot say, and more sequences than are counted in shared memory."""
+    c, lse, scores = _weights_case(scb, 35, torch.bfloat16, [2, 2], [60, 31], 4, 2, 64, 64)
+    c.kc = c.kc[:, :, :1].expand(-1, -1, 2, -1)
+    got = scb.accumulate_attention_weights(c.q, c.kc, lse, scores, c.lens_t(), out=torch.empty_like(scores))
+    _check_weights(ref, c, lse, scores, got)
+    b = 1030
+    c, lse, scores = _weights_case(scb, 36, torch.float16, [1] * b, [i % 9 for i in range(b)], 1, 1, 64, 8)
+    got = scb.accumulate_attention_weights(c.q, c.kc, lse, scores, c.lens_t(), out=torch.empty_like(scores))
+    _check_weights(ref, c, lse, scores, got)
 
 
 def test_weights_of_a_prefix_sum_to_the_batch(scb, ref):
