@@ -10,7 +10,7 @@
 // the exponentials bound it: 16 a clock and SM against 4,096 multiplications).
 //
 // Roles: warps 0-3 and 4-7 the weights of tile 0 and 1, warp 8 the copies (TMA), warp 9 the
-// products.  Each tile has two score buffers in tensor memory.
+// products, warps 10 and 11 the scores of tokens that are not in use.  Each tile has two score buffers in tensor memory.
 #include <limits.h>
 #include <math.h>
 
@@ -20,8 +20,9 @@
 namespace sc {
 namespace {
 
-constexpr int kThreadsW = 320;
+constexpr int kThreadsW = 384;
 constexpr int kTile = 128;           // tokens
+constexpr int kPiece = 1024;         // scores copied by a warp at a time
 constexpr int kMaxSequences = 1024;  // their lengths are held in shared memory
 
 template <int DP, int NR>
@@ -38,6 +39,7 @@ struct WeighParams {
     WeightParams w;
     int32_t chunk_tokens;  // tokens of q a chunk
     FastDiv div_chunk;
+    int32_t pieces;        // of a score row, for the copy
     CUtensorMap k, q;
 };
 
@@ -145,43 +147,79 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = s_tmem;
-    const int per_head = s_first[p.B];
-    const int n_units = per_head * p.Hkv;
+    // Units in the order of sequences, their heads, their tokens; a block takes a run of them.
+    const int n_units = s_first[p.B] * p.Hkv;
+    const int run = (n_units + gridDim.x - 1) / gridDim.x;
+    const int u0 = min(n_units, static_cast<int>(blockIdx.x) * run), u1 = min(n_units, u0 + run);
 
     struct Unit {
         int b, h, t0, len, tok0, n_tok, n_t, c0, c1;
     };
-    auto unit = [&](int u) {
-        Unit x;
-        x.h = u / per_head;
-        const int g = u - x.h * per_head;
-        int lo = 0, hi = p.B;  // the last sequence whose first unit is not behind g
+    auto settle = [&](Unit& x) {  // what follows from sequence and first token
+        x.n_t = x.t0 + kTile < x.len ? 2 : 1;
+        x.c1 = static_cast<int>(fdiv(x.n_tok + wp.chunk_tokens - 1, wp.div_chunk));
+        // queries before the first that sees token t0 see nothing of the unit
+        const int j = p.causal ? x.t0 - (x.len - x.n_tok) : 0;
+        x.c0 = j > 0 ? static_cast<int>(fdiv(j, wp.div_chunk)) : 0;
+    };
+    auto first_unit = [&] {
+        Unit x{};
+        if (u0 >= u1) return x;
+        int lo = 0, hi = p.B;  // the last sequence whose first unit is not behind u0
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (s_first[mid] <= g)
+            if (s_first[mid] * p.Hkv <= u0)
                 lo = mid;
             else
                 hi = mid;
         }
         x.b = lo;
-        x.t0 = (g - s_first[lo]) * 2 * kTile;
         x.len = s_len[lo];
+        const int per_head = s_first[lo + 1] - s_first[lo], in = u0 - s_first[lo] * p.Hkv;
+        x.h = in / per_head;
+        x.t0 = (in - x.h * per_head) * 2 * kTile;
         tokens_of(lo, x.tok0, x.n_tok);
-        x.n_t = x.t0 + kTile < x.len ? 2 : 1;
-        x.c1 = (x.n_tok + wp.chunk_tokens - 1) / wp.chunk_tokens;
-        // queries before the first that sees token t0 see nothing of the unit
-        const int j = p.causal ? x.t0 - (x.len - x.n_tok) : 0;
-        x.c0 = j > 0 ? static_cast<int>(fdiv(j, wp.div_chunk)) : 0;
+        settle(x);
         return x;
+    };
+    auto next_unit = [&](Unit& x) {
+        x.t0 += 2 * kTile;
+        if (x.t0 >= x.len) {
+            x.t0 = 0;
+            if (++x.h == p.Hkv) {
+                x.h = 0;
+                do ++x.b;
+                while (x.b < p.B && s_len[x.b] == 0);
+                if (x.b >= p.B) return;
+                x.len = s_len[x.b];
+                tokens_of(x.b, x.tok0, x.n_tok);
+            }
+        }
+        settle(x);
     };
 
     if (warp == 8) {
         // ---- copies ----
         int kc = 0, qc = 0;
         bool alive = true;
-        for (int u = blockIdx.x; u < n_units && alive; u += gridDim.x) {
-            const Unit x = unit(u);
+        Unit x = first_unit();
+        for (int u = u0; u < u1 && alive; ++u, next_unit(x)) {
             if (x.c0 >= x.c1) continue;
+            // A chunk's lse, asked for before the copies are waited for.
+            constexpr int PL = (NR + 31) / 32;
+            float lse[PL];
+            auto ask = [&](int c) {
+#pragma unroll
+                for (int i = 0; i < PL; ++i) {
+                    const int r = i * 32 + lane;
+                    const int j = static_cast<int>(fdiv(r, p.div_G)), g = r - j * p.G;
+                    const int jj = c * wp.chunk_tokens + j;
+                    lse[i] = r < NR && j < wp.chunk_tokens && jj < x.n_tok
+                                 ? p.lse[(x.tok0 + jj) * p.lse_t + (x.h * p.G + g) * p.lse_h]
+                                 : kNegInf;
+                }
+            };
+            ask(x.c0);
             for (int t = 0; t < x.n_t && alive; ++t, ++kc) {
                 const int s = kc % KST;
                 alive = bar_wait_warp(k_empty(s), (kc / KST & 1) ^ 1, gave_up);
@@ -199,24 +237,19 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                 const int j0 = c * wp.chunk_tokens;
                 int least = INT_MAX;
 #pragma unroll
-                for (int i = 0; i < (NR + 31) / 32; ++i) {
+                for (int i = 0; i < PL; ++i) {
                     const int r = i * 32 + lane;
                     if (r < NR) {
-                        const int j = static_cast<int>(fdiv(r, p.div_G)), g = r - j * p.G;
-                        float x2 = 0.f;
-                        int lim = INT_MIN;  // no row, or another sequence's
-                        if (j < wp.chunk_tokens && j0 + j < x.n_tok) {
-                            const float l = p.lse[(x.tok0 + j0 + j) * p.lse_t + (x.h * p.G + g) * p.lse_h];
-                            if (l != kNegInf) {  // a row that saw nothing gives nothing
-                                x2 = -l * 1.4426950408889634f;
-                                lim = p.causal ? x.len - x.n_tok + j0 + j + 1 : INT_MAX;
-                            }
-                        }
-                        s_neg_lse[s][r] = x2;
+                        // no row, another sequence's, or one that saw nothing: it gives nothing
+                        const bool is = lse[i] != kNegInf;
+                        const int j = static_cast<int>(fdiv(r, p.div_G));
+                        const int lim = !is ? INT_MIN : p.causal ? x.len - x.n_tok + j0 + j + 1 : INT_MAX;
+                        s_neg_lse[s][r] = is ? -lse[i] * 1.4426950408889634f : 0.f;
                         s_lim[s][r] = lim;
                         least = min(least, lim);
                     }
                 }
+                if (c + 1 < x.c1) ask(c + 1);
                 least = __reduce_min_sync(0xffffffffu, least);
                 if (lane == 0) {
                     s_all_seen[s] = least;
@@ -237,8 +270,8 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
             const uint64_t k_desc = desc(s_k, 16, 1024), q_desc = desc(s_q, 16, 1024);
             int kc = 0, qc = 0, it[2] = {0, 0};
             bool alive = true;
-            for (int u = blockIdx.x; u < n_units && alive; u += gridDim.x) {
-                const Unit x = unit(u);
+            Unit x = first_unit();
+            for (int u = u0; u < u1 && alive; ++u, next_unit(x)) {
                 if (x.c0 >= x.c1) continue;
                 for (int c = x.c0; c < x.c1 && alive; ++c, ++qc) {
                     const int qs = qc % QST;
@@ -268,6 +301,27 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
             }
         }
         __syncwarp();
+    } else if (warp >= 10) {
+        // ---- tokens not in use keep their score ----
+        if (p.out != p.scores) {
+            const int rows = p.B * p.Hkv;
+            for (int piece = blockIdx.x * 2 + warp - 10; piece < rows * wp.pieces; piece += gridDim.x * 2) {
+                const int row = piece / wp.pieces, b = row / p.Hkv, h = row - b * p.Hkv;
+                const int i0 = (piece - row * wp.pieces) * kPiece, i1 = min(i0 + kPiece, p.S);
+                const float* in = p.scores + b * p.s_b + h * p.s_h;
+                float* out = p.out + b * p.o_b + h * p.o_h;
+                const int lo = max(i0, s_len[b]);
+                for (int i = lo + lane; i < i1; i += 32 * 16) {
+                    float v[16];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (i + k * 32 < i1) v[k] = in[i + k * 32];
+#pragma unroll
+                    for (int k = 0; k < 16; ++k)
+                        if (i + k * 32 < i1) out[i + k * 32] = v[k];
+                }
+            }
+        }
     } else {
         // ---- weights: one thread a token ----
         const int t = warp >> 2;
@@ -275,13 +329,22 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
         const float2 mul2 = make_float2(p.scale_log2, p.scale_log2);
         int qc = 0, it = 0;
         bool alive = true;
-        for (int u = blockIdx.x; u < n_units && alive; u += gridDim.x) {
-            const Unit x = unit(u);
-            const int tok = x.t0 + t * kTile + (warp & 3) * 32 + lane;
+        const int mine = t * kTile + (warp & 3) * 32 + lane;
+        auto score_of = [&](const Unit& x) {
+            return x.t0 + mine < x.len ? p.scores[x.b * p.s_b + x.h * p.s_h + x.t0 + mine] : 0.f;
+        };
+        Unit x = first_unit();
+        float before = u0 < u1 ? score_of(x) : 0.f;
+        for (int u = u0; u < u1 && alive; ++u) {
+            const int tok = x.t0 + mine;
             const int last = x.t0 + t * kTile + (warp & 3) * 32 + 31;
-            const float* in = p.scores + x.b * p.s_b + x.h * p.s_h;
-            float* out = p.out + x.b * p.o_b + x.h * p.o_h;
-            const float before = tok < x.len ? in[tok] : 0.f;
+            // the next unit's scores are on their way during this one
+            Unit next = x;
+            float next_before = 0.f;
+            if (u + 1 < u1) {
+                next_unit(next);
+                next_before = score_of(next);
+            }
             float2 acc = make_float2(0.f, 0.f), acc2 = acc;
             for (int c = x.c0; c < x.c1; ++c, ++qc) {
                 const int qs = qc % QST;
@@ -330,16 +393,10 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                 __syncwarp();
                 if (lane == 0) bar_arrive(q_empty(qs));
             }
-            if (alive && tok < x.len) out[tok] = before + ((acc.x + acc.y) + (acc2.x + acc2.y));
-        }
-        // Tokens not in use keep their score.
-        if (p.out != p.scores) {
-            for (int row = blockIdx.x; row < p.B * p.Hkv; row += gridDim.x) {
-                const int b = row / p.Hkv, h = row - b * p.Hkv;
-                const float* in = p.scores + b * p.s_b + h * p.s_h;
-                float* out = p.out + b * p.o_b + h * p.o_h;
-                for (int i = s_len[b] + threadIdx.x; i < p.S; i += 256) out[i] = in[i];
-            }
+            if (alive && tok < x.len)
+                p.out[x.b * p.o_b + x.h * p.o_h + tok] = before + ((acc.x + acc.y) + (acc2.x + acc2.y));
+            x = next;
+            before = next_before;
         }
     }
     tc_fence_before();
@@ -403,6 +460,7 @@ cudaError_t launch_weight_tiles(const WeightParams& w, bool half, cudaStream_t s
     p.w = w;
     const int nr = size_product(w.nq, w.G) <= 16 ? 16 : 128;
     p.chunk_tokens = nr / w.G < w.nq ? nr / w.G : w.nq;
+    p.pieces = (w.S + kPiece - 1) / kPiece;
     p.div_chunk = make_fastdiv(static_cast<uint32_t>(p.chunk_tokens));
     const int64_t nk[4] = {w.D, w.S, w.Hkv, w.B}, nqs[4] = {w.D, w.G, w.N, w.Hkv};
     if (!make_map(&p.k, half, w.k, nk, {w.k_t, w.k_h, w.k_b}, kTile, 1) ||
