@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = s_tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, s_tmem, 0);
     auto copies_done = [&](uint32_t bar) {
         cp_async_wait<0>();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
@@ -295,59 +295,69 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         }
     } else if (warp == 11) {
         // ---- products ----
-        if (lane == 0) {
-            constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
-            constexpr uint32_t id_common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
-            constexpr uint32_t id_qk = id_common | ((128u >> 3) << 17);
-            constexpr uint32_t id_pv = id_common | ((static_cast<uint32_t>(DP) >> 3) << 17) | (1u << 16);
-            // Descriptors of the first step; a step's address is added to the low word.
-            const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_ring, 16, 1024),
-                           v_desc = desc(s_ring, 16384, 1024);
-            auto qk = [&](int q, int stage) {
-                const uint64_t qd = q_desc + static_cast<uint32_t>(q * (TILE / 16));
-                const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (TILE / 16));
+        // The warp stays converged, so addresses and descriptors are uniform; one lane issues.
+        constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
+        constexpr uint32_t id_common = (1u << 4) | (fmt << 7) | (fmt << 10) | ((128u >> 4) << 24);
+        constexpr uint32_t id_qk = id_common | ((128u >> 3) << 17);
+        constexpr uint32_t id_pv = id_common | ((static_cast<uint32_t>(DP) >> 3) << 17) | (1u << 16);
+        // Descriptors of the first step; a step's address is added to the low word.
+        const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_ring, 16, 1024),
+                       v_desc = desc(s_ring, 16384, 1024);
+        const bool leader = elect_one();
+        auto qk = [&](int q, int stage) {
+            const uint64_t qd = q_desc + static_cast<uint32_t>(q * (TILE / 16));
+            const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (TILE / 16));
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {
-                    const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
-                    mma_ss(tmem + q * 128, qd + off, kd + off, id_qk, kk > 0);
-                }
-            };
-            auto pv = [&](int q, int stage, bool add) {
-                const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (TILE / 16));
-#pragma unroll
-                for (int kk = 0; kk < kTokTile / 16; ++kk)
-                    mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, vd + kk * (2048 / 16), id_pv,
-                           add || kk > 0);
-            };
-            bool alive = bar_wait(q_full, 0, gave_up) && bar_wait(full(0), 0, gave_up);
-            if (alive) {
-                for (int q = 0; q < n_q; ++q) {
-                    qk(q, 0);
-                    tc_commit(s_full(q));
-                }
-                tc_commit(empty(0));
+            for (int kk = 0; kk < DP / 16; ++kk) {
+                const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
+                mma_ss(tmem + q * 128, qd + off, kd + off, id_qk, kk > 0);
             }
-            for (int i = 0; i < n_tiles && alive; ++i) {
-                const int vl = 2 * i + 1, kl = 2 * i + 2;  // loads V_i, K_{i+1}
-                alive = bar_wait(full(vl % NST), (vl / NST) & 1, gave_up);
-                for (int q = 0; q < n_q && alive; ++q) {
-                    alive = bar_wait(p_full(q), i & 1, gave_up);
-                    if (!alive) break;
-                    tc_fence_after();
-                    pv(q, vl % NST, i > 0);
+        };
+        auto pv = [&](int q, int stage, bool add) {
+            const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (TILE / 16));
+#pragma unroll
+            for (int kk = 0; kk < kTokTile / 16; ++kk)
+                mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, vd + kk * (2048 / 16), id_pv,
+                       add || kk > 0);
+        };
+        bool alive = bar_wait_all(q_full, 0, gave_up) && bar_wait_all(full(0), 0, gave_up);
+        if (alive && leader) {
+            for (int q = 0; q < n_q; ++q) {
+                qk(q, 0);
+                tc_commit(s_full(q));
+            }
+            tc_commit(empty(0));
+        }
+        __syncwarp();
+        int stage = 1 % NST, phase = 0;  // of the next tile to be read
+        for (int i = 0; i < n_tiles && alive; ++i) {
+            const bool more = i + 1 < n_tiles;
+            const int vs = stage, vp = phase;
+            if (++stage == NST) stage = 0, phase ^= 1;
+            const int ks = stage, kp = phase;
+            if (more && ++stage == NST) stage = 0, phase ^= 1;
+            alive = bar_wait_all(full(vs), vp, gave_up);
+            for (int q = 0; q < n_q && alive; ++q) {
+                alive = bar_wait_all(p_full(q), i & 1, gave_up);
+                if (!alive) break;
+                tc_fence_after();
+                if (leader) {
+                    pv(q, vs, i > 0);
                     tc_commit(o_full(q));
-                    if (i + 1 < n_tiles) {
-                        // The weights that this product reads lie where the next scores go.
-                        alive = bar_wait(o_full(q), i & 1, gave_up);
-                        if (alive && q == 0) alive = bar_wait(full(kl % NST), (kl / NST) & 1, gave_up);
-                        if (!alive) break;
-                        qk(q, kl % NST);
-                        tc_commit(s_full(q));
-                    }
+                    if (q == n_q - 1) tc_commit(empty(vs));
                 }
-                if (alive) {
-                    tc_commit(empty(vl % NST));
-                    if (i + 1 < n_tiles) tc_commit(empty(kl % NST));
+                __syncwarp();
+                if (more) {
+                    if (q == 0) alive = bar_wait_all(full(ks), kp, gave_up);
+                    // The weights that this product reads lie where the next scores go.
+                    if (alive) alive = bar_wait_all(o_full(q), i & 1, gave_up);
+                    if (!alive) break;
+                    if (leader) {
+                        qk(q, ks);
+                        tc_commit(s_full(q));
+                        if (q == n_q - 1) tc_commit(empty(ks));
+                    }
+                    __syncwarp();
                 }
             }
         }
@@ -506,7 +516,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     if (lost) {
         // Products may still be running: let them end (again with a limit) before the memory goes.
         __syncthreads();
-        if (threadIdx.x == 11 * 32) {
+        if (warp == 11 && elect_one()) {
             s_gave_up = 0;
             tc_commit(drained);
             bar_wait(drained, 0, gave_up);

@@ -45,6 +45,22 @@ __device__ __forceinline__ bool bar_wait_warp(uint32_t bar, uint32_t parity, vol
     return __shfl_sync(0xffffffffu, ok, 0);
 }
 
+// The same where every lane asks (a warp that stays converged around its products).
+__device__ __forceinline__ bool bar_wait_all(uint32_t bar, uint32_t parity, volatile int* gave_up) {
+    for (int i = 0; i < kWaitLimit; ++i) {
+        if (__all_sync(0xffffffffu, bar_try(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *gave_up)) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
+// One lane of the (converged) warp, the same one each time.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t is;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(is));
+    return is != 0;
+}
+
 __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes)
                  : "memory");
