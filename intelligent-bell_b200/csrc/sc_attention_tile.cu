@@ -336,9 +336,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             if (++stage == NST) stage = 0, phase ^= 1;
             const int ks = stage, kp = phase;
             if (more && ++stage == NST) stage = 0, phase ^= 1;
-            alive = bar_wait_all(full(vs), vp, gave_up);
             for (int q = 0; q < n_q && alive; ++q) {
-                alive = bar_wait_all(p_full(q), i & 1, gave_up);
+                alive = q == 0 ? bar_wait_both(full(vs), vp, p_full(0), i & 1, gave_up)
+                               : bar_wait_all(p_full(q), i & 1, gave_up);
                 if (!alive) break;
                 tc_fence_after();
                 if (leader) {
@@ -348,9 +348,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 }
                 __syncwarp();
                 if (more) {
-                    if (q == 0) alive = bar_wait_all(full(ks), kp, gave_up);
                     // The weights that this product reads lie where the next scores go.
-                    if (alive) alive = bar_wait_all(o_full(q), i & 1, gave_up);
+                    alive = q == 0 ? bar_wait_both(full(ks), kp, o_full(0), i & 1, gave_up)
+                                   : bar_wait_all(o_full(q), i & 1, gave_up);
                     if (!alive) break;
                     if (leader) {
                         qk(q, ks);

@@ -54,6 +54,18 @@ __device__ __forceinline__ bool bar_wait_all(uint32_t bar, uint32_t parity, vola
     *gave_up = 1;
     return false;
 }
+// Two barriers, asked in one go: an answer takes some 200 clocks while the tensor cores read shared
+// memory.
+__device__ __forceinline__ bool bar_wait_both(uint32_t bar0, uint32_t parity0, uint32_t bar1,
+                                              uint32_t parity1, volatile int* gave_up) {
+    for (int i = 0; i < kWaitLimit; ++i) {
+        const bool a = bar_try(bar0, parity0), b = bar_try(bar1, parity1);
+        if (__all_sync(0xffffffffu, a && b)) return true;
+        if (__any_sync(0xffffffffu, *gave_up)) return false;
+    }
+    *gave_up = 1;
+    return false;
+}
 // One lane of the (converged) warp, the same one each time.
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;
@@ -151,6 +163,27 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
+}
+// 2^x of two values without the exponential unit, for x <= 127; NaN stays NaN.  x = n + f with n
+// the nearest integer (read off the low bits of x + 1.5 * 2^23) and |f| <= 1/2; 2^f by a
+// polynomial of degree 5, fitted for relative error (7.5e-8) at Chebyshev nodes; 2^n made of its
+// exponent bits.  Below 2^-126 the result is 2^-126.
+__device__ __forceinline__ float2 exp2_poly(float2 x) {
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
+    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
+    const float2 magic = make_float2(12582912.f, 12582912.f);
+    const float2 t = __fadd2_rn(x, magic);
+    const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
+    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
+    float2 y = __ffma2_rn(f, make_float2(1.3276461977511644e-3f, 1.3276461977511644e-3f),
+                          make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
+    y = __ffma2_rn(y, f, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
+    y = __ffma2_rn(y, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
+    y = __ffma2_rn(y, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
+    y = __ffma2_rn(y, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
+    const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
+                                     __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
+    return __fmul2_rn(y, scale);
 }
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
