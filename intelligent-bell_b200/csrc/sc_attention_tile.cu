@@ -131,7 +131,14 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     const uint32_t drained = bars + 8u * (7 + 2 * NST);
     volatile int* gave_up = &s_gave_up;
 
-    if (threadIdx.x == 0) {
+    if (p.D < DP) {  // columns that no copy writes
+        for (int i = threadIdx.x; i < (2 + NST) * TILE / 16; i += kTThreads)
+            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s_base + 16u * i), "r"(0)
+                         : "memory");
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncthreads();
+    }
+    if (warp == 8 && lane == 0) {
         bar_init(q_full, kTThreads / 32);
         bar_init(drained, 1);
         for (int s = 0; s < NST; ++s) {
@@ -147,18 +154,26 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         s_any_bad = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    // The first tiles of the prefix are on their way before anything else.
+    const int n_loads = 2 * n_tiles;  // K0 V0 K1 V1 ...
+    const int early = tp.tma_p ? min(min(n_loads, NST), 2 * max(0, tiles_p - first)) : 0;
+    auto load_prefix = [&](int i) {
+        const uint32_t bar = full(i % NST);
+        if (lane == 0) bar_expect(bar, TILE);
+        __syncwarp();
+        if (lane < CPR / 8)
+            tma_load(s_ring + i % NST * TILE + lane * 16384, i & 1 ? &tp.vp : &tp.kp, bar, lane * 64,
+                     (first + (i >> 1)) * kTokTile, h, 0);
+    };
+    if (warp == 8) {
+        __syncwarp();
+        for (int i = 0; i < early; ++i) load_prefix(i);
+    }
     if (warp == 11) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
                          smem_addr(&s_tmem))
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
-    if (p.D < DP) {  // columns that no copy writes
-        for (int i = threadIdx.x; i < (2 + NST) * TILE / 16; i += kTThreads)
-            asm volatile("st.shared.v4.b32 [%0], {%1,%1,%1,%1};" ::"r"(s_base + 16u * i), "r"(0)
-                         : "memory");
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        __syncthreads();
     }
     // Chunks of eight columns: a warp-wide copy covers 4 rows x 8 chunks of one panel.
     const int sub = lane >> 3, c8 = lane & 7;
@@ -186,17 +201,15 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         __syncwarp();
         if (lane == 0) bar_arrive(bar);
     };
-    if (warp < 8 || warp == 11) copies_done(q_full);
+    copies_done(q_full);
     constexpr uint32_t kO = 256;  // first column of O0
 
     if (warp >= 8 && warp < 8 + kLoadWarps) {
         // ---- copies ----
         const int lw = warp - 8;
         const bool paged = p.page_table != nullptr;
-        const int n_loads = 2 * n_tiles;
         bool alive = true;
-        for (int i = 0; i < n_loads; ++i) {
-            if (i == 1) copies_done(q_full);  // the first tile is on its way
+        for (int i = early; i < n_loads; ++i) {
             const int s = i % NST;
             const int tile = first + (i >> 1);
             const bool is_v = i & 1;
@@ -207,11 +220,15 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 if (lw == 0) {
                     if (i >= NST) alive = bar_wait_warp(empty(s), ((i / NST) - 1) & 1, gave_up);
                     if (!alive) continue;
+                    if (pre) {
+                        load_prefix(i);
+                        continue;
+                    }
                     if (lane == 0) bar_expect(full(s), TILE);
                     __syncwarp();
-                    const CUtensorMap* map = pre ? (is_v ? &tp.vp : &tp.kp) : (is_v ? &tp.vc : &tp.kc);
-                    if (pre || !paged) {
-                        if (lane < CPR / 8) tma_load(dst + lane * 16384, map, full(s), lane * 64, t0, h, pre ? 0 : b);
+                    const CUtensorMap* map = is_v ? &tp.vc : &tp.kc;
+                    if (!paged) {
+                        if (lane < CPR / 8) tma_load(dst + lane * 16384, map, full(s), lane * 64, t0, h, b);
                     } else {
                         // One lane a box; a page that is not there lies outside the map: zeros.
                         const int box = tp.box_c, n_box = kTokTile / box;
@@ -475,36 +492,54 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 const bool mine = r < n_rows;
                 const int64_t at = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + row - j * p.G;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
-                T* dst = static_cast<T*>(p.out) + (tok0 + j) * p.o_t + (h * p.G + row - j * p.G) * p.o_h;
-                float* po = p.part_o + (part_row + at) * p.D;
-#pragma unroll 1
-                for (int c = 0; c < DP / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld32(o_at + c * 32, o);
-                    tmem_wait_ld();
-                    if (mine) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 8) {
-                            if (c * 32 + e >= p.D) continue;
-                            if (tp.direct) {
-                                uint32_t v[4];
-#pragma unroll
-                                for (int k = 0; k < 4; ++k)
-                                    v[k] = pack2<T>(__uint_as_float(o[e + 2 * k]) * inv,
-                                                    __uint_as_float(o[e + 2 * k + 1]) * inv);
-                                st_v4(dst + c * 32 + e, make_uint4(v[0], v[1], v[2], v[3]));
-                            } else {
-                                st_v4(po + c * 32 + e, make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]));
-                                st_v4(po + c * 32 + e + 4, make_uint4(o[e + 4], o[e + 5], o[e + 6], o[e + 7]));
-                            }
-                        }
-                    }
-                }
                 if (mine) {
                     if (!tp.direct)
                         p.part_ml[part_row + at] = make_float2(m, l);
                     else if (p.lse)
                         p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
+                }
+                // 128 bytes of each of the warp's 32 rows at a time, turned in shared memory (where the
+                // warp's queries were) so that a store covers whole lines: a lane's 16 bytes in 32 rows
+                // took 5 us of a block's time.
+                const uint32_t stage = s_q + q * TILE + (warp & 3) * (TILE / 4);
+                const int per = tp.direct ? 64 : 32;  // columns a pass
+#pragma unroll 1
+                for (int c = 0; c < DP; c += per) {
+                    uint32_t o[64];
+                    tmem_ld32(o_at + c, o);
+                    if (tp.direct) tmem_ld32(o_at + c + 32, o + 32);
+                    tmem_wait_ld();
+                    if (tp.direct) {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e)
+                            o[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
+                                         stage + lane * 128 + ((k ^ (lane & 7)) << 4)),
+                                     "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
+                                     : "memory");
+                    __syncwarp();
+                    const int col = c + c8 * (per / 8);
+#pragma unroll
+                    for (int it = 0; it < 8; ++it) {
+                        const int rr = it * 4 + sub;
+                        const int row2 = r0 + q * kRowTile + (warp & 3) * 32 + rr;
+                        uint4 v;
+                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
+                                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                     : "r"(stage + rr * 128 + ((c8 ^ (rr & 7)) << 4)));
+                        if (row2 < r0 + n_rows && col < p.D) {
+                            const int j2 = static_cast<int>(fdiv(row2, p.div_G));
+                            const int head = h * p.G + row2 - j2 * p.G;
+                            if (tp.direct)
+                                st_v4(static_cast<T*>(p.out) + (tok0 + j2) * p.o_t + head * p.o_h + col, v);
+                            else
+                                st_v4(p.part_o + (part_row + static_cast<int64_t>(tok0 + j2) * p.Hq + head) * p.D + col, v);
+                        }
+                    }
+                    __syncwarp();
                 }
             }
         }
