@@ -493,9 +493,6 @@ cudaError_t preload_attention_type() {
 }
 
 // How the rows and tokens are split over kernels and parts.
-#ifndef SC_ROWS_WAVES
-#define SC_ROWS_WAVES 2
-#endif
 struct Split {
     Variant v;
     bool tile_p;   // the prefix by attend_tiles
@@ -504,9 +501,10 @@ struct Split {
     int32_t tiles_p, tiles_c;  // row tiles (of the kernel that takes them)
     int32_t chunk_p, n_pp, n_cp;
     int64_t units_tile, units_rows;
+    int32_t least, blocks, s_pp, s_cp;  // attend_stream: steps and blocks, and its parts
 };
 
-constexpr int kTileRows = 256, kTileTokens = 128;
+constexpr int kTileRows = 256, kTileTokens = 128, kStepTokens = 64;
 constexpr int kMinTileRows = 64;   // fewer rows: the copies bound both kernels
 constexpr int kMinFusedRows = 96;  // fewer rows a sequence: packing the batch's rows wins
 
@@ -549,15 +547,33 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
             s.direct = s.n_pp == 1 && !cap;
             s.units_tile = size_product(s.n_pp, s.tiles_p, Hkv);
         }
-        // attend_rows: two blocks fit an SM; two rounds of equal parts.
-        s.v = pick_variant(D, s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c);
+        s.v = pick_variant(D, !P || s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c);
         const int64_t mr = 16 * s.v.mt;
         const int32_t P_rows = s.tile_p ? 0 : P;
         if (!s.tile_p) s.tiles_p = static_cast<int32_t>((rows_p + mr - 1) / mr);
         s.tiles_c = static_cast<int32_t>((rows_c + mr - 1) / mr);
+
+        // attend_stream: as many blocks as stay, each with a run of steps; a run is 1 to 4 steps
+        // at least, and long enough that a row tile has 64 parts at most.
+        const int64_t steps_p = (P_rows + kStepTokens - 1) / kStepTokens;
+        const int64_t steps_c = cap ? (cap + kStepTokens - 1) / kStepTokens : 0;
+        const double steps = static_cast<double>(steps_p) * Hkv * s.tiles_p +
+                             static_cast<double>(steps_c) * Hkv * B * s.tiles_c;
+        const int resident = 148 * (s.v.dp == 256 || (s.v.dp == 128 && s.v.mt == 2) ? 1 : 2);
+        s.blocks = steps < 1 ? 0 : static_cast<int32_t>(steps < resident ? steps : resident);
+        const int64_t longest_steps = steps_p > steps_c ? steps_p : steps_c;
+        const double each = steps / resident;
+        int64_t least = each < 1 ? 1 : each > 4 ? 4 : static_cast<int64_t>(each);
+        if (least < (longest_steps + 62) / 63) least = (longest_steps + 62) / 63;
+        s.least = static_cast<int32_t>(least);
+        auto parts = [&](int64_t n) { return n ? static_cast<int32_t>((n + least - 1) / least + (n > 1)) : 0; };
+        s.s_pp = s.tile_p ? s.n_pp : parts(steps_p);
+        s.s_cp = parts(steps_c);
+
+        // attend_rows: two blocks fit an SM; two rounds of equal parts.
         const double work = static_cast<double>(P_rows) * Hkv * s.tiles_p +
                             static_cast<double>(cap) * Hkv * B * s.tiles_c;
-        double chunk = ceil(work / (148.0 * 2 * SC_ROWS_WAVES) / kPartTokens) * kPartTokens;
+        double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
         const double longest = P_rows > cap ? P_rows : cap;
         const double most_parts = 64;
         if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;
@@ -596,7 +612,8 @@ int32_t check_sizes(int64_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, in
 }
 
 int64_t workspace_floats(const Split& s, int64_t N, int32_t Hq, int32_t D) {
-    return s.direct ? 0 : size_product(static_cast<int64_t>(s.n_pp) + s.n_cp, N * Hq, D + 2);
+    const int64_t rows = static_cast<int64_t>(s.n_pp) + s.n_cp, stream = static_cast<int64_t>(s.s_pp) + s.s_cp;
+    return s.direct ? 0 : size_product(rows > stream ? rows : stream, N * Hq, D + 2);
 }
 
 }  // namespace
@@ -605,6 +622,7 @@ cudaError_t preload_attention_kernels() {
     cudaError_t e = preload_attention_type<__half>();
     if (e == cudaSuccess) e = preload_attention_type<__nv_bfloat16>();
     if (e == cudaSuccess) e = preload_attention_tile_kernels();
+    if (e == cudaSuccess) e = preload_attention_stream_kernels();
     return e;
 }
 
@@ -696,25 +714,39 @@ extern "C" int32_t sc_shared_prefix_attention(
     p.div_G = make_fastdiv(static_cast<uint32_t>(p.G));
     p.div_page = make_fastdiv(static_cast<uint32_t>(p.page));
     p.scale_log2 = static_cast<float>(scale * 1.4426950408889634);
-    p.n_pp = s.n_pp, p.n_cp = s.n_cp, p.chunk_p = s.chunk_p, p.tiles_p = s.tiles_p, p.tiles_c = s.tiles_c;
+    p.chunk_p = s.chunk_p, p.tiles_p = s.tiles_p, p.tiles_c = s.tiles_c;
     const int64_t rows = n_tokens * q_heads;
     p.part_o = static_cast<float*>(workspace);
-    p.part_ml = reinterpret_cast<float2*>(p.part_o + (s.n_pp + s.n_cp) * rows * head_dim);
+    auto set_parts = [&](int32_t n_pp, int32_t n_cp) {
+        p.n_pp = n_pp, p.n_cp = n_cp;
+        p.part_ml = reinterpret_cast<float2*>(p.part_o + (n_pp + n_cp) * rows * head_dim);
+    };
+    const bool stream_first = !s.fused && s.blocks > 0;
+    set_parts(stream_first ? s.s_pp : s.n_pp, stream_first ? s.s_cp : s.n_cp);
     p.out = out, p.o_t = out_strides[0], p.o_h = out_strides[1];
     p.lse = lse, p.status = status;
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
     const bool half = dtype == SC_DTYPE_F16;
+    // Few rows: the streaming kernel, or attend_rows where tensor maps cannot say the layout (pages
+    // that no box of 8 rows divides, expanded strides).
+    if (s.units_rows) {
+        bool taken = false;
+        if (stream_first)
+            e = launch_attention_stream(p, half, !s.tile_p && prefix_len > 0, s.v.dp, s.v.mt, s.least, s.blocks, st,
+                                        &taken);
+        if (e == cudaSuccess && !taken) {
+            set_parts(s.n_pp, s.n_cp);
+            e = half ? launch_rows_dp<__half>(p, s.v, s.units_rows, st)
+                     : launch_rows_dp<__nv_bfloat16>(p, s.v, s.units_rows, st);
+        }
+        if (e != cudaSuccess) return cuda_error(e, "attention launch");
+    }
     if (s.units_tile) {
         e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, s.direct,
                                    s.units_tile, st);
         if (e != cudaSuccess) return cuda_error(e, "attention tiles launch");
-    }
-    if (s.units_rows) {
-        e = half ? launch_rows_dp<__half>(p, s.v, s.units_rows, st)
-                 : launch_rows_dp<__nv_bfloat16>(p, s.v, s.units_rows, st);
-        if (e != cudaSuccess) return cuda_error(e, "attention launch");
     }
     if (s.direct) return ok();
     const unsigned blocks = static_cast<unsigned>((rows + kWarps - 1) / kWarps);

@@ -150,4 +150,11 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
                                    bool direct, int64_t units, cudaStream_t s);
 cudaError_t preload_attention_tile_kernels();
 
+// The streaming kernel (sc_attention_stream.cu): few rows, parts of runs of 64-token steps, at least
+// `least` of them; dp: head_dim padded to 64, 128 or 256; mt: 16-row tiles.  *taken is false where
+// its tensor maps cannot say the layout, and nothing is launched.
+cudaError_t launch_attention_stream(const AttnParams& a, bool half, bool with_prefix, int dp, int mt, int least,
+                                    int blocks, cudaStream_t s, bool* taken);
+cudaError_t preload_attention_stream_kernels();
+
 }  // namespace sc

@@ -555,6 +555,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             s_gave_up = 0;
             tc_commit(drained);
             bar_wait(drained, 0, gave_up);
+            let_copies_land();
             if (p.status) atomicOr(p.status, SC_STATUS_WAIT_LIMIT);
         }
         __syncthreads();

@@ -66,6 +66,12 @@ __device__ __forceinline__ bool bar_wait_both(uint32_t bar0, uint32_t parity0, u
     *gave_up = 1;
     return false;
 }
+// After a wait was given up: about a millisecond for copies in flight to land.
+__device__ __forceinline__ void let_copies_land() {
+    const long long t = clock64();
+    while (clock64() - t < 2000000) {
+    }
+}
 // One lane of the (converged) warp, the same one each time.
 __device__ __forceinline__ bool elect_one() {
     uint32_t is;

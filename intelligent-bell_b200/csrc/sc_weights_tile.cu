@@ -420,6 +420,7 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
             s_gave_up = 0;
             tc_commit(drained);
             bar_wait(drained, 0, gave_up);
+            let_copies_land();
             atomicOr(p.status, SC_STATUS_WAIT_LIMIT);
         }
         __syncthreads();
