@@ -50,6 +50,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     __shared__ float s_m[kWarps][MR], s_l[kWarps][MR];
     __shared__ int s_bad;
 
+    let_next_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     unsigned char* s_q = smem;
     unsigned char* s_ring = smem + MR * DP * 2;
@@ -392,6 +393,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
 // One warp a row: o = sum_i 2^(m_i - m) o_i / sum_i 2^(m_i - m) l_i over the parts, in order.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ AttnParams p) {
+    wait_for_previous();
     const int64_t row = static_cast<int64_t>(blockIdx.x) * kWarps + (threadIdx.x >> 5);
     const int lane = threadIdx.x & 31;
     const int64_t all_rows = static_cast<int64_t>(p.N) * p.Hq;
@@ -745,16 +747,14 @@ extern "C" int32_t sc_shared_prefix_attention(
     }
     if (s.units_tile) {
         e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, s.direct,
-                                   s.units_tile, st);
+                                   s.units_tile, s.units_rows > 0, st);
         if (e != cudaSuccess) return cuda_error(e, "attention tiles launch");
     }
     if (s.direct) return ok();
     const unsigned blocks = static_cast<unsigned>((rows + kWarps - 1) / kWarps);
-    if (half)
-        join_parts<__half><<<blocks, kThreads, 0, st>>>(p);
-    else
-        join_parts<__nv_bfloat16><<<blocks, kThreads, 0, st>>>(p);
-    e = cudaGetLastError();
+    const bool after = s.units_tile > 0 || s.units_rows > 0;
+    e = half ? launch_chained(join_parts<__half>, dim3(blocks), kThreads, 0, st, after, p)
+             : launch_chained(join_parts<__nv_bfloat16>, dim3(blocks), kThreads, 0, st, after, p);
     if (e != cudaSuccess) return cuda_error(e, "attention join launch");
     return ok();
 }

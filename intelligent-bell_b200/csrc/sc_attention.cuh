@@ -145,9 +145,10 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 
 // The tensor-core kernel (sc_attention_tile.cu): `splits` parts over the token axis of the prefix,
 // for all rows together, or (per_seq) of the prefix and then each sequence's own cache, for the
-// sequence's rows.  direct: one part, which writes the output.
+// sequence's rows.  direct: one part, which writes the output.  chained: another kernel of the call
+// is before it on the stream.
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
-                                   bool direct, int64_t units, cudaStream_t s);
+                                   bool direct, int64_t units, bool chained, cudaStream_t s);
 cudaError_t preload_attention_tile_kernels();
 
 // The streaming kernel (sc_attention_stream.cu): few rows, parts of runs of 64-token steps, at least

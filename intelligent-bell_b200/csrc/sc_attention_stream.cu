@@ -66,6 +66,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     __shared__ int s_gave_up;
     __shared__ float s_m[kSWarps][MR], s_l[kSWarps][MR];
 
+    let_next_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t s_ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t s_q = s_ring + NST * STAGE;

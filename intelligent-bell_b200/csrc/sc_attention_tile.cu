@@ -84,7 +84,11 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     }
     const int rows = n_tok * p.G;
     const int r0 = rt * 2 * kRowTile;
-    if (r0 >= rows) return;
+    let_next_start();
+    if (r0 >= rows) {
+        wait_for_previous();
+        return;
+    }
     const int n_rows = min(2 * kRowTile, rows - r0);
     const int n_q = n_rows > kRowTile ? 2 : 1;
 
@@ -116,6 +120,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             else if (p.lse)
                 p.lse[row] = kNegInf;
         }
+        wait_for_previous();
         return;
     }
 
@@ -562,22 +567,22 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     }
     if (warp == 11)
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    wait_for_previous();  // nothing is read from it, but this kernel's end stands for its end, too
 }
 
 template <typename T, int DP>
-cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, cudaStream_t s, bool load_only) {
+cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, bool chained, cudaStream_t s, bool load_only) {
     auto kernel = attend_tiles<T, DP>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), TileShape<DP>::kSmem, done);
     if (e != cudaSuccess || load_only) return e;
-    kernel<<<units, kTThreads, TileShape<DP>::kSmem, s>>>(p);
-    return cudaGetLastError();
+    return launch_chained(kernel, dim3(units), kTThreads, TileShape<DP>::kSmem, s, chained, p);
 }
 
 }  // namespace
 
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
-                                   bool direct, int64_t units, cudaStream_t s) {
+                                   bool direct, int64_t units, bool chained, cudaStream_t s) {
     TileParams p{};
     p.a = a;
     p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.direct = direct;
@@ -598,18 +603,18 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
     }
     const unsigned n = static_cast<unsigned>(units);
     if (a.D <= 64)
-        return half ? launch_tiles_dp<__half, 64>(p, n, s, false)
-                    : launch_tiles_dp<__nv_bfloat16, 64>(p, n, s, false);
-    return half ? launch_tiles_dp<__half, 128>(p, n, s, false)
-                : launch_tiles_dp<__nv_bfloat16, 128>(p, n, s, false);
+        return half ? launch_tiles_dp<__half, 64>(p, n, chained, s, false)
+                    : launch_tiles_dp<__nv_bfloat16, 64>(p, n, chained, s, false);
+    return half ? launch_tiles_dp<__half, 128>(p, n, chained, s, false)
+                : launch_tiles_dp<__nv_bfloat16, 128>(p, n, chained, s, false);
 }
 
 cudaError_t preload_attention_tile_kernels() {
     TileParams p{};
-    cudaError_t e = launch_tiles_dp<__half, 64>(p, 0, nullptr, true);
-    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 64>(p, 0, nullptr, true);
-    if (e == cudaSuccess) e = launch_tiles_dp<__half, 128>(p, 0, nullptr, true);
-    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 128>(p, 0, nullptr, true);
+    cudaError_t e = launch_tiles_dp<__half, 64>(p, 0, false, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 64>(p, 0, false, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__half, 128>(p, 0, false, nullptr, true);
+    if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 128>(p, 0, false, nullptr, true);
     return e;
 }
 

@@ -42,6 +42,31 @@ __device__ __forceinline__ uint32_t fdiv(uint32_t n, const FastDiv& f) {
 }
 
 // ---------------------------------------------------------------------------------------
+// Kernels of one call that follow one another on a stream.  `chained`: the launch may start while
+// the kernel before it still runs (once every block of that one has called let_next_start or
+// ended); it calls wait_for_previous before it reads what that one wrote, and in any case before
+// it ends, so that its own end still means the end of everything before it.
+// ---------------------------------------------------------------------------------------
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+template <typename P>
+inline cudaError_t launch_chained(void (*kernel)(P), dim3 grid, unsigned block, size_t smem, cudaStream_t s,
+                                  bool chained, const P& params) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = chained ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kernel, params);
+}
+
+// ---------------------------------------------------------------------------------------
 // Memory access.  Inputs are read once: non-coherent loads that do not allocate in L1.
 // Tuning knobs (compile-time): SC_LOAD_L2_PREFETCH adds a 256-byte L2 prefetch hint to
 // the input loads; SC_STORE_STREAMING marks output stores evict-first.

@@ -89,6 +89,7 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
     __shared__ int s_warp[3][kSelWarps];
     __shared__ int s_pick[2];    // digit, equal ones still wanted
     __shared__ int s_counts[2];  // this block's kept-for-sure and equal tokens
+    let_next_start();
     cg::cluster_group cluster = cg::this_cluster();
     const int rank = static_cast<int>(cluster.block_rank());
     const int ranks = static_cast<int>(cluster.num_blocks());
@@ -251,6 +252,7 @@ struct MoveParams {
 };
 
 __global__ void __launch_bounds__(kMoveThreads) move_rows(const __grid_constant__ MoveParams p) {
+    wait_for_previous();
     const MoveTensor& x = p.x[blockIdx.z];
     const int row = blockIdx.y, b = row / p.H, h = row - b * p.H;
     const int32_t* idx = p.indices + static_cast<int64_t>(row) * p.budget;
@@ -323,6 +325,7 @@ __device__ __forceinline__ void move_slice(const char* src, char* dst, int64_t s
 }
 
 __global__ void __launch_bounds__(kMoveThreads) move_rows_in_place(const __grid_constant__ MoveParams p) {
+    wait_for_previous();
     const int row = blockIdx.y, b = row / p.H, h = row - b * p.H;
     const int32_t* idx = p.indices + static_cast<int64_t>(row) * p.budget;
     const int which = blockIdx.x < 2 * p.slices ? blockIdx.x / p.slices : 2;
@@ -462,14 +465,14 @@ extern "C" int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache
     if (in_place) {
         mp.slice16 = 4;  // 64 bytes: the DRAM access granularity
         mp.slices = (mp.row16 + mp.slice16 - 1) / mp.slice16;
-        move_rows_in_place<<<dim3(2 * mp.slices + 1, static_cast<unsigned>(rows)), kMoveThreads, 0, st>>>(mp);
+        e = launch_chained(move_rows_in_place, dim3(2 * mp.slices + 1, static_cast<unsigned>(rows)), kMoveThreads, 0,
+                           st, true, mp);
     } else {
         const int64_t pieces = budget * (mp.row16 ? mp.row16 : 1);
         const int64_t per = kMoveThreads * kMoveUnroll;
-        move_rows<<<dim3(static_cast<unsigned>((pieces + per - 1) / per), static_cast<unsigned>(rows), 3),
-                    kMoveThreads, 0, st>>>(mp);
+        e = launch_chained(move_rows, dim3(static_cast<unsigned>((pieces + per - 1) / per), static_cast<unsigned>(rows), 3),
+                           kMoveThreads, 0, st, true, mp);
     }
-    e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_error(e, "eviction move launch");
     return ok();
 }
