@@ -499,7 +499,7 @@ struct Split {
     Variant v;
     bool tile_p;   // the prefix by attend_tiles
     bool fused;    // prefix and own caches together by attend_tiles, a sequence's rows at a time
-    bool direct;   // one part, written as the output
+    bool direct;   // no parts of the whole call: the output is written at once
     int32_t tiles_p, tiles_c;  // row tiles (of the kernel that takes them)
     int32_t chunk_p, n_pp, n_cp;
     int64_t units_tile, units_rows;
@@ -508,17 +508,20 @@ struct Split {
 
 constexpr int kTileRows = 256, kTileTokens = 128, kStepTokens = 64;
 constexpr int kMinTileRows = 64;   // fewer rows: the copies bound both kernels
+constexpr int kSms = 148;          // blocks of attend_tiles at a time
+constexpr int kTailParts = 16;     // of a unit in the last round, at most
+constexpr int kMaxFused = 1024;    // sequences: every block counts their units
 constexpr int kMinFusedRows = 96;  // fewer rows a sequence: packing the batch's rows wins
 
 // Parts of the token axis for attend_tiles: the number that ends soonest, in units of one step
-// (256 rows x 128 tokens, about 1.3 us), counting whole waves of 148 blocks, a block's start and
-// end (2.5 steps), and the parts' way through memory.
+// (256 rows x 128 tokens, about 2 us), counting whole rounds of 148 blocks, a block's start and
+// end (4 steps), and the parts' way through memory.
 int32_t plan_parts(double blocks, int64_t steps, double rows, int32_t D) {
     int32_t best = 1;
     double best_cost = 0.;
     for (int32_t n = 1; n <= 64 && (n == 1 || n * 2 <= steps); ++n) {
-        const double waves = ceil(blocks * n / 148.0);
-        double cost = waves * (static_cast<double>((steps + n - 1) / n) + 2.5) * 1.3;
+        const double waves = ceil(blocks * n / kSms);
+        double cost = waves * (static_cast<double>((steps + n - 1) / n) + 4.0) * 2.0;
         if (n > 1) cost += 2.0 + n * rows * D * 8.0 / 5e6;
         if (n == 1 || cost < best_cost) best = n, best_cost = cost;
     }
@@ -530,17 +533,16 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
     const int64_t G = Hq / Hkv;
     const int64_t rows_p = N * G, rows_c = cap ? nq * G : 0;
     Split s{};
-    s.fused = D <= 128 && cap && rows_c >= kMinFusedRows;
+    s.fused = D <= 128 && cap && rows_c >= kMinFusedRows && B <= kMaxFused;
     s.tile_p = !s.fused && D <= 128 && P && rows_p >= kMinTileRows;
     const double rows = static_cast<double>(N) * Hq;
     if (s.fused) {
         s.tiles_c = static_cast<int32_t>((rows_c + kTileRows - 1) / kTileRows);
-        const double most = static_cast<double>(rows_p) / kTileRows + B;  // ragged: fewer than B * tiles_c
-        const double all = static_cast<double>(B) * s.tiles_c;
         const int64_t steps = (P + kTileTokens - 1) / kTileTokens + (cap + kTileTokens - 1) / kTileTokens;
-        s.n_pp = plan_parts((most < all ? most : all) * Hkv, steps, rows, D);
-        s.direct = s.n_pp == 1;
-        s.units_tile = size_product(size_product(s.n_pp, s.tiles_c, Hkv), B);
+        const int64_t most = rows_p / kTileRows + B, all = size_product(B, s.tiles_c);  // ragged: fewer than all
+        s.n_pp = steps < 2 ? 1 : steps / 2 < kTailParts ? static_cast<int32_t>(steps / 2) : kTailParts;
+        s.direct = true;
+        s.units_tile = size_product(most < all ? most : all, Hkv) + (s.n_pp > 1 ? kSms - 1 : 0);
     } else {
         if (s.tile_p) {
             s.tiles_p = static_cast<int32_t>((rows_p + kTileRows - 1) / kTileRows);
@@ -615,6 +617,7 @@ int32_t check_sizes(int64_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, in
 
 int64_t workspace_floats(const Split& s, int64_t N, int32_t Hq, int32_t D) {
     const int64_t rows = static_cast<int64_t>(s.n_pp) + s.n_cp, stream = static_cast<int64_t>(s.s_pp) + s.s_cp;
+    if (s.fused) return s.n_pp > 1 ? static_cast<int64_t>(kSms) * kTileRows * (D + 2) : 0;
     return s.direct ? 0 : size_product(rows > stream ? rows : stream, N * Hq, D + 2);
 }
 
@@ -721,7 +724,8 @@ extern "C" int32_t sc_shared_prefix_attention(
     p.part_o = static_cast<float*>(workspace);
     auto set_parts = [&](int32_t n_pp, int32_t n_cp) {
         p.n_pp = n_pp, p.n_cp = n_cp;
-        p.part_ml = reinterpret_cast<float2*>(p.part_o + (n_pp + n_cp) * rows * head_dim);
+        const int64_t part_rows = s.fused ? static_cast<int64_t>(kSms) * kTileRows : (n_pp + n_cp) * rows;
+        p.part_ml = reinterpret_cast<float2*>(p.part_o + part_rows * head_dim);
     };
     const bool stream_first = !s.fused && s.blocks > 0;
     set_parts(stream_first ? s.s_pp : s.n_pp, stream_first ? s.s_cp : s.n_cp);
@@ -746,7 +750,7 @@ extern "C" int32_t sc_shared_prefix_attention(
         if (e != cudaSuccess) return cuda_error(e, "attention launch");
     }
     if (s.units_tile) {
-        e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, s.direct,
+        e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, kSms,
                                    s.units_tile, s.units_rows > 0, st);
         if (e != cudaSuccess) return cuda_error(e, "attention tiles launch");
     }

@@ -143,12 +143,12 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-// The tensor-core kernel (sc_attention_tile.cu): `splits` parts over the token axis of the prefix,
-// for all rows together, or (per_seq) of the prefix and then each sequence's own cache, for the
-// sequence's rows.  direct: one part, which writes the output.  chained: another kernel of the call
-// is before it on the stream.
+// The tensor-core kernel (sc_attention_tile.cu), over the prefix for all rows together in `splits`
+// parts, or (per_seq) over the prefix and then each sequence's own cache for the sequence's rows,
+// output included: rounds of `sms` units, the last one's split into up to `splits` parts.
+// chained: another kernel of the call is before it on the stream.
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
-                                   bool direct, int64_t units, bool chained, cudaStream_t s);
+                                   int sms, int64_t units, bool chained, cudaStream_t s);
 cudaError_t preload_attention_tile_kernels();
 
 // The streaming kernel (sc_attention_stream.cu): few rows, parts of runs of 64-token steps, at least

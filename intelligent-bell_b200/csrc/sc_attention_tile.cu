@@ -41,9 +41,9 @@ struct TileShape {
 struct TileParams {
     AttnParams a;
     int32_t per_seq;   // rows are those of one sequence, and its own cache follows the prefix
-    int32_t tiles;     // 256-row tiles, at most
-    int32_t splits;    // parts of the token axis
-    int32_t direct;    // one part: write the output itself
+    int32_t tiles;     // 256-row tiles of all rows together (not per_seq)
+    int32_t splits;    // parts of the token axis (per_seq: of the last round's units, at most)
+    int32_t sms;       // blocks of a round
     int32_t tma_p, tma_c;  // whether the maps below are in use
     int32_t box_c;         // rows of a box of the own caches
     CUtensorMap kp, vp, kc, vc;
@@ -52,6 +52,68 @@ struct TileParams {
 // Byte offset of 16-byte chunk c (of a 128-row tile's row r).
 __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
     return static_cast<uint32_t>((c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// A sequence's rows in units of 256 of one KV head (per_seq).  All units take equally long, so they
+// run in rounds of one unit an SM; those of the last, unfilled round are split over the SMs that
+// would be idle: into `parts` parts each, whose sums join_tail adds up.  Called by whole warps.
+struct Round {
+    int units, full, rem, parts;  // units before the last round, in it, and parts of each there
+};
+__device__ __forceinline__ int units_of(const AttnParams& p, int b) {
+    int n = p.nq;
+    if (p.cu_q != nullptr) {
+        const int a = p.cu_q[b], e = p.cu_q[b + 1];
+        n = a >= 0 && e >= a && e <= p.N && e - a <= p.nq ? e - a : 0;
+    }
+    return (n * p.G + 2 * kRowTile - 1) / (2 * kRowTile);
+}
+__device__ __forceinline__ Round rounds(const TileParams& tp) {
+    const AttnParams& p = tp.a;
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    if (p.cu_q == nullptr)
+        n = p.B * units_of(p, 0);
+    else
+        for (int b0 = 0; b0 < p.B; b0 += 32)
+            n += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? units_of(p, b0 + lane) : 0);
+    Round r;
+    r.units = n * p.Hkv;
+    r.full = r.units / tp.sms * tp.sms;
+    r.rem = r.units - r.full;
+    r.parts = r.rem ? max(1, min(tp.splits, tp.sms / r.rem)) : 1;
+    return r;
+}
+// Unit u as sequence, head and row tile; units of a sequence lie together.
+__device__ __forceinline__ void locate(const AttnParams& p, int u, int& b, int& h, int& rt) {
+    const int lane = threadIdx.x & 31;
+    int in = u, own = 0;
+    if (p.cu_q == nullptr) {
+        own = units_of(p, 0);
+        b = u / (own * p.Hkv);
+        in = u - b * own * p.Hkv;
+    } else {
+        for (int b0 = 0;; b0 += 32) {
+            const int n = b0 + lane < p.B ? units_of(p, b0 + lane) : 0;
+            int upto = n;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, d);
+                if (lane >= d) upto += y;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, in < upto * p.Hkv);
+            if (past || b0 + 32 >= p.B) {
+                const int at = past ? __ffs(past) - 1 : 31;
+                in -= __shfl_sync(0xffffffffu, upto - n, at) * p.Hkv;
+                own = __shfl_sync(0xffffffffu, n, at);
+                b = b0 + at;
+                break;
+            }
+            in -= __shfl_sync(0xffffffffu, upto, 31) * p.Hkv;
+        }
+    }
+    h = own ? in / own : 0;
+    rt = in - h * own;
 }
 
 template <typename T, int DP>
@@ -69,22 +131,38 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    int u = blockIdx.x;
-    const int split = u % tp.splits;
-    u /= tp.splits;
-    const int rt = u % tp.tiles;
-    u /= tp.tiles;
-    const int h = u % p.Hkv, b = u / p.Hkv;
+    int b = 0, h, rt, split = 0, splits, slot = 0;
     int tok0 = 0, n_tok, len = 0;
+    let_next_start();
     if (tp.per_seq) {
+        const Round r = rounds(tp);
+        int u = blockIdx.x;
+        splits = 1;
+        if (u >= r.full) {
+            slot = u - r.full;
+            if (slot >= r.rem * r.parts) {
+                wait_for_previous();
+                return;
+            }
+            splits = r.parts;
+            split = slot % splits;
+            u = r.full + slot / splits;
+        }
+        locate(p, u, b, h, rt);
         sequence_tokens(p, b, tok0, n_tok);
         len = p.cap ? cache_length(p, b) : 0;
     } else {
+        int u = blockIdx.x;
+        splits = tp.splits;
+        split = u % splits;
+        u /= splits;
+        rt = u % tp.tiles;
+        h = u / tp.tiles;
         n_tok = used_tokens(p);
     }
+    const bool direct = splits == 1 && (tp.per_seq || p.n_pp + p.n_cp == 1);
     const int rows = n_tok * p.G;
     const int r0 = rt * 2 * kRowTile;
-    let_next_start();
     if (r0 >= rows) {
         wait_for_previous();
         return;
@@ -97,13 +175,18 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     const int vis = max(0, min(len, see + static_cast<int>(fdiv(r0 + n_rows - 1, p.div_G)) + 1));
     const int tiles_p = (p.P + kTokTile - 1) / kTokTile;
     const int tiles_all = tiles_p + (vis + kTokTile - 1) / kTokTile;
-    const int per = (tiles_all + tp.splits - 1) / tp.splits;
+    const int per = (tiles_all + splits - 1) / splits;
     const int first = split * per;
     const int n_tiles = max(0, min(per, tiles_all - first));
-    const int64_t part_row = static_cast<int64_t>(split) * p.N * p.Hq;
+    // Where row r of the unit goes as a part: per_seq, its slot of 256 rows; else its place in the call.
+    auto part_at = [&](int r) -> int64_t {
+        if (tp.per_seq) return static_cast<int64_t>(slot) * (2 * kRowTile) + r;
+        const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
+        return (static_cast<int64_t>(split) * p.N + tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
+    };
 
     if (n_tiles == 0) {
-        if (tp.direct) {
+        if (direct) {
             for (int i = threadIdx.x; i < n_rows * (p.D / 8); i += kTThreads) {
                 const int r = i / (p.D / 8), c = i - r * (p.D / 8);
                 const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
@@ -115,8 +198,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         for (int r = threadIdx.x; r < n_rows; r += kTThreads) {
             const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
             const int64_t row = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
-            if (!tp.direct)
-                p.part_ml[part_row + row] = make_float2(kNegInf, 0.f);
+            if (!direct)
+                p.part_ml[part_at(r)] = make_float2(kNegInf, 0.f);
             else if (p.lse)
                 p.lse[row] = kNegInf;
         }
@@ -498,8 +581,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 const int64_t at = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + row - j * p.G;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
                 if (mine) {
-                    if (!tp.direct)
-                        p.part_ml[part_row + at] = make_float2(m, l);
+                    if (!direct)
+                        p.part_ml[part_at(r)] = make_float2(m, l);
                     else if (p.lse)
                         p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
                 }
@@ -507,14 +590,14 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 // warp's queries were) so that a store covers whole lines: a lane's 16 bytes in 32 rows
                 // took 5 us of a block's time.
                 const uint32_t stage = s_q + q * TILE + (warp & 3) * (TILE / 4);
-                const int per = tp.direct ? 64 : 32;  // columns a pass
+                const int per = direct ? 64 : 32;  // columns a pass
 #pragma unroll 1
                 for (int c = 0; c < DP; c += per) {
                     uint32_t o[64];
                     tmem_ld32(o_at + c, o);
-                    if (tp.direct) tmem_ld32(o_at + c + 32, o + 32);
+                    if (direct) tmem_ld32(o_at + c + 32, o + 32);
                     tmem_wait_ld();
-                    if (tp.direct) {
+                    if (direct) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)
                             o[e] = pack2<T>(__uint_as_float(o[2 * e]) * inv, __uint_as_float(o[2 * e + 1]) * inv);
@@ -538,10 +621,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         if (row2 < r0 + n_rows && col < p.D) {
                             const int j2 = static_cast<int>(fdiv(row2, p.div_G));
                             const int head = h * p.G + row2 - j2 * p.G;
-                            if (tp.direct)
+                            if (direct)
                                 st_v4(static_cast<T*>(p.out) + (tok0 + j2) * p.o_t + head * p.o_h + col, v);
                             else
-                                st_v4(p.part_o + (part_row + static_cast<int64_t>(tok0 + j2) * p.Hq + head) * p.D + col, v);
+                                st_v4(p.part_o + part_at(row2 - r0) * p.D + col, v);
                         }
                     }
                     __syncwarp();
@@ -570,22 +653,70 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     wait_for_previous();  // nothing is read from it, but this kernel's end stands for its end, too
 }
 
+// Rows of the last round's units: their parts joined, a warp a row.
+constexpr int kTailRows = 32;  // rows a block
+template <typename T>
+__global__ void __launch_bounds__(128) join_tail(const __grid_constant__ TileParams tp) {
+    wait_for_previous();
+    const AttnParams& p = tp.a;
+    const Round rd = rounds(tp);
+    const int unit = blockIdx.x / (2 * kRowTile / kTailRows);
+    if (unit >= rd.rem || rd.parts == 1) return;
+    int b, h, rt, tok0, n_tok;
+    locate(p, rd.full + unit, b, h, rt);
+    sequence_tokens(p, b, tok0, n_tok);
+    const int lane = threadIdx.x & 31;
+    const int first = (blockIdx.x % (2 * kRowTile / kTailRows)) * kTailRows;
+    for (int r = first + (threadIdx.x >> 5); r < first + kTailRows; r += 4) {
+        const int row = rt * 2 * kRowTile + r;
+        if (row >= n_tok * p.G) break;
+        const int64_t at = static_cast<int64_t>(unit) * rd.parts * (2 * kRowTile) + r;
+        // a lane a part
+        const float2 ml = lane < rd.parts ? p.part_ml[at + lane * (2 * kRowTile)] : make_float2(kNegInf, 0.f);
+        float m = ml.x;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+        const float w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
+        float sum = ml.x == kNegInf && ml.y == 0.f ? 0.f : w * ml.y;
+#pragma unroll
+        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int i = 0; i < rd.parts; ++i) {
+            const float wi = __shfl_sync(0xffffffffu, w, i);
+            if (wi == 0.f || lane * 4 >= p.D) continue;
+            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + i * (2 * kRowTile)) * p.D + lane * 4);
+            a.x += wi * v.x, a.y += wi * v.y, a.z += wi * v.z, a.w += wi * v.w;
+        }
+        const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        const int j = static_cast<int>(fdiv(row, p.div_G)), head = h * p.G + row - j * p.G;
+        if (lane * 4 < p.D)
+            st_v2(static_cast<T*>(p.out) + (tok0 + j) * p.o_t + head * p.o_h + lane * 4,
+                  make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)));
+        if (p.lse && lane == 0)
+            p.lse[static_cast<int64_t>(tok0 + j) * p.Hq + head] =
+                sum == 0.f ? kNegInf : (m + log2f(sum)) * 0.6931471805599453f;
+    }
+}
+
 template <typename T, int DP>
 cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, bool chained, cudaStream_t s, bool load_only) {
     auto kernel = attend_tiles<T, DP>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), TileShape<DP>::kSmem, done);
     if (e != cudaSuccess || load_only) return e;
-    return launch_chained(kernel, dim3(units), kTThreads, TileShape<DP>::kSmem, s, chained, p);
+    e = launch_chained(kernel, dim3(units), kTThreads, TileShape<DP>::kSmem, s, chained, p);
+    if (e != cudaSuccess || !p.per_seq || p.splits == 1) return e;
+    return launch_chained(join_tail<T>, dim3(static_cast<unsigned>((p.sms - 1) * (2 * kRowTile / kTailRows))), 128, 0, s,
+                          true, p);
 }
 
 }  // namespace
 
 cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq, int tiles, int splits,
-                                   bool direct, int64_t units, bool chained, cudaStream_t s) {
+                                   int sms, int64_t units, bool chained, cudaStream_t s) {
     TileParams p{};
     p.a = a;
-    p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.direct = direct;
+    p.per_seq = per_seq, p.tiles = tiles, p.splits = splits, p.sms = sms;
     if (a.P) {
         const int64_t n[4] = {a.D, a.P, a.Hkv, 1};
         p.tma_p = make_map(&p.kp, half, a.kp, n, {a.kp_t, a.kp_h, 0}, kTokTile, 1) &&
@@ -615,6 +746,9 @@ cudaError_t preload_attention_tile_kernels() {
     if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 64>(p, 0, false, nullptr, true);
     if (e == cudaSuccess) e = launch_tiles_dp<__half, 128>(p, 0, false, nullptr, true);
     if (e == cudaSuccess) e = launch_tiles_dp<__nv_bfloat16, 128>(p, 0, false, nullptr, true);
+    cudaFuncAttributes attr;
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, join_tail<__half>);
+    if (e == cudaSuccess) e = cudaFuncGetAttributes(&attr, join_tail<__nv_bfloat16>);
     return e;
 }
 

@@ -108,6 +108,7 @@ SHAPES = [
     ([257], [0], 1, 1, 128, 0, 4, 0),               # rows that see nothing
     ([1] * 40, list(range(40)), 14, 2, 128, 700, 40, 8),
     ([1] * 70, [3] * 70, 4, 4, 64, 300, 3, 0),
+    ([100] * 2 + [7, 0, 64] + [1] * 35 + [80], [100] * 2 + [9, 0, 70] + [3] * 35 + [300], 8, 2, 64, 400, 300, 0),
 ]
 
 
@@ -295,6 +296,14 @@ def test_two_captured_graphs_and_new_lengths(scb, ref):
     torch.cuda.synchronize()
     for c, o in zip(cases, outs):
         c.check(ref, *o)
+
+
+def test_more_units_than_multiprocessors(scb, ref):
+    """Whole rounds of units and a last one in parts."""
+    q_lens = [300, 64, 1, 257, 129, 400]
+    lens = [320, 64, 1, 300, 500, 401]
+    c = Case(24, torch.bfloat16, q_lens, lens, 32, 32, 64, 700, 500)
+    c.check(ref, *c.run(scb))
 
 
 def test_long_prefix_splits(scb):
