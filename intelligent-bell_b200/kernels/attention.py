@@ -16,7 +16,7 @@ import torch
 
 from .. import _lib
 from .paged import _status_word
-from .staging import step_arguments
+from .staging import Plans, step_arguments
 from .validation import require_apart, require_cuda, require_no_grad, same_view
 
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -139,6 +139,59 @@ def _on_device(what: str, tensors: list, device: torch.device) -> list:
     return [None if t is None else next(moved) for t in tensors]
 
 
+_LAYOUTS = Plans()
+_WORKSPACES = Plans()
+
+
+class _Layout:
+    """Sizes of a call and its tensors' strides in one host array."""
+
+    __slots__ = ("n", "hq", "hk", "d", "p_len", "rows", "cap", "array", "qs", "kps", "vps", "kcs", "vcs",
+                 "scale")
+
+    def __init__(self, q, k_prefix, v_prefix, k_cache, v_cache) -> None:
+        ref = k_prefix if k_prefix is not None else k_cache
+        if ref is None:
+            raise ValueError("neither a prefix nor caches given")
+        if (k_prefix is None) != (v_prefix is None) or (k_cache is None) != (v_cache is None):
+            raise ValueError("keys and values must be given together")
+        if ref.ndim < 2:
+            raise ValueError(f"keys must be [.., Hkv, D], got {tuple(ref.shape)}")
+        self.hk = hk = ref.shape[-2]
+        self.n, self.hq, self.d = _check_queries(q, hk)
+        d, dtype, dev = self.d, q.dtype, q.device
+        self.scale = 1.0 / math.sqrt(d)
+        strides = [*_rows3("q", q)]
+        self.p_len = self.rows = self.cap = 0
+        if k_prefix is not None:
+            self.p_len = k_prefix.shape[0]
+            shape = (self.p_len, hk, d)
+            _like("k_prefix", k_prefix, shape, dtype, dev)
+            _like("v_prefix", v_prefix, shape, dtype, dev)
+            strides += [*_rows3("k_prefix", k_prefix), *_rows3("v_prefix", v_prefix)]
+        else:
+            strides += [0] * 4
+        if k_cache is not None:
+            if k_cache.ndim != 4:
+                raise ValueError(f"caches must be [B, S, Hkv, D], got {tuple(k_cache.shape)}")
+            self.rows, self.cap = k_cache.shape[0], k_cache.shape[1]
+            shape = (self.rows, self.cap, hk, d)
+            _like("k_cache", k_cache, shape, dtype, dev)
+            _like("v_cache", v_cache, shape, dtype, dev)
+            strides += [*_rows4("k_cache", k_cache), *_rows4("v_cache", v_cache)]
+        self.array = (ctypes.c_int64 * 12)(*strides)
+        base = ctypes.addressof(self.array)
+        self.qs, self.kps, self.vps, self.kcs, self.vcs = (base + 8 * i for i in (0, 2, 4, 6, 9))
+
+
+def _aligned(*tensors) -> bool:
+    bits = 0
+    for t in tensors:
+        if t is not None:
+            bits |= t.data_ptr()
+    return not bits & 15
+
+
 def shared_prefix_attention(
     q: torch.Tensor,
     k_prefix: torch.Tensor | None,
@@ -177,34 +230,17 @@ def shared_prefix_attention(
     """
     require_cuda(q)
     require_no_grad("shared_prefix_attention", q, k_prefix, v_prefix, k_cache, v_cache, out)
-    dev = q.device
-    ref = k_prefix if k_prefix is not None else k_cache
-    if ref is None:
-        raise ValueError("neither a prefix nor caches given")
-    if (k_prefix is None) != (v_prefix is None) or (k_cache is None) != (v_cache is None):
-        raise ValueError("keys and values must be given together")
-    if ref.ndim < 2:
-        raise ValueError(f"keys must be [.., Hkv, D], got {tuple(ref.shape)}")
-    hk = ref.shape[-2]
-    n, hq, d = _check_queries(q, hk)
-    dtype = q.dtype
-    st = _lib.stride_buffer()
-    qs = st.put(_rows3("q", q))
-    p_len, kps, vps = 0, None, None
-    if k_prefix is not None:
-        p_len = k_prefix.shape[0]
-        shape = (p_len, hk, d)
-        _like("k_prefix", k_prefix, shape, dtype, dev)
-        _like("v_prefix", v_prefix, shape, dtype, dev)
-        kps, vps = st.put(_rows3("k_prefix", k_prefix)), st.put(_rows3("v_prefix", v_prefix))
-    batch, cap, page, n_pages, table, lens, kcs, vcs = 0, 0, 1, 0, None, None, None, None
+    dev, dtype = q.device, q.dtype
+    key = [q.shape, q.stride(), dtype, dev]
+    for t in (k_prefix, v_prefix, k_cache, v_cache):
+        key += (None,) if t is None else (t.shape, t.stride(), t.dtype, t.device)
+    key = tuple(key)
+    lay = _LAYOUTS.get(key)
+    if lay is None or not _aligned(q, k_prefix, v_prefix, k_cache, v_cache):
+        lay = _LAYOUTS.keep(key, _Layout(q, k_prefix, v_prefix, k_cache, v_cache))
+    n, hq, hk, d, p_len = lay.n, lay.hq, lay.hk, lay.d, lay.p_len
+    batch, cap, page, n_pages, table, lens = 0, 0, 1, 0, None, None
     if k_cache is not None:
-        if k_cache.ndim != 4:
-            raise ValueError(f"caches must be [B, S, Hkv, D], got {tuple(k_cache.shape)}")
-        shape = (k_cache.shape[0], k_cache.shape[1], hk, d)
-        _like("k_cache", k_cache, shape, dtype, dev)
-        _like("v_cache", v_cache, shape, dtype, dev)
-        kcs, vcs = st.put(_rows4("k_cache", k_cache)), st.put(_rows4("v_cache", v_cache))
         if page_table is not None:
             table = page_table if isinstance(page_table, torch.Tensor) else torch.as_tensor(page_table)
             if table.ndim != 2:
@@ -213,10 +249,10 @@ def shared_prefix_attention(
                 table = table.to(torch.int32)
             if table.stride(1) != 1 and table.shape[1] > 1:
                 table = table.contiguous()
-            batch, page, n_pages = table.shape[0], shape[1], shape[0]
+            batch, page, n_pages = table.shape[0], lay.cap, lay.rows
             cap = table.shape[1] * page
         else:
-            batch, cap = shape[0], shape[1]
+            batch, cap = lay.rows, lay.cap
             page = max(cap, 1)
         lens = _lengths("cache_lens", cache_lens, batch, cap)
     elif page_table is not None or cache_lens is not None:
@@ -231,28 +267,29 @@ def shared_prefix_attention(
     else:
         _like("out", out, (n, hq, d), dtype, dev)
         require_apart("out", out, q, k_prefix, v_prefix, k_cache, v_cache)
-    os = st.put(_rows3("out", out))
-    lse = torch.empty((n, hq), dtype=torch.float32, device=dev)
+    lse = q.new_empty((n, hq), dtype=torch.float32)
     if n == 0 or hq == 0:
         return out, lse
     table, lens, cu = _on_device("shared_prefix_attention", [table, lens, cu], dev)
     if scale is None:
-        scale = 1.0 / math.sqrt(d)
+        scale = lay.scale
     elif not math.isfinite(scale):
         raise ValueError(f"scale must be finite, got {scale}")
     lib = _lib.load()
-    size = ctypes.c_int64()
+    sizes = (n, batch, hq, hk, d, nq, p_len, cap, page)
+    need = _WORKSPACES.get(sizes)
+    if need is None:
+        size = ctypes.c_int64()
+        _lib.check(lib.sc_shared_prefix_attention_workspace(*sizes, ctypes.addressof(size)),
+                   "shared_prefix_attention")
+        need = _WORKSPACES.keep(sizes, size.value)
     with _lib.on_device(dev):
-        rc = lib.sc_shared_prefix_attention_workspace(n, batch, hq, hk, d, nq, p_len, cap, page,
-                                                      ctypes.addressof(size))
-        if rc:
-            _lib.check(rc, "shared_prefix_attention")
-        need = size.value
-        work = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        work = q.new_empty(need, dtype=torch.uint8) if need else None
+        os = _lib.stride_buffer().put(_rows3("out", out))
         rc = lib.sc_shared_prefix_attention(
-            n, batch, hq, hk, d, _lib.DTYPE_CODE[dtype], q.data_ptr(), qs,
-            p_len, _lib.ptr(k_prefix), kps, _lib.ptr(v_prefix), vps,
-            cap, _lib.ptr(k_cache), kcs, _lib.ptr(v_cache), vcs, _lib.ptr(lens),
+            n, batch, hq, hk, d, _lib.DTYPE_CODE[dtype], q.data_ptr(), lay.qs,
+            p_len, _lib.ptr(k_prefix), lay.kps, _lib.ptr(v_prefix), lay.vps,
+            cap, _lib.ptr(k_cache), lay.kcs, _lib.ptr(v_cache), lay.vcs, _lib.ptr(lens),
             _lib.ptr(table), table.stride(0) if table is not None else 0, page, n_pages,
             _lib.ptr(cu), nq, scale, out.data_ptr(), os, lse.data_ptr(),
             _lib.ptr(work), need, _status_word(dev).data_ptr(), _lib.stream_handle(dev))

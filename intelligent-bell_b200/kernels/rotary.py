@@ -9,6 +9,7 @@ the usual ways to scale the frequencies for contexts longer than the trained one
 
 from __future__ import annotations
 
+import ctypes
 import math
 from dataclasses import dataclass
 
@@ -17,7 +18,7 @@ import torch
 
 from .. import _lib
 from .restore import DEFAULT_THETA
-from .staging import step_arguments
+from .staging import Plans, step_arguments
 from .validation import require_apart, require_cuda, require_no_grad, same_view
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -132,6 +133,42 @@ def _layout(name: str, x: torch.Tensor) -> tuple[int, int, int, int, tuple[int, 
     raise ValueError(f"{name} must be [T, H, D] or [B, H, T, D], got {tuple(x.shape)}")
 
 
+class _Plan:
+    """What follows from the layouts of queries and keys alone: sizes, and strides (of the inputs
+    and of new contiguous outputs) in one host array."""
+
+    __slots__ = ("sizes", "code", "array", "q", "k", "fresh_q", "fresh_k")
+
+    def __init__(self, q: torch.Tensor, k: torch.Tensor | None, rotary_dim: int | None) -> None:
+        if q.dtype not in _DTYPES:
+            raise TypeError(f"q must be float16, bfloat16 or float32, got {q.dtype}")
+        self.code = _lib.DTYPE_CODE[q.dtype]
+        b, t, hq, d, qs = _layout("q", q)
+        hk, ks = 0, (0, 0, 0, 0)
+        if k is not None:
+            kb, kt, hk, kd, ks = _layout("k", k)
+            if (kb, kt, kd, k.ndim) != (b, t, d, q.ndim):
+                raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
+            if k.dtype != q.dtype:
+                raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
+            if k.device != q.device:
+                raise ValueError(f"k is on {k.device}, q on {q.device}")
+        rd = d if rotary_dim is None else int(rotary_dim)
+        if rd < 0 or rd % 2 or rd > d:
+            raise ValueError(f"rotary_dim must be even and at most head_dim {d}, got {rd}")
+        self.sizes = (b, t, hq, hk, d, rd)
+
+        def fresh(h: int) -> tuple[int, int, int, int]:  # (batch, token, head, element) strides
+            return (0, h * d, d, 1) if q.ndim == 3 else (h * t * d, d, t * d, 1)
+
+        self.array = (ctypes.c_int64 * 16)(*qs, *ks, *fresh(hq), *fresh(hk))
+        base = ctypes.addressof(self.array)
+        self.q, self.k, self.fresh_q, self.fresh_k = (base + 32 * i for i in range(4))
+
+
+_PLANS = Plans()
+
+
 def apply_rotary(
     q: torch.Tensor,
     k: torch.Tensor | None,
@@ -163,33 +200,22 @@ def apply_rotary(
     rounded once.  Returns ``q_out``, or ``(q_out, k_out)`` when keys are given.
     """
     require_cuda(q)
-    if q.dtype not in _DTYPES:
-        raise TypeError(f"q must be float16, bfloat16 or float32, got {q.dtype}")
     require_no_grad("apply_rotary", q, k, q_out, k_out)
     dev = q.device
-    b, t, hq, d, qs = _layout("q", q)
-    hk, ks = 0, None
-    if k is not None:
-        kb, kt, hk, kd, ks = _layout("k", k)
-        if (kb, kt, kd, k.ndim) != (b, t, d, q.ndim):
-            raise ValueError(f"k {tuple(k.shape)} does not match q {tuple(q.shape)}")
-        if k.dtype != q.dtype:
-            raise TypeError(f"k must be {q.dtype} like q, got {k.dtype}")
-        if k.device != dev:
-            raise ValueError(f"k is on {k.device}, q on {dev}")
-    elif k_out is not None:
+    key = (q.shape, q.stride(), q.dtype, rotary_dim,
+           None if k is None else (k.shape, k.stride(), k.dtype, k.device == dev))
+    plan = _PLANS.get(key) or _PLANS.keep(key, _Plan(q, k, rotary_dim))
+    if k is None and k_out is not None:
         raise ValueError("k_out given without k")
-    rd = d if rotary_dim is None else int(rotary_dim)
-    if rd < 0 or rd % 2 or rd > d:
-        raise ValueError(f"rotary_dim must be even and at most head_dim {d}, got {rd}")
-    outs = []
-    for name, x, out, other in (("q_out", q, q_out, k), ("k_out", k, k_out, q)):
-        if x is None:
-            outs.append(None)
-            continue
-        if out is None:
-            out = torch.empty_like(x, memory_format=torch.contiguous_format)
-        else:
+    b, t, hq, hk, d, rd = plan.sizes
+    qo = torch.empty_like(q, memory_format=torch.contiguous_format) if q_out is None else q_out
+    ko = k_out
+    if k is not None and k_out is None:
+        ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+    if q_out is not None or k_out is not None:
+        for name, x, out, given, other in (("q_out", q, qo, q_out, k), ("k_out", k, ko, k_out, q)):
+            if given is None:
+                continue
             if out.shape != x.shape or out.device != dev:
                 raise ValueError(f"{name} must have shape {tuple(x.shape)} on {dev}, "
                                  f"got {tuple(out.shape)} on {out.device}")
@@ -199,8 +225,6 @@ def apply_rotary(
                 require_apart(name, out)
             else:
                 require_apart(name, out, x, other)
-        outs.append(out)
-    qo, ko = outs
     if q_out is not None and k_out is not None and not (same_view(qo, q) and same_view(ko, k)):
         require_apart("k_out", ko, qo)
 
@@ -223,17 +247,14 @@ def apply_rotary(
     if b * t == 0 or d == 0:
         return qo if k is None else (qo, ko)
     _, freq_ptr, mult = _frequencies(rd, float(theta), scaling)
-    _, _, _, _, qos = _layout("q_out", qo)
-    kos = _layout("k_out", ko)[4] if ko is not None else None
     lib = _lib.load()
     st = _lib.stride_buffer()
+    qos = plan.fresh_q if q_out is None else st.put(_layout("q_out", qo)[4])
+    kos = None if ko is None else plan.fresh_k if k_out is None else st.put(_layout("k_out", ko)[4])
     with _lib.on_device(dev):
         rc = lib.sc_rope_apply(
-            b, t, hq, hk, d, rd, 1 if interleaved else 0,
-            q.data_ptr(), st.put(qs), _lib.ptr(k), st.put(ks) if ks else None,
-            _lib.DTYPE_CODE[q.dtype], pos_ptr, pos64, st.put(ps), start,
-            freq_ptr, mult, 1 if inverse else 0,
-            qo.data_ptr(), st.put(qos), _lib.ptr(ko), st.put(kos) if kos else None,
-            _lib.stream_handle(dev))
+            b, t, hq, hk, d, rd, 1 if interleaved else 0, q.data_ptr(), plan.q, _lib.ptr(k), plan.k, plan.code,
+            pos_ptr, pos64, st.put(ps), start, freq_ptr, mult, 1 if inverse else 0,
+            qo.data_ptr(), qos, _lib.ptr(ko), kos, _lib.stream_handle(dev))
     _lib.check(rc, "apply_rotary")
     return qo if k is None else (qo, ko)

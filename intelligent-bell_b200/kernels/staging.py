@@ -67,3 +67,15 @@ def step_arguments(what: str, tensors: list[torch.Tensor], device: torch.device)
         raise RuntimeError(f"{what}: host arguments cannot be captured into a CUDA graph; "
                            f"pass tensors on {device}")
     return to_device(tensors, device)
+
+
+class Plans(dict):
+    """What follows from shapes, strides and types alone (checked once, kept by them)."""
+
+    MOST = 512
+
+    def keep(self, key, plan):
+        if len(self) >= self.MOST:
+            self.clear()
+        self[key] = plan
+        return plan
