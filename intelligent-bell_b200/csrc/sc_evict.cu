@@ -86,8 +86,9 @@ __device__ __forceinline__ int warps_before(int x, int& total, int* s_warp) {
 template <int KPT>
 __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_constant__ SelectParams p) {
     __shared__ uint32_t s_hist[kBins];
+    __shared__ uint32_t s_all[2][kBins];  // the first block's: the cluster's histograms, in turn
     __shared__ int s_warp[3][kSelWarps];
-    __shared__ int s_pick[2];    // digit, equal ones still wanted
+    __shared__ int2 s_pick[2];   // digit, equal ones still wanted; in turn
     __shared__ int s_counts[2];  // this block's kept-for-sure and equal tokens
     let_next_start();
     cg::cluster_group cluster = cg::this_cluster();
@@ -99,8 +100,6 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
         else
             __syncthreads();
     };
-    // The cluster's histogram is the first block's.
-    uint32_t* all_hist = cluster.map_shared_rank(s_hist, 0);
     const int row = blockIdx.x / ranks;
     const int b = row / p.H, h = row - b * p.H;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -126,6 +125,11 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
         const int t = t0 + 32 * j;
         raw[j] = t >= lo && t < hi ? __ldg(scores + t) : 0.f;
     }
+    if (ranks > 1) {
+        if (rank == 0)
+            for (int i = threadIdx.x; i < kBins; i += kSelThreads) s_all[0][i] = 0;
+        cluster.sync();
+    }
     uint32_t keys[KPT];
 #pragma unroll
     for (int j = 0; j < KPT; ++j) keys[j] = order_key(raw[j]);
@@ -149,40 +153,35 @@ __global__ void __launch_bounds__(kSelThreads) select_tokens(const __grid_consta
         }
         if (ranks > 1) {
             __syncthreads();
-            uint32_t mine[kBins / kSelThreads];
-#pragma unroll
-            for (int j = 0; j < kBins / kSelThreads; ++j) mine[j] = s_hist[threadIdx.x + j * kSelThreads];
-            cluster.sync();  // the first block's own counts are complete, too
-            if (rank != 0) {
-#pragma unroll
-                for (int j = 0; j < kBins / kSelThreads; ++j)
-                    if (mine[j]) atomicAdd(&all_hist[threadIdx.x + j * kSelThreads], mine[j]);
+            uint32_t* all = cluster.map_shared_rank(s_all[pass & 1], 0);
+            for (int i = threadIdx.x; i < kBins; i += kSelThreads) {
+                if (s_hist[i]) atomicAdd(&all[i], s_hist[i]);
+                if (rank == 0) s_all[(pass + 1) & 1][i] = 0;  // last read a pass ago
             }
         }
         sync_all();
         if (rank == 0) {
             // Bins in descending order, two a thread.
             static_assert(kBins == 2 * kSelThreads, "two bins a thread");
+            const uint32_t* all = ranks > 1 ? s_all[pass & 1] : s_hist;
             const int bin = kBins - 1 - 2 * threadIdx.x;
-            const int n0 = static_cast<int>(s_hist[bin]), n1 = static_cast<int>(s_hist[bin - 1]);
+            const int n0 = static_cast<int>(all[bin]), n1 = static_cast<int>(all[bin - 1]);
             const int upto = warp_scan(n0 + n1, lane);
             int total;
             const int before =
                 warps_before(__shfl_sync(0xffffffffu, upto, 31), total, s_warp[0]) + upto - n0 - n1;
             if (want > 0 && before < want && before + n0 + n1 >= want) {
                 const bool second = before + n0 < want;
-                s_pick[0] = second ? bin - 1 : bin;
-                s_pick[1] = want - before - (second ? n0 : 0);
+                const int2 pick = make_int2(second ? bin - 1 : bin, want - before - (second ? n0 : 0));
+                for (int r = 0; r < ranks; ++r) *cluster.map_shared_rank(&s_pick[pass & 1], r) = pick;
             }
         }
         sync_all();
         if (want > 0) {
-            const int* pick = cluster.map_shared_rank(s_pick, 0);
-            const int digit = pick[0], left = pick[1];
-            key |= static_cast<uint32_t>(digit) << shift;
-            want = left;
+            const int2 pick = s_pick[pass & 1];
+            key |= static_cast<uint32_t>(pick.x) << shift;
+            want = pick.y;
         }
-        if (ranks > 1) cluster.sync();  // everybody has read the choice and the histogram
     }
     // Free tokens above `key` stay, and the first `want` equal to it (want = 0: none do).
     const int wanted = want;
