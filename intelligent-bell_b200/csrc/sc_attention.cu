@@ -503,6 +503,7 @@ struct Split {
     int32_t tiles_p, tiles_c;  // row tiles (of the kernel that takes them)
     int32_t chunk_p, n_pp, n_cp;
     int64_t units_tile, units_rows;
+    int32_t sms_left;  // SMs beside attend_tiles; 0: all, one kernel after the other
     int32_t least, blocks, s_pp, s_cp;  // attend_stream: steps and blocks, and its parts
 };
 
@@ -546,8 +547,23 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
     } else {
         if (s.tile_p) {
             s.tiles_p = static_cast<int32_t>((rows_p + kTileRows - 1) / kTileRows);
-            s.n_pp = plan_parts(static_cast<double>(s.tiles_p) * Hkv, (P + kTileTokens - 1) / kTileTokens,
-                                rows, D);
+            const double blocks = static_cast<double>(s.tiles_p) * Hkv;
+            const int64_t tile_steps = (P + kTileTokens - 1) / kTileTokens;
+            s.n_pp = plan_parts(blocks, tile_steps, rows, D);
+            if (cap) {
+                // attend_tiles on some SMs beside attend_stream on the others: both have some 10 us of
+                // start and end, which this way pass at the same time.  A stream block takes 1 us a step.
+                const double stream_steps = 0.75 * ((cap + kStepTokens - 1) / kStepTokens) * Hkv *
+                                            static_cast<double>(B) * ((rows_c + 31) / 32);
+                double best = -1.;
+                for (int32_t n = 1; n <= 64 && n <= tile_steps && blocks * n <= kSms - 16; ++n) {
+                    const int left = kSms - static_cast<int>(blocks * n);
+                    const double tile_us = 10.0 + static_cast<double>((tile_steps + n - 1) / n) * (D <= 64 ? 1.5 : 2.0);
+                    const double stream_us = 8.0 + stream_steps / (2.0 * left);
+                    const double cost = (tile_us > stream_us ? tile_us : stream_us) + n * rows * D * 8.0 / 5e6;
+                    if (best < 0. || cost < best) best = cost, s.n_pp = n, s.sms_left = left;
+                }
+            }
             s.direct = s.n_pp == 1 && !cap;
             s.units_tile = size_product(s.n_pp, s.tiles_p, Hkv);
         }
@@ -563,7 +579,7 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
         const int64_t steps_c = cap ? (cap + kStepTokens - 1) / kStepTokens : 0;
         const double steps = static_cast<double>(steps_p) * Hkv * s.tiles_p +
                              static_cast<double>(steps_c) * Hkv * B * s.tiles_c;
-        const int resident = 148 * (s.v.dp == 256 || (s.v.dp == 128 && s.v.mt == 2) ? 1 : 2);
+        const int resident = (s.sms_left ? s.sms_left : kSms) * (s.v.dp == 256 || (s.v.dp == 128 && s.v.mt == 2) ? 1 : 2);
         s.blocks = steps < 1 ? 0 : static_cast<int32_t>(steps < resident ? steps : resident);
         const int64_t longest_steps = steps_p > steps_c ? steps_p : steps_c;
         const double each = steps / resident;
@@ -727,32 +743,30 @@ extern "C" int32_t sc_shared_prefix_attention(
         const int64_t part_rows = s.fused ? static_cast<int64_t>(kSms) * kTileRows : (n_pp + n_cp) * rows;
         p.part_ml = reinterpret_cast<float2*>(p.part_o + part_rows * head_dim);
     };
-    const bool stream_first = !s.fused && s.blocks > 0;
-    set_parts(stream_first ? s.s_pp : s.n_pp, stream_first ? s.s_cp : s.n_cp);
+    const bool half = dtype == SC_DTYPE_F16, with_prefix = !s.tile_p && prefix_len > 0;
+    // Few rows: the streaming kernel, or attend_rows where tensor maps cannot say the layout (pages
+    // that no box of 8 rows divides, expanded strides).
+    StreamMaps maps{};
+    const bool streams = s.units_rows && s.blocks > 0 && make_stream_maps(p, half, with_prefix, &maps);
+    set_parts(streams ? s.s_pp : s.n_pp, streams ? s.s_cp : s.n_cp);
     p.out = out, p.o_t = out_strides[0], p.o_h = out_strides[1];
     p.lse = lse, p.status = status;
 
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     cudaError_t e = cudaSuccess;
-    const bool half = dtype == SC_DTYPE_F16;
-    // Few rows: the streaming kernel, or attend_rows where tensor maps cannot say the layout (pages
-    // that no box of 8 rows divides, expanded strides).
-    if (s.units_rows) {
-        bool taken = false;
-        if (stream_first)
-            e = launch_attention_stream(p, half, !s.tile_p && prefix_len > 0, s.v.dp, s.v.mt, s.least, s.blocks, st,
-                                        &taken);
-        if (e == cudaSuccess && !taken) {
-            set_parts(s.n_pp, s.n_cp);
-            e = half ? launch_rows_dp<__half>(p, s.v, s.units_rows, st)
-                     : launch_rows_dp<__nv_bfloat16>(p, s.v, s.units_rows, st);
-        }
-        if (e != cudaSuccess) return cuda_error(e, "attention launch");
-    }
     if (s.units_tile) {
         e = launch_attention_tiles(p, half, s.fused, s.fused ? s.tiles_c : s.tiles_p, s.n_pp, kSms,
-                                   s.units_tile, s.units_rows > 0, st);
+                                   s.units_tile, false, st);
         if (e != cudaSuccess) return cuda_error(e, "attention tiles launch");
+    }
+    if (s.units_rows) {
+        if (streams)
+            e = launch_attention_stream(p, maps, half, with_prefix, s.v.dp, s.v.mt, s.least, s.blocks,
+                                        s.units_tile > 0, st);
+        else
+            e = half ? launch_rows_dp<__half>(p, s.v, s.units_rows, st)
+                     : launch_rows_dp<__nv_bfloat16>(p, s.v, s.units_rows, st);
+        if (e != cudaSuccess) return cuda_error(e, "attention launch");
     }
     if (s.direct) return ok();
     const unsigned blocks = static_cast<unsigned>((rows + kWarps - 1) / kWarps);

@@ -152,10 +152,15 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
 cudaError_t preload_attention_tile_kernels();
 
 // The streaming kernel (sc_attention_stream.cu): few rows, parts of runs of 64-token steps, at least
-// `least` of them; dp: head_dim padded to 64, 128 or 256; mt: 16-row tiles.  *taken is false where
-// its tensor maps cannot say the layout, and nothing is launched.
-cudaError_t launch_attention_stream(const AttnParams& a, bool half, bool with_prefix, int dp, int mt, int least,
-                                    int blocks, cudaStream_t s, bool* taken);
+// `least` of them; dp: head_dim padded to 64, 128 or 256; mt: 16-row tiles.  make_stream_maps is
+// false where tensor maps cannot say the layout.
+struct StreamMaps {
+    alignas(64) unsigned char map[4][128];
+    int box;
+};
+bool make_stream_maps(const AttnParams& a, bool half, bool with_prefix, StreamMaps* m);
+cudaError_t launch_attention_stream(const AttnParams& a, const StreamMaps& m, bool half, bool with_prefix, int dp,
+                                    int mt, int least, int blocks, bool chained, cudaStream_t s);
 cudaError_t preload_attention_stream_kernels();
 
 }  // namespace sc

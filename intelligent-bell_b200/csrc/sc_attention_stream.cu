@@ -143,7 +143,10 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     int64_t run = (all + gridDim.x - 1) / gridDim.x;
     if (run < sp.least) run = sp.least;
     const int64_t g0 = blockIdx.x * run, g1 = min(all, g0 + run);
-    if (g0 >= g1) return;
+    if (g0 >= g1) {
+        wait_for_previous();
+        return;
+    }
 
     // Where a step lies.  first: the step at which its row tile begins.
     struct Place {
@@ -296,6 +299,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
         }
         cp_async_wait<0>();
         if (!alive) let_copies_land();
+        wait_for_previous();
         return;
     }
 
@@ -554,63 +558,66 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
         next_tile(x);
     }
     if (!alive && lane == 0 && p.status) atomicOr(p.status, SC_STATUS_WAIT_LIMIT);
+    wait_for_previous();  // nothing is read from it, but this kernel's end stands for its end, too
 }
 
 template <typename T, int DP, int MT>
-cudaError_t launch_stream(const StreamParams& p, unsigned blocks, cudaStream_t s, bool load_only) {
+cudaError_t launch_stream(const StreamParams& p, unsigned blocks, bool chained, cudaStream_t s, bool load_only) {
     using Shape = StreamShape<DP, MT>;
     auto kernel = attend_stream<T, DP, MT>;
     static std::atomic<uint64_t> done{0};
     cudaError_t e = allow_shared_memory(reinterpret_cast<const void*>(kernel), Shape::kSmem, done);
     if (e != cudaSuccess || load_only) return e;
-    kernel<<<blocks, kSThreads, Shape::kSmem, s>>>(p);
-    return cudaGetLastError();
+    return launch_chained(kernel, dim3(blocks), kSThreads, Shape::kSmem, s, chained, p);
 }
 
 template <typename T>
-cudaError_t launch_stream_dp(const StreamParams& p, int dp, int mt, unsigned blocks, cudaStream_t s, bool load_only) {
+cudaError_t launch_stream_dp(const StreamParams& p, int dp, int mt, unsigned blocks, bool chained, cudaStream_t s,
+                             bool load_only) {
     if (dp == 64)
-        return mt == 1 ? launch_stream<T, 64, 1>(p, blocks, s, load_only) : launch_stream<T, 64, 2>(p, blocks, s, load_only);
+        return mt == 1 ? launch_stream<T, 64, 1>(p, blocks, chained, s, load_only) : launch_stream<T, 64, 2>(p, blocks, chained, s, load_only);
     if (dp == 128)
-        return mt == 1 ? launch_stream<T, 128, 1>(p, blocks, s, load_only)
-                       : launch_stream<T, 128, 2>(p, blocks, s, load_only);
-    return launch_stream<T, 256, 1>(p, blocks, s, load_only);
+        return mt == 1 ? launch_stream<T, 128, 1>(p, blocks, chained, s, load_only)
+                       : launch_stream<T, 128, 2>(p, blocks, chained, s, load_only);
+    return launch_stream<T, 256, 1>(p, blocks, chained, s, load_only);
 }
 
 }  // namespace
 
-bool stream_maps_fit(const AttnParams& a, bool half, bool with_prefix, void* out) {
-    StreamParams& p = *static_cast<StreamParams*>(out);
+bool make_stream_maps(const AttnParams& a, bool half, bool with_prefix, StreamMaps* m) {
+    static_assert(sizeof(m->map[0]) == sizeof(CUtensorMap), "room for a map");
+    auto* map = reinterpret_cast<CUtensorMap*>(m->map);
     if (with_prefix) {
         const int64_t n[4] = {a.D, a.P, a.Hkv, 1};
-        if (!make_map(&p.kp, half, a.kp, n, {a.kp_t, a.kp_h, 0}, kStep, 1) ||
-            !make_map(&p.vp, half, a.vp, n, {a.vp_t, a.vp_h, 0}, kStep, 1))
+        if (!make_map(&map[0], half, a.kp, n, {a.kp_t, a.kp_h, 0}, kStep, 1) ||
+            !make_map(&map[1], half, a.vp, n, {a.vp_t, a.vp_h, 0}, kStep, 1))
             return false;
     }
-    p.box = kStep;
+    m->box = kStep;
     if (a.cap) {
         const bool paged = a.page_table != nullptr;
-        while (paged && a.page % p.box) p.box /= 2;
+        while (paged && a.page % m->box) m->box /= 2;
         const int64_t n[4] = {a.D, paged ? a.page : a.cap, a.Hkv, paged ? a.n_pages : a.B};
         // a box starts at a swizzle atom: 8 rows
-        if (p.box < 8 || (a.B + 31) / 32 > kMaxChunks ||
-            !make_map(&p.kc, half, a.kc, n, {a.kc_t, a.kc_h, a.kc_b}, p.box, 1) ||
-            !make_map(&p.vc, half, a.vc, n, {a.vc_t, a.vc_h, a.vc_b}, p.box, 1))
+        if (m->box < 8 || (a.B + 31) / 32 > kMaxChunks ||
+            !make_map(&map[2], half, a.kc, n, {a.kc_t, a.kc_h, a.kc_b}, m->box, 1) ||
+            !make_map(&map[3], half, a.vc, n, {a.vc_t, a.vc_h, a.vc_b}, m->box, 1))
             return false;
     }
     return true;
 }
 
-cudaError_t launch_attention_stream(const AttnParams& a, bool half, bool with_prefix, int dp, int mt, int least,
-                                    int blocks, cudaStream_t s, bool* taken) {
+cudaError_t launch_attention_stream(const AttnParams& a, const StreamMaps& m, bool half, bool with_prefix, int dp,
+                                    int mt, int least, int blocks, bool chained, cudaStream_t s) {
     StreamParams p{};
     p.a = a;
     p.least = least;
+    p.box = m.box;
     p.with_prefix = with_prefix;
-    *taken = stream_maps_fit(a, half, with_prefix, &p);
-    if (!*taken) return cudaSuccess;
-    return half ? launch_stream_dp<__half>(p, dp, mt, static_cast<unsigned>(blocks), s, false)
-                : launch_stream_dp<__nv_bfloat16>(p, dp, mt, static_cast<unsigned>(blocks), s, false);
+    const auto* map = reinterpret_cast<const CUtensorMap*>(m.map);
+    p.kp = map[0], p.vp = map[1], p.kc = map[2], p.vc = map[3];
+    return half ? launch_stream_dp<__half>(p, dp, mt, static_cast<unsigned>(blocks), chained, s, false)
+                : launch_stream_dp<__nv_bfloat16>(p, dp, mt, static_cast<unsigned>(blocks), chained, s, false);
 }
 
 cudaError_t preload_attention_stream_kernels() {
@@ -618,8 +625,8 @@ cudaError_t preload_attention_stream_kernels() {
     const int shapes[5][2] = {{64, 1}, {64, 2}, {128, 1}, {128, 2}, {256, 1}};
     cudaError_t e = cudaSuccess;
     for (const auto& x : shapes) {
-        if (e == cudaSuccess) e = launch_stream_dp<__half>(p, x[0], x[1], 0, nullptr, true);
-        if (e == cudaSuccess) e = launch_stream_dp<__nv_bfloat16>(p, x[0], x[1], 0, nullptr, true);
+        if (e == cudaSuccess) e = launch_stream_dp<__half>(p, x[0], x[1], 0, false, nullptr, true);
+        if (e == cudaSuccess) e = launch_stream_dp<__nv_bfloat16>(p, x[0], x[1], 0, false, nullptr, true);
     }
     return e;
 }

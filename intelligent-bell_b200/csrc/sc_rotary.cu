@@ -25,7 +25,7 @@
 namespace sc {
 namespace {
 
-constexpr int kRThreads = 256;
+constexpr int kRThreads = 128;
 constexpr int kMaxRotary = 512;       // frequencies travel as kernel parameters
 constexpr int kMaxTokensPerBlock = 32;
 constexpr int kTableEntries = 2048;   // float2 entries of the block's table
