@@ -112,18 +112,25 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
     if constexpr (std::is_same<T, __half>::value) {
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     } else {
-        asm volatile(
+        asm(
             "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, "
             "{%8,%9}, {%0,%1,%2,%3};"
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
             : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
+}
+
+// An 8 x 8 matrix of 16-bit values, two a lane, transposed.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+    uint32_t y;
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -152,7 +159,7 @@ cudaError_t launch_attention_tiles(const AttnParams& a, bool half, bool per_seq,
 cudaError_t preload_attention_tile_kernels();
 
 // The streaming kernel (sc_attention_stream.cu): few rows, parts of runs of 64-token steps, at least
-// `least` of them; dp: head_dim padded to 64, 128 or 256; mt: 16-row tiles.  make_stream_maps is
+// `least` of them; dp: head_dim padded to 64, 128 or 256; mt: 16-row tiles (0: one of 8 rows).  make_stream_maps is
 // false where tensor maps cannot say the layout.
 struct StreamMaps {
     alignas(64) unsigned char map[4][128];

@@ -24,12 +24,12 @@ constexpr int kMaxChunks = 256;  // of 32 sequences
 
 template <int DP, int MT>
 struct StreamShape {
-    static constexpr int kRows = 16 * MT;
+    static constexpr int kRows = MT == 0 ? 8 : 16 * MT;  // MT = 0: eight rows, see below
     static constexpr int kStageBytes = 2 * kStep * DP * 2;
     // Two blocks an SM but where registers or shared memory allow one.
     static constexpr int kBlocks = DP == 256 || (DP == 128 && MT == 2) ? 1 : 2;
-    static constexpr int kStages = DP == 64 ? (MT == 1 ? 6 : 5) : DP == 128 ? (MT == 1 ? 3 : 6) : 2;
-    static constexpr int kQueries = MT == 1 && DP < 256 ? 1 : 2;  // row tiles of queries in shared memory
+    static constexpr int kStages = DP == 64 ? (MT <= 1 ? 6 : 5) : DP == 128 ? (MT <= 1 ? 3 : 6) : 2;
+    static constexpr int kQueries = MT == 0 || (MT == 1 && DP < 256) ? 1 : 2;  // row tiles of queries in shared memory
     static constexpr int kQ = kRows * DP * 2;
     static constexpr int kJoin = 16 * DP * 4;
     static constexpr int kSmem = kStages * kStageBytes + kQueries * kQ + kJoin + 1024;
@@ -57,7 +57,9 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     using Shape = StreamShape<DP, MT>;
     constexpr int MR = Shape::kRows, NST = Shape::kStages, CPR = DP / 8;
     constexpr int STAGE = Shape::kStageBytes, QB = Shape::kQueries;
-    constexpr bool kHeld = MT == 1 && DP < 256;  // queries in registers
+    constexpr bool kEight = MT == 0;
+    constexpr bool kHeld = kEight || (MT == 1 && DP < 256);  // queries in registers
+    constexpr int MTN = MT == 0 ? 1 : MT;
     const AttnParams& p = sp.a;
     extern __shared__ unsigned char smem_raw[];
     __shared__ __align__(8) uint64_t s_bars[2 * NST + 2 * QB];
@@ -313,8 +315,15 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
         if (++qs == QB) qs = 0, q_phase ^= 1;
 
         // The queries of 16 rows stay in registers.
-        uint32_t qf[kHeld ? DP / 16 : 1][4];
-        if constexpr (kHeld) {
+        // (Eight rows: two registers of a product's second operand for each 16 columns.)
+        uint32_t qf[kEight ? DP / 32 : kHeld ? DP / 16 : 1][4];
+        if constexpr (kEight) {
+#pragma unroll
+            for (int kk = 0; kk < DP / 16; kk += 2)
+                ldmatrix4(qf[kk / 2], q_at + q_chunk<MR>(lane & 7, kk * 2 + (lane >> 3)));
+            __syncwarp();
+            if (lane == 0) bar_arrive(q_done);
+        } else if constexpr (kHeld) {
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk)
                 ldmatrix4(qf[kk], q_at + q_chunk<MR>(lane & 15, kk * 2 + (lane >> 4)));
@@ -322,22 +331,26 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             if (lane == 0) bar_arrive(q_done);
         }
 
-        float o[MT][DP / 8][4];
-        float m[MT][2], l[MT][2];
-        int lim[MT][2];  // tokens below it are seen
+        // 16 MT rows: o[mt][k] is 16 rows x 8 columns, row lane / 4 (+ 8).  Eight rows: the products are
+        // turned over, o[0][k] is 16 columns x 8 rows, rows 2 (lane % 4) and + 1, and half of the
+        // 16-row products' work and registers is gone.
+        constexpr int OK = kEight ? DP / 16 : DP / 8;
+        float o[MTN][OK][4];
+        float m[MTN][2], l[MTN][2];
+        int lim[MTN][2];  // tokens below it are seen
         const int see = x.len - x.n_tok;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int mt = 0; mt < MTN; ++mt) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 m[mt][e] = kNegInf;
                 l[mt][e] = 0.f;
-                const int r = mt * 16 + e * 8 + (lane >> 2);
+                const int r = kEight ? (lane & 3) * 2 + e : mt * 16 + e * 8 + (lane >> 2);
                 const int jq = static_cast<int>(fdiv(min(r0 + r, rows - 1), p.div_G));
                 lim[mt][e] = x.pre ? x.len : min(x.len, see + jq + 1);
             }
 #pragma unroll
-            for (int k = 0; k < DP / 8; ++k)
+            for (int k = 0; k < OK; ++k)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[mt][k][e] = 0.f;
         }
@@ -363,6 +376,73 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
+                if constexpr (kEight) {
+                    // S^T = K Q^T in two chains
+                    float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+#pragma unroll
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        uint32_t a[4];
+                        ldmatrix4(a, kt + kv_chunk<DP>(warp * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+                        mma16816<T>(s[kk & 1], a, qf[kk / 2][(kk & 1) * 2], qf[kk / 2][(kk & 1) * 2 + 1]);
+                    }
+                    float mx[2] = {m[0][0], m[0][1]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        float v = (s[0][e] + s[1][e]) * p.scale_log2;
+                        if (mask) {
+                            const int t = tt + (lane >> 2) + (e >> 1) * 8;
+                            bool seen = t < lim[0][e & 1];
+                            if (bad) seen = seen && !((bad >> ((t & (kStep - 1)) / sp.box)) & 1);
+                            if (!seen) v = kNegInf;
+                        }
+                        s[0][e] = v;
+                        mx[e & 1] = fmaxf(mx[e & 1], v);
+                    }
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], d));
+                        mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], d));
+                    }
+                    if (__any_sync(0xffffffffu, mx[0] > m[0][0] || mx[1] > m[0][1])) {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            const float f = mx[e] == kNegInf ? 1.f : exp2_fast(m[0][e] - mx[e]);
+                            m[0][e] = mx[e];
+                            l[0][e] *= f;
+#pragma unroll
+                            for (int k = 0; k < OK; ++k) {
+                                o[0][k][e] *= f;
+                                o[0][k][e + 2] *= f;
+                            }
+                        }
+                    }
+                    const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        s[0][e] = exp2_fast(s[0][e] - base[e & 1]);
+                        l[0][e & 1] += s[0][e];
+                    }
+                    // O^T += V^T P^T: the weights turned within the warp; for bfloat16 their rounding error
+                    // as a second product.
+                    uint32_t hi[2], lo[2];
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t w = pack2<T>(s[0][2 * e], s[0][2 * e + 1]);
+                        hi[e] = turn8x8(w);
+                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                            const float2 r = unpack2<T>(w);
+                            lo[e] = turn8x8(pack2<T>(s[0][2 * e] - r.x, s[0][2 * e + 1] - r.y));
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        uint32_t a[4];
+                        ldmatrix4_t(a, vt + kv_chunk<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                                         k * 2 + ((lane >> 3) & 1)));
+                        mma16816<T>(o[0][k], a, hi[0], hi[1]);
+                        if constexpr (std::is_same<T, __nv_bfloat16>::value) mma16816<T>(o[0][k], a, lo[0], lo[1]);
+                    }
+                } else {
                 float s[MT][2][4];
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
@@ -462,6 +542,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                         }
                     }
                 }
+                }
             }
             __syncwarp();
             if (lane == 0) bar_arrive(empty(stage));
@@ -474,14 +555,16 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
 
         // Join the four warps' states.
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MTN; ++mt)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 1);
-                l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], 2);
-                if ((lane & 3) == 0) {
-                    s_m[warp][mt * 16 + e * 8 + (lane >> 2)] = m[mt][e];
-                    s_l[warp][mt * 16 + e * 8 + (lane >> 2)] = l[mt][e];
+#pragma unroll
+                for (int d = kEight ? 4 : 1; d < (kEight ? 32 : 4); d <<= 1)
+                    l[mt][e] += __shfl_xor_sync(0xffffffffu, l[mt][e], d);
+                const int r = kEight ? lane * 2 + e : mt * 16 + e * 8 + (lane >> 2);
+                if (kEight ? lane < 4 : (lane & 3) == 0) {
+                    s_m[warp][r] = m[mt][e];
+                    s_l[warp][r] = l[mt][e];
                 }
             }
         auto meet = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
@@ -493,6 +576,55 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
         const bool last = x.j + n == x.steps;
         // Eight rows at a time, as a tree: warps 2 and 3 leave theirs, 0 and 1 add them, 1 leaves its sum,
         // 0 adds that and writes.  (Four warps in turn through one buffer: 6,300 clocks a part.)
+        if constexpr (kEight) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = (lane & 3) * 2 + e;
+                float top = s_m[0][r];
+#pragma unroll
+                for (int w = 1; w < kSWarps; ++w) top = fmaxf(top, s_m[w][r]);
+                const float f = m[0][e] == kNegInf ? 0.f : exp2_fast(m[0][e] - top);
+#pragma unroll
+                for (int k = 0; k < OK; ++k) {
+                    o[0][k][e] *= f;
+                    o[0][k][e + 2] *= f;
+                }
+            }
+            float4* slot = reinterpret_cast<float4*>(s_join) + (warp & 1) * (2 * DP) + lane;
+            auto leave = [&] {
+#pragma unroll
+                for (int k = 0; k < OK; ++k) slot[k * 32] = make_float4(o[0][k][0], o[0][k][1], o[0][k][2], o[0][k][3]);
+            };
+            auto take = [&](const float4* from) {
+#pragma unroll
+                for (int k = 0; k < OK; ++k) {
+                    const float4 v = from[k * 32];
+                    o[0][k][0] += v.x, o[0][k][1] += v.y, o[0][k][2] += v.z, o[0][k][3] += v.w;
+                }
+            };
+            if (warp >= 2) leave();
+            meet();
+            if (warp < 2) take(slot);
+            if (warp == 1) leave();
+            meet();
+            if (warp == 0) {
+                take(slot + 2 * DP);
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int r = (lane & 3) * 2 + e;
+                    if (r >= n_rows) continue;
+                    const int row = r0 + r, jq = static_cast<int>(fdiv(row, p.div_G));
+                    float* dst = p.part_o + (part * all_rows + static_cast<int64_t>(x.tok0 + jq) * p.Hq + x.h * p.G +
+                                             row - jq * p.G) * p.D + (lane >> 2);
+#pragma unroll
+                    for (int k = 0; k < OK; ++k) {
+                        if (k * 16 < p.D) dst[k * 16] = o[0][k][e];
+                        if (k * 16 + 8 < p.D) dst[k * 16 + 8] = o[0][k][e + 2];
+                    }
+                }
+            }
+            meet();
+        } else {
 #pragma unroll
         for (int half = 0; half < 2 * MT; ++half) {
             if (half * 8 >= n_rows) break;
@@ -540,6 +672,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             }
             meet();
         }
+        }
         for (int r = threadIdx.x; r < n_rows; r += 32 * kSWarps) {
             float top = s_m[0][r], sum = 0.f;
 #pragma unroll
@@ -574,6 +707,10 @@ cudaError_t launch_stream(const StreamParams& p, unsigned blocks, bool chained, 
 template <typename T>
 cudaError_t launch_stream_dp(const StreamParams& p, int dp, int mt, unsigned blocks, bool chained, cudaStream_t s,
                              bool load_only) {
+    if (mt == 0)
+        return dp == 64    ? launch_stream<T, 64, 0>(p, blocks, chained, s, load_only)
+               : dp == 128 ? launch_stream<T, 128, 0>(p, blocks, chained, s, load_only)
+                           : launch_stream<T, 256, 0>(p, blocks, chained, s, load_only);
     if (dp == 64)
         return mt == 1 ? launch_stream<T, 64, 1>(p, blocks, chained, s, load_only) : launch_stream<T, 64, 2>(p, blocks, chained, s, load_only);
     if (dp == 128)
@@ -622,7 +759,7 @@ cudaError_t launch_attention_stream(const AttnParams& a, const StreamMaps& m, bo
 
 cudaError_t preload_attention_stream_kernels() {
     StreamParams p{};
-    const int shapes[5][2] = {{64, 1}, {64, 2}, {128, 1}, {128, 2}, {256, 1}};
+    const int shapes[8][2] = {{64, 0}, {64, 1}, {64, 2}, {128, 0}, {128, 1}, {128, 2}, {256, 0}, {256, 1}};
     cudaError_t e = cudaSuccess;
     for (const auto& x : shapes) {
         if (e == cudaSuccess) e = launch_stream_dp<__half>(p, x[0], x[1], 0, false, nullptr, true);

@@ -98,6 +98,10 @@ SHAPES = [
     ([4], [9], 10, 2, 256, 90, 12, 0),
     ([1, 1], [300, 257], 5, 1, 96, 300, 300, 128),
     ([1, 1], [10, 10], 16, 1, 8, 20, 10, 0),
+    ([1, 1], [130, 77], 8, 1, 256, 70, 140, 16),    # eight rows and fewer
+    ([2, 1, 2], [65, 0, 3], 8, 2, 128, 130, 70, 24),
+    ([1, 1, 1], [64, 200, 1], 5, 1, 40, 0, 200, 0),
+    ([1] * 3, [1, 70, 129], 24, 2, 128, None, 130, 0),
     ([17, 31], [60, 31], 12, 4, 128, None, 64, 0),  # no prefix
     ([1, 1, 1], [0, 0, 0], 4, 2, 64, 0, 5, 0),      # nothing to see at all
     # many rows of a KV head: 256-row tiles
