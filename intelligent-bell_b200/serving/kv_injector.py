@@ -6,7 +6,7 @@ layer in a preallocated ``[B, H, capacity, D]`` buffer: ``update`` copies the ne
 in place instead of re-concatenating the whole layer (kv_injector.py:97-100), ``truncate``
 only moves the length (kv_injector.py:104-115), and the restore kernels write straight
 into ``append_views`` (the ``[T, H, D] -> [1, H, T, D]`` permute of kv_injector.py:222-232
-becomes store addressing).
+becomes store addressing).  ``evict`` cuts a layer to its heaviest tokens in place.
 
 ``MultiLayerKVInjector`` keeps the interface of kv_injector.py:136-498 over a
 ``KVRestorePipeline``: unified pinned slabs ``[L, blocks, chunk, H, D]`` with one
@@ -23,6 +23,7 @@ import torch
 
 from ..cache.pinned_pool import PinnedKVPool
 from ..cache.pipeline import KVRestorePipeline
+from ..kernels.evict import Evicted, evict_tokens
 from ..kernels.restore import dequant_kv_cache
 from ..kernels.shift import rope_shift_keys, token_major
 
@@ -121,8 +122,33 @@ class SpecDynamicCache:
         v = self._v[layer_idx][0, :, start:start + n_tokens].permute(1, 0, 2)
         return k, v
 
+    def append_slots(self, layer_idx: int, n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """``[B, H, n_tokens, D]`` views of the next tokens of every batch row, for a kernel to write
+        into; call :meth:`commit` once written."""
+        start = self._len[layer_idx]
+        return (self._k[layer_idx][:, :, start:start + n_tokens],
+                self._v[layer_idx][:, :, start:start + n_tokens])
+
     def commit(self, layer_idx: int, n_tokens: int) -> None:
         self._len[layer_idx] += int(n_tokens)
+
+    def evict(self, layer_idx: int, scores: torch.Tensor, budget: int, *, keep_first: int = 0,
+              keep_recent: int = 0) -> Evicted | None:
+        """Cut the layer to its ``budget`` heaviest tokens of each head, in place.
+
+        ``scores`` float32 ``[B, H, >= length]`` (accumulated attention weights) moves along.  None
+        when the layer holds no more than ``budget`` tokens; see :func:`evict_tokens`.
+        """
+        n, m = self._len[layer_idx], int(budget)
+        if n <= m:
+            return None
+        k = self._k[layer_idx][:, :, :n].transpose(1, 2)
+        v = self._v[layer_idx][:, :, :n].transpose(1, 2)
+        scores = scores[..., :n]
+        out = evict_tokens(k, v, scores, m, keep_first=keep_first, keep_recent=keep_recent,
+                           k_out=k[:, :m], v_out=v[:, :m], scores_out=scores[..., :m])
+        self._len[layer_idx] = m
+        return out
 
     def _append(self, layer_idx: int, like: torch.Tensor, t: int):
         b, h, _, d = like.shape
