@@ -491,47 +491,16 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     const int seen = (pre ? p.P : own_limit) - t0;  // columns below it count
                     const bool bad = !pre && *reinterpret_cast<volatile int*>(&s_any_bad) != 0;
                     const bool masked = __any_sync(0xffffffffu, seen < kTokTile) || bad;
-                    uint32_t x[128];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, x + c * 32);
-                    tmem_wait_ld();
-                    if (p.scale_log2 <= 0.f) {  // the order turns: scale before the maximum
-#pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            x[e] = __float_as_uint(__uint_as_float(x[e]) * p.scale_log2);
-                    }
-                    if (masked) {
-                        uint32_t on[4];  // a bit a column: this row sees it
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            const int n = seen - c * 32;
-                            on[c] = n >= 32 ? 0xffffffffu : n <= 0 ? 0u : (1u << n) - 1u;
-                            if (bad)
-                                for (int e = 0; e < 32; ++e)
-                                    if (!s_ok[i & 3][c * 32 + e]) on[c] &= ~(1u << e);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            if (!((on[e >> 5] >> (e & 31)) & 1)) x[e] = __float_as_uint(kNegInf);
-                    }
-                    float top = kNegInf;
-                    {
-                        float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-                        for (int e = 0; e < 128; e += 2)
-                            t4[(e >> 1) & 3] = max3(t4[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
-                        top = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3]));
-                    }
-                    const float mul = p.scale_log2 > 0.f ? p.scale_log2 : 1.f;
-                    top *= mul;
-                    const bool raise = top > m + kRaise || (m == kNegInf && top > m);
-                    if (__any_sync(0xffffffffu, raise)) {
+                    // A score above the maximum in use by 2^8 raises it, and O with it.
+                    auto raised = [&](float top) {
+                        const bool raise = top > m + kRaise || (m == kNegInf && top > m);
+                        if (!__any_sync(0xffffffffu, raise)) return;
                         const float f = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
                         if (i > 0) {
                             alive = bar_wait_warp(o_full(q), (i - 1) & 1, gave_up);
-                            if (!alive) break;
+                            if (!alive) return;
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < DP / 32; ++c) {
@@ -543,29 +512,87 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                                 tmem_st32(o_at + c * 32, o);
                             }
                         }
-                    }
-                    const float base = m == kNegInf ? 0.f : m;
-                    const float2 mul2 = make_float2(mul, mul), sub2 = make_float2(-base, -base);
-                    float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+                    };
+                    if (!masked && p.scale_log2 > 0.f) {
+                        // All scores in registers, one pass.
+                        uint32_t x[128];
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[16];
+                        for (int c = 0; c < 4; ++c) tmem_ld32(s_at + c * 32, x + c * 32);
+                        tmem_wait_ld();
+                        float t4[4] = {kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-                        for (int e = 0; e < 16; ++e) {
-                            float2 v = make_float2(__uint_as_float(x[c * 32 + 2 * e]),
-                                                   __uint_as_float(x[c * 32 + 2 * e + 1]));
-                            v = __ffma2_rn(v, mul2, sub2);
-                            v.x = exp2_fast(v.x);
-                            v.y = exp2_fast(v.y);
-                            if (e & 1)
-                                sum2 = __fadd2_rn(sum2, v);
-                            else
-                                sum = __fadd2_rn(sum, v);
-                            w[e] = pack2<T>(v.x, v.y);  // 16-bit weights, as the product takes them
+                        for (int e = 0; e < 128; e += 2)
+                            t4[(e >> 1) & 3] = max3(t4[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
+                        raised(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2);
+                        if (!alive) break;
+                        const float base = m == kNegInf ? 0.f : m;
+                        const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                        float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                float2 v = make_float2(__uint_as_float(x[c * 32 + 2 * e]),
+                                                       __uint_as_float(x[c * 32 + 2 * e + 1]));
+                                v = __ffma2_rn(v, mul2, sub2);
+                                v.x = exp2_fast(v.x);
+                                v.y = exp2_fast(v.y);
+                                if (e & 1)
+                                    sum2 = __fadd2_rn(sum2, v);
+                                else
+                                    sum = __fadd2_rn(sum, v);
+                                w[e] = pack2<T>(v.x, v.y);  // 16-bit weights, as the product takes them
+                            }
+                            tmem_st16(s_at + c * 16, w);
                         }
-                        tmem_st16(s_at + c * 16, w);
+                        l += (sum.x + sum.y) + (sum2.x + sum2.y);
+                    } else {
+                        // A tile's end, a mask, or a scale that turns the order: the few of these take short
+                        // loops, which leave the others' instructions together (a kernel of 131,072
+                        // tokens and 512 rows a head: 459 -> 452 us).
+                        const bool turned = p.scale_log2 <= 0.f;
+                        const float mul = turned ? 1.f : p.scale_log2;
+                        auto scores = [&](int c, uint32_t (&x)[16]) {  // 16 columns, what is hidden -inf
+                            tmem_ld16(s_at + c, x);
+                            tmem_wait_ld();
+                            uint32_t on = 0;
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) on |= (c + e < seen ? 1u : 0u) << e;
+                            if (bad)
+                                for (int e = 0; e < 16; ++e)
+                                    if (!s_ok[i & 3][c + e]) on &= ~(1u << e);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) {
+                                const float v = __uint_as_float(x[e]) * (turned ? p.scale_log2 : 1.f);
+                                x[e] = __float_as_uint((on >> e) & 1 ? v : kNegInf);
+                            }
+                        };
+                        float top = kNegInf;
+#pragma unroll 1
+                        for (int c = 0; c < kTokTile; c += 16) {
+                            uint32_t x[16];
+                            scores(c, x);
+#pragma unroll
+                            for (int e = 0; e < 16; ++e) top = fmaxf(top, __uint_as_float(x[e]));
+                        }
+                        raised(top * mul);
+                        if (!alive) break;
+                        const float base = m == kNegInf ? 0.f : m;
+#pragma unroll 1
+                        for (int c = 0; c < kTokTile; c += 16) {
+                            uint32_t x[16], w[8];
+                            scores(c, x);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float v0 = exp2_fast(fmaf(__uint_as_float(x[2 * e]), mul, -base));
+                                const float v1 = exp2_fast(fmaf(__uint_as_float(x[2 * e + 1]), mul, -base));
+                                l += v0 + v1;
+                                w[e] = pack2<T>(v0, v1);
+                            }
+                            tmem_st8(s_at + c / 2, w);  // over columns already read
+                        }
                     }
-                    l += (sum.x + sum.y) + (sum2.x + sum2.y);
                     tmem_wait_st();
                 }
                 tc_fence_before();
@@ -591,6 +618,18 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 // took 5 us of a block's time.
                 const uint32_t stage = s_q + q * TILE + (warp & 3) * (TILE / 4);
                 const int per = direct ? 64 : 32;  // columns a pass
+                char* dst[8];  // a lane's part of eight rows
+#pragma unroll
+                for (int it = 0; it < 8; ++it) {
+                    const int row2 = r0 + q * kRowTile + (warp & 3) * 32 + it * 4 + sub;
+                    dst[it] = nullptr;
+                    if (row2 < r0 + n_rows) {
+                        const int j2 = static_cast<int>(fdiv(row2, p.div_G)), head = h * p.G + row2 - j2 * p.G;
+                        dst[it] = direct ? reinterpret_cast<char*>(static_cast<T*>(p.out) + (tok0 + j2) * p.o_t + head * p.o_h)
+                                         : reinterpret_cast<char*>(p.part_o + part_at(row2 - r0) * p.D);
+                        dst[it] += c8 * 16;
+                    }
+                }
 #pragma unroll 1
                 for (int c = 0; c < DP; c += per) {
                     uint32_t o[64];
@@ -613,19 +652,11 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
 #pragma unroll
                     for (int it = 0; it < 8; ++it) {
                         const int rr = it * 4 + sub;
-                        const int row2 = r0 + q * kRowTile + (warp & 3) * 32 + rr;
                         uint4 v;
                         asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
                                      : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                                      : "r"(stage + rr * 128 + ((c8 ^ (rr & 7)) << 4)));
-                        if (row2 < r0 + n_rows && col < p.D) {
-                            const int j2 = static_cast<int>(fdiv(row2, p.div_G));
-                            const int head = h * p.G + row2 - j2 * p.G;
-                            if (direct)
-                                st_v4(static_cast<T*>(p.out) + (tok0 + j2) * p.o_t + head * p.o_h + col, v);
-                            else
-                                st_v4(p.part_o + part_at(row2 - r0) * p.D + col, v);
-                        }
+                        if (dst[it] != nullptr && col < p.D) st_v4(dst[it] + c * (direct ? 2 : 4), v);
                     }
                     __syncwarp();
                 }

@@ -157,6 +157,11 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
+__device__ __forceinline__ void tmem_st8(uint32_t addr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(addr),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
@@ -169,27 +174,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     float y;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(y) : "f"(a), "f"(b), "f"(c));
     return y;
-}
-// 2^x of two values without the exponential unit, for x <= 127; NaN stays NaN.  x = n + f with n
-// the nearest integer (read off the low bits of x + 1.5 * 2^23) and |f| <= 1/2; 2^f by a
-// polynomial of degree 5, fitted for relative error (7.5e-8) at Chebyshev nodes; 2^n made of its
-// exponent bits.  Below 2^-126 the result is 2^-126.
-__device__ __forceinline__ float2 exp2_poly(float2 x) {
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.x));  // -126
-    asm("max.NaN.f32 %0, %0, 0fC2FC0000;" : "+f"(x.y));
-    const float2 magic = make_float2(12582912.f, 12582912.f);
-    const float2 t = __fadd2_rn(x, magic);
-    const float2 n = __fadd2_rn(t, make_float2(-12582912.f, -12582912.f));
-    const float2 f = __ffma2_rn(n, make_float2(-1.f, -1.f), x);
-    float2 y = __ffma2_rn(f, make_float2(1.3276461977511644e-3f, 1.3276461977511644e-3f),
-                          make_float2(9.675540961325169e-3f, 9.675540961325169e-3f));
-    y = __ffma2_rn(y, f, make_float2(5.550713464617729e-2f, 5.550713464617729e-2f));
-    y = __ffma2_rn(y, f, make_float2(0.24022120237350464f, 0.24022120237350464f));
-    y = __ffma2_rn(y, f, make_float2(0.6931469440460205f, 0.6931469440460205f));
-    y = __ffma2_rn(y, f, make_float2(1.0000001192092896f, 1.0000001192092896f));
-    const float2 scale = make_float2(__uint_as_float((__float_as_uint(t.x) << 23) + 0x3f800000u),
-                                     __uint_as_float((__float_as_uint(t.y) << 23) + 0x3f800000u));
-    return __fmul2_rn(y, scale);
 }
 __device__ __forceinline__ void tmem_wait_ld() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -227,10 +211,9 @@ inline EncodeTiled encode_tiled() {
 }
 
 // A map of [n3][n2][n1][n0] 16-bit elements (strides in elements) in boxes of 64 columns x `rows` x
-// `rows2`.
-// False where a map cannot say it: the kernel then copies without one.
-inline bool make_map(CUtensorMap* map, bool half, const void* base, const int64_t (&n)[4], const int64_t (&st)[3],
-              int rows, int rows2) {
+// `rows2`.  False where a map cannot say it: the kernel then copies without one.
+inline bool make_map(CUtensorMap* map, bool half, const void* base, const int64_t (&n)[4],
+                     const int64_t (&st)[3], int rows, int rows2) {
     const EncodeTiled encode = encode_tiled();
     if (!encode) return false;
     cuuint64_t dims[4], strides[3];
@@ -244,7 +227,8 @@ inline bool make_map(CUtensorMap* map, bool half, const void* base, const int64_
         if (s <= 0 || s % 8 || s * 2 >= (int64_t(1) << 40)) return false;
         strides[i] = static_cast<cuuint64_t>(s * 2);
     }
-    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(rows2), 1}, step[4] = {1, 1, 1, 1};
+    const cuuint32_t box[4] = {64, static_cast<cuuint32_t>(rows), static_cast<cuuint32_t>(rows2), 1};
+    const cuuint32_t step[4] = {1, 1, 1, 1};
     return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                   const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
                   CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
