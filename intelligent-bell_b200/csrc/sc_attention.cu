@@ -8,6 +8,15 @@
 // together: rows of one KV head are packed (token, head of the group) over the whole batch, so a
 // prefix token is loaded once for 16 or 32 rows instead of once per sequence.
 //
+// Three kernels write parts, by the rows that one KV head has in common (plan_split):
+//   attend_tiles (sc_attention_tile.cu)    64 rows and more over the prefix, 96 and more of one
+//                                          sequence over prefix and own cache: tensor memory;
+//   attend_stream (sc_attention_stream.cu) fewer: HBM bounds it;
+//   attend_rows (here)                     what tensor maps cannot say: pages that no box of 8 rows
+//                                          divides, expanded strides, more than 8,192 sequences.
+// 64 sequences of one token, 32 query heads of 128 on 8 KV heads, 8,192 shared tokens, own caches
+// of up to 512: 45 us, of which reading everything once takes 16.
+//
 // attend_rows: 16 * MT rows of one KV head against one part.  The four warps take turns at tiles
 // of TK tokens; each keeps its own ring of tiles in shared memory (cp.async, 16 bytes a lane),
 // its own softmax state and its own 16-bit-input, fp32-accumulating matrix products, and the
@@ -23,6 +32,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
+constexpr int kSms = 148;          // blocks of attend_tiles at a time
 constexpr int kPartTokens = 64;    // parts are multiples of this many tokens
 constexpr int kMaxPagesPerPart = 2048;
 
@@ -49,6 +59,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     __shared__ int32_t s_page[kMaxPagesPerPart];
     __shared__ float s_m[kWarps][MR], s_l[kWarps][MR];
     __shared__ int s_bad;
+    __shared__ int s_odd[2 * DP], s_any_odd;
 
     let_next_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -112,7 +123,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     }
     const bool paged = !is_prefix && p.page_table != nullptr;
     int first_page = 0;
-    if (threadIdx.x == 0) s_bad = 0;
+    if (threadIdx.x == 0) s_bad = s_any_odd = 0;
+    for (int i = threadIdx.x; i < 2 * DP; i += kThreads) s_odd[i] = kNoToken;
     if (paged || p.D < DP) __syncthreads();
     if (paged) {
         first_page = static_cast<int>(fdiv(t0, p.div_page));
@@ -216,7 +228,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
     }
     // Tiles that end below it are seen whole by every row.
-    const int whole = bad ? -1 : is_prefix ? t1 : min(t1, see + static_cast<int>(fdiv(r0, p.div_G)) + 1);
+    const int seen_whole = is_prefix ? t1 : min(t1, see + static_cast<int>(fdiv(r0, p.div_G)) + 1);
+    const int whole = bad ? -1 : seen_whole;
 
     const uint32_t q_addr = smem_addr(s_q);
     for (int i = 0; i < my_tiles; ++i) {
@@ -298,6 +311,11 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
                     l[mt][e >> 1] += w;
                 }
         }
+        if (!is_prefix && tt + TK > seen_whole && seen_whole < t1) {  // some rows do not see some of the tokens
+            for (int c = lane; c < TK * CPR; c += 32)
+                take_out_odd<T>(vt + chunk_at<DP>(c / CPR, c % CPR), tt + c / CPR, s_odd + c % CPR * 8, DP, &s_any_odd);
+            __syncwarp();
+        }
         // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
         // rounding error goes in as a second product, since this kernel waits for memory and
         // the products are free.
@@ -377,6 +395,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
         const int64_t at = part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
         *reinterpret_cast<float4*>(p.part_o + at * p.D + c) = acc;
     }
+    const bool odd = s_any_odd != 0;
+    if (odd) __syncthreads();
     for (int r = threadIdx.x; r < n_rows; r += kThreads) {
         float all = s_m[0][r], sum = 0.f;
 #pragma unroll
@@ -385,8 +405,9 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
         for (int w = 0; w < kWarps; ++w)
             sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - all));
         const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
-        p.part_ml[part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G] =
-            make_float2(all, sum);
+        const int64_t at = part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
+        p.part_ml[at] = make_float2(all, sum);
+        if (odd) add_odd(p.part_o + at * p.D, p.D, s_odd, DP, min(t1, see + j + 1));
     }
 }
 
@@ -471,7 +492,7 @@ __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ A
 // 11 -> 5 us, but 2,048 rows of 12 parts 5 -> 8.
 template <typename T>
 cudaError_t launch_join(const AttnParams& p, int64_t rows, bool chained, cudaStream_t s) {
-    if (rows >= 148 * 8 || p.n_pp + p.n_cp < 4)
+    if (rows >= kSms * 8 || p.n_pp + p.n_cp < 4)
         return launch_chained(join_parts<T, 1>, dim3(static_cast<unsigned>((rows + kWarps - 1) / kWarps)), kThreads,
                               0, s, chained, p);
     return launch_chained(join_parts<T, kWarps>, dim3(static_cast<unsigned>(rows)), kThreads, 0, s, chained, p);
@@ -539,7 +560,6 @@ struct Split {
 
 constexpr int kTileRows = 256, kTileTokens = 128, kStepTokens = 64;
 constexpr int kMinTileRows = 64;   // fewer rows: the copies bound both kernels
-constexpr int kSms = 148;          // blocks of attend_tiles at a time
 constexpr int kTailParts = 16;     // of a unit in the last round, at most
 constexpr int kMaxFused = 1024;    // sequences: every block counts their units
 constexpr int kMinFusedRows = 96;  // fewer rows a sequence: packing the batch's rows wins
@@ -597,9 +617,9 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
             s.direct = s.n_pp == 1 && !cap;
             s.units_tile = size_product(s.n_pp, s.tiles_p, Hkv);
         }
-        s.v = pick_variant(D, !P || s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c);
-        const int64_t mr = 16 * s.v.mt;
         const int64_t rows_most = !P || s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c;
+        s.v = pick_variant(D, rows_most);
+        const int64_t mr = 16 * s.v.mt;
         s.stream_mt = rows_most <= 8 ? 0 : s.v.mt;
         const int32_t P_rows = s.tile_p ? 0 : P;
         if (!s.tile_p) s.tiles_p = static_cast<int32_t>((rows_p + mr - 1) / mr);
@@ -609,6 +629,9 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
         // at least, and long enough that a row tile has 64 parts at most.
         const int64_t steps_p = (P_rows + kStepTokens - 1) / kStepTokens;
         const int64_t steps_c = cap ? (cap + kStepTokens - 1) / kStepTokens : 0;
+        // (32 sequences' steps are counted in 32 bits)
+        if (size_product(size_product(B < 32 ? B : 32, Hkv), s.tiles_c * 2 * s.v.mt, steps_c) >= (int64_t(1) << 31))
+            return set_error(SC_ERR_INVALID_ARGUMENT, "too many rows and tokens in one call; split it");
         const double steps = static_cast<double>(steps_p) * Hkv * s.tiles_p +
                              static_cast<double>(steps_c) * Hkv * B * s.tiles_c;
         const int resident = (s.sms_left ? s.sms_left : kSms) * (s.v.dp == 256 || (s.v.dp == 128 && s.v.mt == 2) ? 1 : 2);
@@ -625,7 +648,7 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
         // attend_rows: two blocks fit an SM; two rounds of equal parts.
         const double work = static_cast<double>(P_rows) * Hkv * s.tiles_p +
                             static_cast<double>(cap) * Hkv * B * s.tiles_c;
-        double chunk = ceil(work / (148.0 * 2 * 2) / kPartTokens) * kPartTokens;
+        double chunk = ceil(work / (kSms * 2 * 2) / kPartTokens) * kPartTokens;
         const double longest = P_rows > cap ? P_rows : cap;
         const double most_parts = 64;
         if (chunk < longest / most_parts) chunk = ceil(longest / most_parts / kPartTokens) * kPartTokens;
@@ -718,7 +741,8 @@ extern "C" int32_t sc_shared_prefix_attention(
     if (rc != SC_OK) return rc;
     if (dtype != SC_DTYPE_F16 && dtype != SC_DTYPE_BF16)
         return set_error(SC_ERR_INVALID_DTYPE, "dtype code %d: float16 or bfloat16", dtype);
-    if (!isfinite(scale)) return set_error(SC_ERR_INVALID_ARGUMENT, "scale must be finite, got %g", scale);
+    if (!isfinite(static_cast<float>(scale * 1.4426950408889634)))
+        return set_error(SC_ERR_INVALID_ARGUMENT, "scale must be finite in float32, got %g", scale);
     if (n_tokens == 0 || q_heads == 0) return ok();
     if (!cu_q_lens && batch && n_tokens != max_q_len * batch)
         return set_error(SC_ERR_INVALID_ARGUMENT, "%lld tokens are not %d sequences of %lld",

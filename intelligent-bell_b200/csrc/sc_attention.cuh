@@ -170,4 +170,57 @@ cudaError_t launch_attention_stream(const AttnParams& a, const StreamMaps& m, bo
                                     int mt, int least, int blocks, bool chained, cudaStream_t s);
 cudaError_t preload_attention_stream_kernels();
 
+// ---- values that are not finite ----
+// A token that some rows of a tile do not see has weight zero there, and 0 x infinity would be NaN.  So
+// where a tile holds such tokens, values that are not finite leave the product: zeros take their
+// place, the first token with +infinity and with -infinity (NaN: both) is kept for each column, and
+// the rows that see it get them at the end.
+constexpr int kNoToken = 0x7fffffff;
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t at) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+    return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t at, uint4 v) {
+    asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(at), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w)
+                 : "memory");
+}
+// Two values with those that are not finite (all exponent bits set) made zero.
+template <typename T>
+__device__ __forceinline__ uint32_t finite_part(uint32_t v) {
+    constexpr uint32_t e = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    if ((v & e) == e) v &= 0xffff0000u;
+    if ((v >> 16 & e) == e) v &= 0xffffu;
+    return v;
+}
+template <typename T>
+__device__ __forceinline__ uint4 finite_part(uint4 v) {
+    return make_uint4(finite_part<T>(v.x), finite_part<T>(v.y), finite_part<T>(v.z), finite_part<T>(v.w));
+}
+// One chunk (8 columns) of a token's values in shared memory; first: those columns of kNoToken-filled
+// [2][columns].  Out of line: what it costs where nothing is odd is a load and a few comparisons.
+template <typename T>
+__device__ __noinline__ void take_out_odd(uint32_t at, int token, int* first, int columns, int* any) {
+    const uint4 v = ld_shared_v4(at), f = finite_part<T>(v);
+    if (f.x == v.x && f.y == v.y && f.z == v.z && f.w == v.w) return;
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const float2 x2 = unpack2<T>(w[e / 2]);
+        const float x = e & 1 ? x2.y : x2.x;
+        if (isfinite(x)) continue;
+        if (!(x < 0.f)) atomicMin(first + e, token);
+        if (!(x > 0.f)) atomicMin(first + columns + e, token);
+    }
+    st_shared_v4(at, f);
+    *any = 1;
+}
+// Row of sums `o` that sees the tokens below `limit`.
+static __device__ __noinline__ void add_odd(float* o, int n, const int* first, int columns, int limit) {
+    for (int c = 0; c < n; ++c) {
+        if (first[c] < limit) o[c] += -kNegInf;
+        if (first[columns + c] < limit) o[c] += kNegInf;
+    }
+}
+
 }  // namespace sc

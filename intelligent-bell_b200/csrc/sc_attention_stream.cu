@@ -9,7 +9,8 @@
 // first keys.  Warps 0-3 take 16 of a step's tokens each, with a softmax state of their own
 // (16-bit-input matrix products, fp32 sums), joined when the part ends.
 // (Blocks of one part, cp.async by every warp with its address arithmetic: 750 instructions for
-// 16 tokens, 4.7 TB/s at best and 33 us for the 64 ragged caches that now take NN.)
+// 16 tokens, 4.7 TB/s at best and 33 us for 64 ragged caches of up to 1,024
+// tokens; this way 19.)
 #include <math.h>
 
 #include "sc_tensor.cuh"
@@ -67,6 +68,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     __shared__ int s_bad[NST];  // a bit a box of a step: its page is not there
     __shared__ int s_gave_up;
     __shared__ float s_m[kSWarps][MR], s_l[kSWarps][MR];
+    __shared__ int s_odd[2 * DP], s_any_odd;
 
     let_next_start();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -114,8 +116,10 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             bar_init(q_empty(s), kSWarps);
         }
         s_gave_up = 0;
+        s_any_odd = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    for (int i = threadIdx.x; i < 2 * DP; i += kSThreads) s_odd[i] = kNoToken;
     // Steps of 32 sequences at a time (of one KV head).
     const int chunks = p.cap ? (p.B + 31) / 32 : 0;
     for (int c = warp; c < chunks; c += kSThreads / 32) {
@@ -376,6 +380,14 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
                 }
+                if (whole < x.len && tt + 16 > whole) {  // some rows do not see some of the tokens
+                    for (int i2 = lane; i2 < 16 * CPR; i2 += 32) {
+                        const int r = i2 / CPR, c = i2 - r * CPR;
+                        take_out_odd<T>(vt + kv_chunk<DP>(warp * 16 + r, c), tt + r, s_odd + c * 8, DP, &s_any_odd);
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
                 if constexpr (kEight) {
                     // S^T = K Q^T in two chains
                     float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
@@ -443,105 +455,105 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                         if constexpr (std::is_same<T, __nv_bfloat16>::value) mma16816<T>(o[0][k], a, lo[0], lo[1]);
                     }
                 } else {
-                float s[MT][2][4];
+                    float s[MT][2][4];
 #pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
+                    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int k = 0; k < 2; ++k)
+                        for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) s[mt][k][e] = 0.f;
+                            for (int e = 0; e < 4; ++e) s[mt][k][e] = 0.f;
 #pragma unroll
-                for (int kk = 0; kk < DP / 16; ++kk) {
-                    uint32_t kb[4];
-                    ldmatrix4(kb, kt + kv_chunk<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3),
-                                                    kk * 2 + ((lane >> 3) & 1)));
-                    if constexpr (kHeld) {
-                        mma16816<T>(s[0][0], qf[kk], kb[0], kb[1]);
-                        mma16816<T>(s[0][1], qf[kk], kb[2], kb[3]);
-                    } else {
+                    for (int kk = 0; kk < DP / 16; ++kk) {
+                        uint32_t kb[4];
+                        ldmatrix4(kb, kt + kv_chunk<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                                        kk * 2 + ((lane >> 3) & 1)));
+                        if constexpr (kHeld) {
+                            mma16816<T>(s[0][0], qf[kk], kb[0], kb[1]);
+                            mma16816<T>(s[0][1], qf[kk], kb[2], kb[3]);
+                        } else {
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            uint32_t a[4];
-                            ldmatrix4(a, q_at + q_chunk<MR>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)));
-                            mma16816<T>(s[mt][0], a, kb[0], kb[1]);
-                            mma16816<T>(s[mt][1], a, kb[2], kb[3]);
-                        }
-                    }
-                }
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt) {
-                    float mx[2] = {m[mt][0], m[mt][1]};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            float v = s[mt][k][e] * p.scale_log2;
-                            if (mask) {
-                                const int t = tt + k * 8 + (lane & 3) * 2 + (e & 1);
-                                bool seen = t < lim[mt][e >> 1];
-                                if (bad) seen = seen && !((bad >> ((t & (kStep - 1)) / sp.box)) & 1);
-                                if (!seen) v = kNegInf;
-                            }
-                            s[mt][k][e] = v;
-                            mx[e >> 1] = fmaxf(mx[e >> 1], v);
-                        }
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-                        mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-                    }
-                    if (__any_sync(0xffffffffu, mx[0] > m[mt][0] || mx[1] > m[mt][1])) {
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float f = mx[e] == kNegInf ? 1.f : exp2_fast(m[mt][e] - mx[e]);
-                            m[mt][e] = mx[e];
-                            l[mt][e] *= f;
-#pragma unroll
-                            for (int k = 0; k < DP / 8; ++k) {
-                                o[mt][k][2 * e] *= f;
-                                o[mt][k][2 * e + 1] *= f;
+                            for (int mt = 0; mt < MT; ++mt) {
+                                uint32_t a[4];
+                                ldmatrix4(a, q_at + q_chunk<MR>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)));
+                                mma16816<T>(s[mt][0], a, kb[0], kb[1]);
+                                mma16816<T>(s[mt][1], a, kb[2], kb[3]);
                             }
                         }
                     }
-                    const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
-#pragma unroll
-                    for (int k = 0; k < 2; ++k)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float w = exp2_fast(s[mt][k][e] - base[e >> 1]);
-                            s[mt][k][e] = w;
-                            l[mt][e >> 1] += w;
-                        }
-                }
-                // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
-                // rounding error goes in as a second product: the copies, not the products, bound this.
-                uint32_t hi[MT][4], lo[MT][4];
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float a = s[mt][e >> 1][2 * (e & 1)], b = s[mt][e >> 1][2 * (e & 1) + 1];
-                        hi[mt][e] = pack2<T>(a, b);
-                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                            const float2 r = unpack2<T>(hi[mt][e]);
-                            lo[mt][e] = pack2<T>(a - r.x, b - r.y);
-                        }
-                    }
-#pragma unroll
-                for (int k = 0; k < DP / 16; ++k) {
-                    uint32_t vb[4];
-                    ldmatrix4_t(vb, vt + kv_chunk<DP>(warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3),
-                                                      k * 2 + (lane >> 4)));
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        mma16816<T>(o[mt][2 * k], hi[mt], vb[0], vb[1]);
-                        mma16816<T>(o[mt][2 * k + 1], hi[mt], vb[2], vb[3]);
-                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                            mma16816<T>(o[mt][2 * k], lo[mt], vb[0], vb[1]);
-                            mma16816<T>(o[mt][2 * k + 1], lo[mt], vb[2], vb[3]);
+                        float mx[2] = {m[mt][0], m[mt][1]};
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                float v = s[mt][k][e] * p.scale_log2;
+                                if (mask) {
+                                    const int t = tt + k * 8 + (lane & 3) * 2 + (e & 1);
+                                    bool seen = t < lim[mt][e >> 1];
+                                    if (bad) seen = seen && !((bad >> ((t & (kStep - 1)) / sp.box)) & 1);
+                                    if (!seen) v = kNegInf;
+                                }
+                                s[mt][k][e] = v;
+                                mx[e >> 1] = fmaxf(mx[e >> 1], v);
+                            }
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
+                            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
+                        }
+                        if (__any_sync(0xffffffffu, mx[0] > m[mt][0] || mx[1] > m[mt][1])) {
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const float f = mx[e] == kNegInf ? 1.f : exp2_fast(m[mt][e] - mx[e]);
+                                m[mt][e] = mx[e];
+                                l[mt][e] *= f;
+#pragma unroll
+                                for (int k = 0; k < DP / 8; ++k) {
+                                    o[mt][k][2 * e] *= f;
+                                    o[mt][k][2 * e + 1] *= f;
+                                }
+                            }
+                        }
+                        const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float w = exp2_fast(s[mt][k][e] - base[e >> 1]);
+                                s[mt][k][e] = w;
+                                l[mt][e >> 1] += w;
+                            }
+                    }
+                    // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
+                    // rounding error goes in as a second product: the copies, not the products, bound this.
+                    uint32_t hi[MT][4], lo[MT][4];
+#pragma unroll
+                    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float a = s[mt][e >> 1][2 * (e & 1)], b = s[mt][e >> 1][2 * (e & 1) + 1];
+                            hi[mt][e] = pack2<T>(a, b);
+                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                                const float2 r = unpack2<T>(hi[mt][e]);
+                                lo[mt][e] = pack2<T>(a - r.x, b - r.y);
+                            }
+                        }
+#pragma unroll
+                    for (int k = 0; k < DP / 16; ++k) {
+                        uint32_t vb[4];
+                        ldmatrix4_t(vb, vt + kv_chunk<DP>(warp * 16 + (lane & 7) + (((lane >> 3) & 1) << 3),
+                                                          k * 2 + (lane >> 4)));
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            mma16816<T>(o[mt][2 * k], hi[mt], vb[0], vb[1]);
+                            mma16816<T>(o[mt][2 * k + 1], hi[mt], vb[2], vb[3]);
+                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+                                mma16816<T>(o[mt][2 * k], lo[mt], vb[0], vb[1]);
+                                mma16816<T>(o[mt][2 * k + 1], lo[mt], vb[2], vb[3]);
+                            }
                         }
                     }
-                }
                 }
             }
             __syncwarp();
@@ -673,6 +685,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             meet();
         }
         }
+        const bool odd = *reinterpret_cast<volatile int*>(&s_any_odd) != 0;
         for (int r = threadIdx.x; r < n_rows; r += 32 * kSWarps) {
             float top = s_m[0][r], sum = 0.f;
 #pragma unroll
@@ -683,10 +696,16 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             const int jq = static_cast<int>(fdiv(r0 + r, p.div_G));
             const int64_t row = static_cast<int64_t>(x.tok0 + jq) * p.Hq + x.h * p.G + r0 + r - jq * p.G;
             p.part_ml[part * all_rows + row] = make_float2(top, sum);
+            if (odd) add_odd(p.part_o + (part * all_rows + row) * p.D, p.D, s_odd, DP, min(x.len, see + jq + 1));
             if (last)  // parts that this row tile does not have
                 for (int k = part + 1; k < parts_end; ++k) p.part_ml[k * all_rows + row] = make_float2(kNegInf, 0.f);
         }
         meet();
+        if (odd) {
+            for (int i = threadIdx.x; i < 2 * DP; i += 32 * kSWarps) s_odd[i] = kNoToken;
+            if (threadIdx.x == 0) s_any_odd = 0;
+            meet();
+        }
         g += n;
         next_tile(x);
     }

@@ -116,6 +116,26 @@ __device__ __forceinline__ void locate(const AttnParams& p, int u, int& b, int& 
     rt = in - h * own;
 }
 
+// What take_out_odd kept, added to a warp's rows in tensor memory.
+template <int DP>
+__device__ __noinline__ void add_odd_tmem(uint32_t o_at, const int* first, int limit) {
+#pragma unroll 1
+    for (int c = 0; c < DP; c += 16) {
+        uint32_t o[16];
+        tmem_ld16(o_at + c, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            float v = __uint_as_float(o[e]);
+            if (first[c + e] < limit) v += -kNegInf;
+            if (first[DP + c + e] < limit) v += kNegInf;
+            o[e] = __float_as_uint(v);
+        }
+        tmem_st16(o_at + c, o);
+    }
+    tmem_wait_st();
+}
+
 template <typename T, int DP>
 __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_constant__ TileParams tp) {
     using Shape = TileShape<DP>;
@@ -128,6 +148,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     __shared__ int s_gave_up;
     __shared__ int s_any_bad, s_copy;
     __shared__ unsigned char s_ok[4][kTokTile];
+    __shared__ int s_odd[2 * DP], s_any_odd;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -173,6 +194,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     // Token tiles: the prefix's, then the own cache's that the last row sees.
     const int see = len - n_tok;
     const int vis = max(0, min(len, see + static_cast<int>(fdiv(r0 + n_rows - 1, p.div_G)) + 1));
+    const int whole = min(len, see + static_cast<int>(fdiv(r0, p.div_G)) + 1);  // tokens all rows see
     const int tiles_p = (p.P + kTokTile - 1) / kTokTile;
     const int tiles_all = tiles_p + (vis + kTokTile - 1) / kTokTile;
     const int per = (tiles_all + splits - 1) / splits;
@@ -240,8 +262,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         }
         s_gave_up = 0;
         s_any_bad = 0;
+        s_any_odd = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
+    if (threadIdx.x < 2 * DP) s_odd[threadIdx.x] = kNoToken;
     // The first tiles of the prefix are on their way before anything else.
     const int n_loads = 2 * n_tiles;  // K0 V0 K1 V1 ...
     const int early = tp.tma_p ? min(min(n_loads, NST), 2 * max(0, tiles_p - first)) : 0;
@@ -304,7 +328,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             const bool pre = tile < tiles_p;
             const int t0 = pre ? tile * kTokTile : (tile - tiles_p) * kTokTile;
             const uint32_t dst = s_ring + s * TILE;
-            if (pre ? tp.tma_p : tp.tma_c && (!is_v || t0 + kTokTile <= len)) {
+            if (pre ? tp.tma_p : tp.tma_c && (!is_v || t0 + kTokTile <= whole)) {
                 if (lw == 0) {
                     if (i >= NST) alive = bar_wait_warp(empty(s), ((i / NST) - 1) & 1, gave_up);
                     if (!alive) continue;
@@ -394,6 +418,15 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             }
             cp_async_commit();
             cp_async_wait<0>();
+            if (is_v && !pre && whole < vis && t0 + kTokTile > whole) {
+                // each lane what it copied itself
+                for (int g = lw; g < 32; g += kLoadWarps)
+                    for (int pn = 0; pn < CPR / 8; ++pn) {
+                        const int r = g * 4 + sub, c = pn * 8 + c8;
+                        const uint32_t at = dst + tile_chunk(r, c);
+                        take_out_odd<T>(at, t0 + r, s_odd + c * 8, DP, &s_any_odd);
+                    }
+            }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             asm volatile("bar.sync 1, %0;" ::"n"(32 * kLoadWarps) : "memory");
             if (lw == 0 && lane == 0) bar_arrive(full(s));
@@ -607,6 +640,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 const bool mine = r < n_rows;
                 const int64_t at = static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + row - j * p.G;
                 const float inv = l == 0.f ? 0.f : 1.f / l;
+                if (*reinterpret_cast<volatile int*>(&s_any_odd)) add_odd_tmem<DP>(o_at, s_odd, own_limit);
                 if (mine) {
                     if (!direct)
                         p.part_ml[part_at(r)] = make_float2(m, l);
@@ -643,19 +677,14 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     }
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(
-                                         stage + lane * 128 + ((k ^ (lane & 7)) << 4)),
-                                     "r"(o[4 * k]), "r"(o[4 * k + 1]), "r"(o[4 * k + 2]), "r"(o[4 * k + 3])
-                                     : "memory");
+                        st_shared_v4(stage + lane * 128 + ((k ^ (lane & 7)) << 4),
+                                     make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]));
                     __syncwarp();
                     const int col = c + c8 * (per / 8);
 #pragma unroll
                     for (int it = 0; it < 8; ++it) {
                         const int rr = it * 4 + sub;
-                        uint4 v;
-                        asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];"
-                                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                     : "r"(stage + rr * 128 + ((c8 ^ (rr & 7)) << 4)));
+                        const uint4 v = ld_shared_v4(stage + rr * 128 + ((c8 ^ (rr & 7)) << 4));
                         if (dst[it] != nullptr && col < p.D) st_v4(dst[it] + c * (direct ? 2 : 4), v);
                     }
                     __syncwarp();

@@ -17,7 +17,9 @@
 // What bounds it: HBM (two 16-bit values read and written for 3 multiplications).  A block
 // loads the slices of its rows first, then tabulates its tokens' cosines and sines in shared
 // memory while they are in flight (64 per token at R = 128, used by every head of q and k), then
-// turns and stores.
+// turns and stores.  32 + 8 heads of 128 for 8,192 tokens: 36.3 us, a plain copy of the same bytes
+// 32.7.  Blocks of 128 threads with two items each in flight (one or four: 39.2 and 39.6 us for
+// 35.5; 512 threads: 51.9).
 #include <math.h>
 
 #include "sc_common.cuh"

@@ -10,7 +10,11 @@
 // the exponentials bound it: 16 a clock and SM against 4,096 multiplications).
 //
 // Roles: warps 0-3 and 4-7 the weights of tile 0 and 1, warp 8 the copies (TMA), warp 9 the
-// products, warps 10 and 11 the scores of tokens that are not in use.  Each tile has two score buffers in tensor memory.
+// products, warps 10 and 11 the scores of tokens that are not in use.  Each tile has two score
+// buffers in tensor memory.
+//
+// Measured, 32 query heads on 8 KV heads of 128: one query of each of 16 sequences of up to 8,192
+// tokens 29 us (22 at a copy's rate); 64 queries on 32,768 tokens 37, the exponentials alone 15.
 #include <limits.h>
 #include <math.h>
 
@@ -264,7 +268,7 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
     } else if (warp == 9) {
         // ---- products ----
         // The warp stays converged, so addresses and descriptors are uniform; one lane issues.
-        // (One lane in a branch of its own: 40.4 instead of WW us for 16 x up to 8,192 tokens.)
+        // (One lane in a branch of its own: 40.4 instead of 36.7 us for 16 x up to 8,192 tokens.)
         constexpr uint32_t fmt = std::is_same<T, __half>::value ? 0u : 1u;
         constexpr uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) |
                                    ((static_cast<uint32_t>(NR) >> 3) << 17) | ((128u >> 4) << 24);

@@ -205,6 +205,52 @@ def test_not_a_number_reaches_its_rows_alone(scb):
     assert torch.isfinite(out[:, 2:]).all() and bits_equal(out[:, 2:], want[0][:, 2:])
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("shape", [
+    # q_lens, lens, hq, hk, d, prefix, cap, page
+    ([2, 3], [40, 3], 8, 4, 128, 70, 40, 0),      # 8 rows a tile
+    ([4, 2], [33, 2], 8, 2, 64, 70, 40, 8),       # 16
+    ([9, 5], [64, 70], 8, 2, 128, None, 70, 0),   # 32
+    ([6], [17], 8, 1, 256, 30, 20, 0),
+    ([6, 4], [70, 3], 8, 2, 64, 30, 70, 1),       # pages of one token
+    ([150, 70], [150, 300], 4, 2, 128, 130, 300, 0),  # 256-row tiles
+    ([130], [129], 4, 2, 64, 20, 140, 24),
+])
+@pytest.mark.parametrize("expanded", [False, True])
+def test_values_that_are_not_finite_stay_with_the_rows_that_see_them(scb, ref, dtype, shape, expanded):
+    """NaN and infinities among the values of a sequence's last tokens: earlier rows do not see them."""
+    c = Case(31, dtype, *shape)
+    if expanded:  # one KV head for all, by a stride of zero
+        c.kc, c.vc = c.kc[..., :1, :].expand(*c.kc.shape[:-2], shape[3], -1), c.vc[..., :1, :]
+    page = shape[7]
+    at = lambda b, t: (int(c.table[b, t // page]), t % page) if page else (b, t)
+    for b, (n, length) in enumerate(zip(c.q_lens, c.lens)):
+        for t, column, v in ((length - 1, 3, math.nan), (length - 1, 5, math.inf), (length - n // 2, 5, -math.inf),
+                             (length - n // 2, 17, math.inf), (length - n + 1, 20, -math.inf)):
+            if 0 <= t < length:
+                i, j = at(b, t)
+                c.vc[i, j, 0, column] = v
+    if expanded:
+        c.vc = c.vc.expand(c.kc.shape)
+    out, lse = c.run(scb)
+    want, _, _, _ = ref.attention(*[None if x is None else x.cpu() for x in (c.q, c.kp, c.vp, c.kc, c.vc)], c.lens,
+                                  c.q_lens, page_table=None if c.table is None else c.table.cpu())
+    got = out.cpu().double()
+    assert not torch.isfinite(want).all() and torch.isfinite(want).any()
+    # bf16 weights go into the product in two pieces, w = hi + lo with |lo| <= 2^-9 w of either sign or zero:
+    # hi inf + lo inf is inf - inf or inf + 0 inf, which is NaN, where lo <= 0.
+    assert (torch.isfinite(got) == torch.isfinite(want)).all()
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    if dtype == torch.bfloat16:
+        same |= torch.isnan(got)
+    assert (same | torch.isfinite(want)).all()
+    # the others as if zeros stood there
+    c.vc = torch.where(torch.isfinite(c.vc), c.vc, torch.zeros_like(c.vc))
+    clean, clean_lse = c.run(scb)
+    c.check(ref, torch.where(torch.isfinite(want).to(DEV), out, clean), lse)
+    c.check(ref, clean, clean_lse)
+
+
 def test_scores_of_minus_infinity_are_hidden(scb, ref):
     """A key of -inf along a positive query hides its token, as a mask of the lowest value does."""
     c = Case(18, torch.float16, [1, 1], [5, 5], 2, 1, 64, 30, 5)
