@@ -372,17 +372,9 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                     tc_fence_after();
                     const bool masked = last >= s_all_seen[qs];
                     const uint32_t at = tmem + (t * 2 + buf) * NR + lanes;
-                    constexpr int W = NR < 32 ? NR : 32;
-#pragma unroll 1
-                    for (int c0 = 0; c0 < NR; c0 += W) {
-                        uint32_t s[W];
-                        if constexpr (W == 32)
-                            tmem_ld32(at + c0, s);
-                        else
-                            tmem_ld16(at + c0, s);
-                        tmem_wait_ld();
+                    auto weigh = [&](const uint32_t* s, int c0, int n) {
 #pragma unroll
-                        for (int e = 0; e < W; e += 4) {
+                        for (int e = 0; e < n; e += 4) {
                             const float4 nl = *reinterpret_cast<const float4*>(&s_neg_lse[qs][c0 + e]);
                             float2 v0 = make_float2(__uint_as_float(s[e]), __uint_as_float(s[e + 1]));
                             float2 v1 = make_float2(__uint_as_float(s[e + 2]), __uint_as_float(s[e + 3]));
@@ -397,6 +389,21 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                             }
                             acc = __fadd2_rn(acc, v0);
                             acc2 = __fadd2_rn(acc2, v1);
+                        }
+                    };
+                    if constexpr (NR == 16) {
+                        uint32_t s[16];
+                        tmem_ld16(at, s);
+                        tmem_wait_ld();
+                        weigh(s, 0, 16);
+                    } else {
+#pragma unroll 1
+                        for (int c0 = 0; c0 < NR; c0 += 64) {
+                            uint32_t s[64];
+                            tmem_ld32(at + c0, s);
+                            tmem_ld32(at + c0 + 32, s + 32);
+                            tmem_wait_ld();
+                            weigh(s, c0, 64);
                         }
                     }
                     tc_fence_before();
