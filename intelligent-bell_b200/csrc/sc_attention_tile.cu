@@ -652,18 +652,13 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 // took 5 us of a block's time.
                 const uint32_t stage = s_q + q * TILE + (warp & 3) * (TILE / 4);
                 const int per = direct ? 64 : 32;  // columns a pass
-                char* dst[8];  // a lane's part of eight rows
-#pragma unroll
-                for (int it = 0; it < 8; ++it) {
-                    const int row2 = r0 + q * kRowTile + (warp & 3) * 32 + it * 4 + sub;
-                    dst[it] = nullptr;
-                    if (row2 < r0 + n_rows) {
-                        const int j2 = static_cast<int>(fdiv(row2, p.div_G)), head = h * p.G + row2 - j2 * p.G;
-                        dst[it] = direct ? reinterpret_cast<char*>(static_cast<T*>(p.out) + (tok0 + j2) * p.o_t + head * p.o_h)
-                                         : reinterpret_cast<char*>(p.part_o + part_at(row2 - r0) * p.D);
-                        dst[it] += c8 * 16;
-                    }
-                }
+                // Each lane knows where its row goes; a store asks the lane whose row it is.  (Eight rows'
+                // places worked out by every lane: 3 us more, for fetching the instructions of it.)
+                char* to = nullptr;
+                if (mine)
+                    to = direct ? reinterpret_cast<char*>(static_cast<T*>(p.out) + (tok0 + j) * p.o_t +
+                                                          (h * p.G + row - j * p.G) * p.o_h)
+                                : reinterpret_cast<char*>(p.part_o + part_at(r) * p.D);
 #pragma unroll 1
                 for (int c = 0; c < DP; c += per) {
                     uint32_t o[64];
@@ -685,7 +680,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     for (int it = 0; it < 8; ++it) {
                         const int rr = it * 4 + sub;
                         const uint4 v = ld_shared_v4(stage + rr * 128 + ((c8 ^ (rr & 7)) << 4));
-                        if (dst[it] != nullptr && col < p.D) st_v4(dst[it] + c * (direct ? 2 : 4), v);
+                        char* dst = reinterpret_cast<char*>(
+                            __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(to), rr));
+                        if (dst != nullptr && col < p.D) st_v4(dst + c * (direct ? 2 : 4) + c8 * 16, v);
                     }
                     __syncwarp();
                 }
