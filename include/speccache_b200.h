@@ -375,6 +375,8 @@ SC_API int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_heads, i
  * Attention of a batch that shares a prefix: each sequence's queries see the whole prefix and,
  * of the sequence's own cache, the tokens t <= len - n + j (query j of n), so the newest query
  * sees all of it.  A row that sees nothing gives zeros and a log-sum-exp of -infinity.
+ * What a row does not see never reaches it, NaN and infinities included; an infinite value that it
+ * sees gives an infinity or NaN.
  *
  *  q, out       [n_tokens, q_heads, head_dim], the sequences' tokens one after another; strides
  *               {token, head}; unit stride along head_dim in every tensor
@@ -386,7 +388,7 @@ SC_API int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_heads, i
  *  cache_lens   device int32 [batch], tokens in use (the queries' own among them); NULL: all
  *  page_table   device int32, row stride page_table_stride
  *  cu_q_lens    device int32 [batch + 1], each sequence's first token; NULL: max_q_len each.
- *               Rows behind the last sequence are left as they were.
+ *               Rows before the first sequence and behind the last are left as they were.
  *  lse          float32 [n_tokens, q_heads], natural logarithm, contiguous; may be NULL
  *  workspace    of sc_shared_prefix_attention_workspace bytes, 16-byte aligned, for this call
  *               alone until its work has completed

@@ -423,6 +423,7 @@ __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ A
     const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kWarps + warp : blockIdx.x;
     const int64_t all_rows = static_cast<int64_t>(p.N) * p.Hq;
     if (row >= static_cast<int64_t>(used_tokens(p)) * p.Hq) return;
+    if (p.cu_q != nullptr && row < static_cast<int64_t>(p.cu_q[0]) * p.Hq) return;  // of no sequence
     const int parts = p.n_pp + p.n_cp;
     const int each = (parts + W - 1) / W, i0 = W == 1 ? 0 : warp * each, i1 = min(parts, i0 + each);
     float m = kNegInf;

@@ -320,7 +320,7 @@ extern "C" int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_head
     const int32_t kh = k ? k_heads : 0;
     const int64_t rows = size_product(batch, n_tokens, static_cast<int64_t>(q_heads) + kh);
     if (size_product(rows, (head_dim + 1) / 2) >= (int64_t(1) << 31) * kRThreads ||
-        rows >= (int64_t(1) << 31))
+        rows >= (int64_t(1) << 31) || size_product(static_cast<int64_t>(q_heads) + kh, head_dim) >= (int64_t(1) << 24))
         return set_error(SC_ERR_INVALID_ARGUMENT, "%lld rows in one call; split it", (long long)rows);
     if (rows == 0 || head_dim == 0) return ok();
     if ((q_heads && (!q || !q_out || !q_strides || !qo_strides)) ||

@@ -124,7 +124,12 @@ def _lengths(name: str, lens, batch: int, most: int):
         raise ValueError(f"{name} must be [{batch}], got {tuple(lens.shape)}")
     if not lens.is_cuda and batch and (int(lens.min()) < 0 or int(lens.max()) > most):
         raise ValueError(f"{name} must lie in [0, {most}]")
-    return lens.to(torch.int32).contiguous()
+    return _int32(lens).contiguous()
+
+
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """Lengths or page ids as int32; what int32 cannot hold stays out of range."""
+    return t.clamp(-1, 2 ** 31 - 1).to(torch.int32) if t.dtype == torch.int64 else t.to(torch.int32)
 
 
 def _on_device(what: str, tensors: list, device: torch.device) -> list:
@@ -217,8 +222,8 @@ def shared_prefix_attention(
         cache_lens: ``[B]`` tokens in use, the queries' own among them (default: all).  Query j of
             a sequence's n sees its cache's tokens ``t <= len - n + j``.
         q_lens: ``[B]`` host query counts; or ``cu_q_lens`` int32 ``[B + 1]`` starts on the device
-            with ``max_q_len``.  Default: N / B each.  Rows behind the last sequence are left
-            as they were (in outputs allocated here: undefined).
+            with ``max_q_len``.  Default: N / B each.  Rows before the first sequence and behind the
+            last are left as they were (in outputs allocated here: undefined).
         page_table: int32 ``[B, max_pages]``.  A bad id's tokens count as masked, a bad device
             length as 0, both reported by :func:`paged_status`.
         scale: of the scores, default ``D ** -0.5``.
@@ -226,7 +231,8 @@ def shared_prefix_attention(
 
     Any strides with a contiguous, 16-byte aligned head; ``D`` a multiple of 8 up to 256.  Scores,
     sums and accumulators are float32.  Returns ``(out, lse)`` with float32 ``lse [N, Hq]`` (natural
-    logarithm); a row that sees nothing is zero with ``lse = -inf``.
+    logarithm); a row that sees nothing is zero with ``lse = -inf``.  What a row does not see never
+    reaches it, NaN and infinities included.
     """
     require_cuda(q)
     require_no_grad("shared_prefix_attention", q, k_prefix, v_prefix, k_cache, v_cache, out)
@@ -246,7 +252,7 @@ def shared_prefix_attention(
             if table.ndim != 2:
                 raise ValueError(f"page_table must be [B, max_pages], got {tuple(table.shape)}")
             if table.dtype != torch.int32:
-                table = table.to(torch.int32)
+                table = _int32(table)
             if table.stride(1) != 1 and table.shape[1] > 1:
                 table = table.contiguous()
             batch, page, n_pages = table.shape[0], lay.cap, lay.rows

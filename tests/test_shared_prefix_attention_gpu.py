@@ -183,6 +183,27 @@ def test_nothing_is_read_behind_the_lengths(scb, ref, page, q_len):
     c.check(ref, *got)
 
 
+def test_rows_before_the_first_sequence_and_wide_device_integers(scb, ref):
+    for n, d in ((2, 128), (40, 64)):  # streamed, and 256-row tiles
+        c = Case(29, torch.float16, [n, n], [n + 20, n + 3], 8, 2, d, 70, n + 20, 8)
+        q = torch.cat((torch.full_like(c.q[:3], float("nan")), c.q, c.q[:2]))
+        out = torch.full_like(q, 5.0)
+        cu = torch.tensor([3, 3 + n, 3 + 2 * n], dtype=torch.int32, device=DEV)
+        _, lse = scb.shared_prefix_attention(q, c.kp, c.vp, c.kc, c.vc, c.lens_t().long(), page_table=c.table.long(),
+                                             cu_q_lens=cu, max_q_len=n, out=out)
+        assert (out[:3] == 5).all() and (out[-2:] == 5).all()
+        c.check(ref, out[3:-2], lse[3:-2])
+    # 64-bit lengths and page ids that 32 bits cannot hold are out of range, not some others
+    scb.paged_status(DEV)
+    lens, table = torch.tensor([2 ** 32 + 5, 43], device=DEV), c.table.long()
+    table[1, 0] += 2 ** 32
+    out, lse = scb.shared_prefix_attention(c.q, c.kp, c.vp, c.kc, c.vc, lens, page_table=table, q_lens=c.q_lens)
+    assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_SEQ_LEN | scb._lib.SC_STATUS_BAD_PAGE_ID
+    c.lens, c.table = [0, 43], c.table.clone()
+    c.table[1, 0] = -1
+    c.check(ref, out, lse)
+
+
 def test_scores_that_grow_along_the_tokens(scb, ref):
     """The running maximum is passed again and again, by little and by much."""
     for n in (1, 50):
