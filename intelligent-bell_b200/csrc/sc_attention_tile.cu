@@ -710,48 +710,62 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     wait_for_previous();  // nothing is read from it, but this kernel's end stands for its end, too
 }
 
-// Rows of the last round's units: their parts joined, a warp a row.
-constexpr int kTailRows = 32;  // rows a block
+// Rows of the last round's units: their parts joined, a warp a row, eight parts' loads in flight.
+// (A part at a time waited for memory: two sequences of 40 tokens x 32 heads behind 16,384 76 us, this
+// way 53; one of 24 tokens behind 8,192 59 and 29.)
+constexpr int kTailRows = 8;     // rows a block at a time
+constexpr int kTailBlocks = 16;  // an SM: one turn for 74 units, the most that are split
+constexpr int kTailLoads = 8;
 template <typename T>
 __global__ void __launch_bounds__(128) join_tail(const __grid_constant__ TileParams tp) {
-    wait_for_previous();
     const AttnParams& p = tp.a;
     const Round rd = rounds(tp);
-    const int unit = blockIdx.x / (2 * kRowTile / kTailRows);
-    if (unit >= rd.rem || rd.parts == 1) return;
-    int b, h, rt, tok0, n_tok;
-    locate(p, rd.full + unit, b, h, rt);
-    sequence_tokens(p, b, tok0, n_tok);
+    constexpr int kGroups = 2 * kRowTile / kTailRows;  // of a unit's rows
     const int lane = threadIdx.x & 31;
-    const int first = (blockIdx.x % (2 * kRowTile / kTailRows)) * kTailRows;
-    for (int r = first + (threadIdx.x >> 5); r < first + kTailRows; r += 4) {
-        const int row = rt * 2 * kRowTile + r;
-        if (row >= n_tok * p.G) break;
-        const int64_t at = static_cast<int64_t>(unit) * rd.parts * (2 * kRowTile) + r;
-        // a lane a part
-        const float2 ml = lane < rd.parts ? p.part_ml[at + lane * (2 * kRowTile)] : make_float2(kNegInf, 0.f);
-        float m = ml.x;
+    wait_for_previous();
+    if (rd.parts == 1) return;
+    for (int g = blockIdx.x; g < rd.rem * kGroups; g += gridDim.x) {
+        const int unit = g / kGroups, first = (g - unit * kGroups) * kTailRows;
+        int b, h, rt, tok0, n_tok;
+        locate(p, rd.full + unit, b, h, rt);
+        sequence_tokens(p, b, tok0, n_tok);
+        for (int r = first + (threadIdx.x >> 5); r < first + kTailRows; r += 4) {
+            const int row = rt * 2 * kRowTile + r;
+            if (row >= n_tok * p.G) break;
+            const int64_t at = static_cast<int64_t>(unit) * rd.parts * (2 * kRowTile) + r;
+            // a lane a part
+            const float2 ml = lane < rd.parts ? p.part_ml[at + lane * (2 * kRowTile)] : make_float2(kNegInf, 0.f);
+            float m = ml.x;
 #pragma unroll
-        for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-        const float w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
-        float sum = ml.x == kNegInf && ml.y == 0.f ? 0.f : w * ml.y;
+            for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+            const float w = ml.x == kNegInf ? 0.f : exp2_fast(ml.x - m);
+            float sum = ml.x == kNegInf && ml.y == 0.f ? 0.f : w * ml.y;
 #pragma unroll
-        for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int i = 0; i < rd.parts; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (wi == 0.f || lane * 4 >= p.D) continue;
-            const float4 v = *reinterpret_cast<const float4*>(p.part_o + (at + i * (2 * kRowTile)) * p.D + lane * 4);
-            a.x += wi * v.x, a.y += wi * v.y, a.z += wi * v.z, a.w += wi * v.w;
+            for (int x = 16; x; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < rd.parts; i += kTailLoads) {
+                float wi[kTailLoads];
+                float4 v[kTailLoads];
+#pragma unroll
+                for (int k = 0; k < kTailLoads; ++k) {
+                    wi[k] = __shfl_sync(0xffffffffu, w, i + k);  // 0 behind the last part
+                    v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (!(wi[k] == 0.f) && lane * 4 < p.D)
+                        v[k] = *reinterpret_cast<const float4*>(p.part_o + (at + (i + k) * (2 * kRowTile)) * p.D + lane * 4);
+                }
+#pragma unroll
+                for (int k = 0; k < kTailLoads; ++k)
+                    a.x += wi[k] * v[k].x, a.y += wi[k] * v[k].y, a.z += wi[k] * v[k].z, a.w += wi[k] * v[k].w;
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int j = static_cast<int>(fdiv(row, p.div_G)), head = h * p.G + row - j * p.G;
+            if (lane * 4 < p.D)
+                st_v2(static_cast<T*>(p.out) + (tok0 + j) * p.o_t + head * p.o_h + lane * 4,
+                      make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)));
+            if (p.lse && lane == 0)
+                p.lse[static_cast<int64_t>(tok0 + j) * p.Hq + head] =
+                    sum == 0.f ? kNegInf : (m + log2f(sum)) * 0.6931471805599453f;
         }
-        const float inv = sum == 0.f ? 0.f : 1.f / sum;
-        const int j = static_cast<int>(fdiv(row, p.div_G)), head = h * p.G + row - j * p.G;
-        if (lane * 4 < p.D)
-            st_v2(static_cast<T*>(p.out) + (tok0 + j) * p.o_t + head * p.o_h + lane * 4,
-                  make_uint2(pack2<T>(a.x * inv, a.y * inv), pack2<T>(a.z * inv, a.w * inv)));
-        if (p.lse && lane == 0)
-            p.lse[static_cast<int64_t>(tok0 + j) * p.Hq + head] =
-                sum == 0.f ? kNegInf : (m + log2f(sum)) * 0.6931471805599453f;
     }
 }
 
@@ -763,8 +777,7 @@ cudaError_t launch_tiles_dp(const TileParams& p, unsigned units, bool chained, c
     if (e != cudaSuccess || load_only) return e;
     e = launch_chained(kernel, dim3(units), kTThreads, TileShape<DP>::kSmem, s, chained, p);
     if (e != cudaSuccess || !p.per_seq || p.splits == 1) return e;
-    return launch_chained(join_tail<T>, dim3(static_cast<unsigned>((p.sms - 1) * (2 * kRowTile / kTailRows))), 128, 0, s,
-                          true, p);
+    return launch_chained(join_tail<T>, dim3(static_cast<unsigned>(p.sms * kTailBlocks)), 128, 0, s, true, p);
 }
 
 }  // namespace
