@@ -9,8 +9,8 @@
 // first keys.  Warps 0-3 take 16 of a step's tokens each, with a softmax state of their own
 // (16-bit-input matrix products, fp32 sums), joined when the part ends.
 // (Blocks of one part, cp.async by every warp with its address arithmetic: 750 instructions for
-// 16 tokens, 4.7 TB/s at best and 33 us for 64 ragged caches of up to 1,024
-// tokens; this way 19.)
+// 16 tokens, 4.7 TB/s at best and 33 us for 64 ragged caches of up to 512 tokens, 73 MB; this way 18,
+// of which a block's set-up and first data take 5 and a part's end 1.2.)
 #include <math.h>
 
 #include "sc_tensor.cuh"

@@ -582,8 +582,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         l += (sum.x + sum.y) + (sum2.x + sum2.y);
                     } else {
                         // A tile's end, a mask, or a scale that turns the order: the few of these take short
-                        // loops, which leave the others' instructions together (a kernel of 131,072
-                        // tokens and 512 rows a head: 459 -> 452 us).
+                        // loops, which leave the others' instructions together (eight prompts of up to
+                        // 512 tokens behind 8,192: 459 us, this way 452).
                         const bool turned = p.scale_log2 <= 0.f;
                         const float mul = turned ? 1.f : p.scale_log2;
                         auto scores = [&](int c, uint32_t (&x)[16]) {  // 16 columns, what is hidden -inf
