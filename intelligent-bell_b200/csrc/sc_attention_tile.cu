@@ -7,7 +7,7 @@
 //   P = 2^(s - m)     one thread a row: no shuffles; written over S as 16 bits,
 //   O += P V          A operand from tensor memory, fp32 accumulators in tensor memory.
 // Two row tiles take turns: while the tensor cores work on one, eight warps turn the other's
-// scores into weights.  The running maximum that scales O is only raised when a score passes it
+// scores into weights.  (With one row tile, two token tiles' scores do.)  The running maximum that scales O is only raised when a score passes it
 // by 2^8, so O is rarely rescaled (weights up to 2^8 and their fp32 sums lose nothing).
 //
 // Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies, warp 11 issues
@@ -147,7 +147,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     __shared__ uint32_t s_tmem;
     __shared__ int s_gave_up;
     __shared__ int s_any_bad, s_copy;
-    __shared__ unsigned char s_ok[4][kTokTile];
+    // Tokens of a tile whose page is there.  A tile's keys may be loaded while the softmax is still at
+    // the tile three (five stages) or six (eight) before it.
+    constexpr int kOks = NST == 5 ? 4 : 8;
+    __shared__ unsigned char s_ok[kOks][kTokTile];
     __shared__ int s_odd[2 * DP], s_any_odd;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -336,10 +339,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         load_prefix(i);
                         continue;
                     }
-                    if (lane == 0) bar_expect(full(s), TILE);
-                    __syncwarp();
                     const CUtensorMap* map = is_v ? &tp.vc : &tp.kc;
                     if (!paged) {
+                        if (lane == 0) bar_expect(full(s), TILE);
+                        __syncwarp();
                         if (lane < CPR / 8) tma_load(dst + lane * 16384, map, full(s), lane * 64, t0, h, b);
                     } else {
                         // One lane a box; a page that is not there lies outside the map: zeros.
@@ -355,7 +358,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             if (!ok) id = static_cast<int>(p.n_pages);
                         }
                         if (!is_v) {
-                            const int local = (i >> 1) & 3;
+                            const int local = (i >> 1) % kOks;
                             for (int e = lane / n_box; e < box; e += 32 / n_box) s_ok[local][bx * box + e] = ok;
                             if (!ok) {
                                 s_any_bad = 1;
@@ -363,6 +366,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             }
                             __syncwarp();
                         }
+                        if (lane == 0) bar_expect(full(s), TILE);
+                        __syncwarp();
                         for (int pn = lane / n_box; pn < CPR / 8; pn += 32 / n_box)
                             tma_load(dst + pn * 16384 + bx * box * 128, map, full(s), pn * 64, in, h, id);
                     }
@@ -400,7 +405,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         in = id >= 0 && id < p.n_pages;
                         if (in) off = id * st_b + (t - pg * p.page) * st_t;
                         if (!is_v && c8 == 0) {
-                            s_ok[(i >> 1) & 3][r] = in;
+                            s_ok[(i >> 1) % kOks][r] = in;
                             if (!in) {
                                 s_any_bad = 1;
                                 if (p.status) atomicOr(p.status, SC_STATUS_BAD_PAGE_ID);
@@ -442,33 +447,60 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         const uint64_t q_desc = desc(s_q, 16, 1024), k_desc = desc(s_ring, 16, 1024),
                        v_desc = desc(s_ring, 16384, 1024);
         const bool leader = elect_one();
-        auto qk = [&](int q, int stage) {
+        auto qk = [&](int q, int stage, int to) {
             const uint64_t qd = q_desc + static_cast<uint32_t>(q * (TILE / 16));
             const uint64_t kd = k_desc + static_cast<uint32_t>(stage * (TILE / 16));
 #pragma unroll
             for (int kk = 0; kk < DP / 16; ++kk) {
                 const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) / 16;
-                mma_ss(tmem + q * 128, qd + off, kd + off, id_qk, kk > 0);
+                mma_ss(tmem + to * 128, qd + off, kd + off, id_qk, kk > 0);
             }
         };
-        auto pv = [&](int q, int stage, bool add) {
+        auto pv = [&](int q, int stage, int from, bool add) {
             const uint64_t vd = v_desc + static_cast<uint32_t>(stage * (TILE / 16));
 #pragma unroll
             for (int kk = 0; kk < kTokTile / 16; ++kk)
-                mma_ts(tmem + kO + q * DP, tmem + q * 128 + kk * 8, vd + kk * (2048 / 16), id_pv,
+                mma_ts(tmem + kO + q * DP, tmem + from * 128 + kk * 8, vd + kk * (2048 / 16), id_pv,
                        add || kk > 0);
         };
         bool alive = bar_wait_all(q_full, 0, gave_up) && bar_wait_all(full(0), 0, gave_up);
         if (alive && leader) {
             for (int q = 0; q < n_q; ++q) {
-                qk(q, 0);
+                qk(q, 0, q);
                 tc_commit(s_full(q));
             }
             tc_commit(empty(0));
         }
         __syncwarp();
+        // One row tile: the next tile's scores go where those of a second row tile would be, while the
+        // softmax works on this one's.
+        for (int i = 0; n_q == 1 && i < n_tiles && alive; ++i) {
+            const int buf = i & 1, v = 2 * i + 1, k = 2 * i + 2;  // places in the order of loads
+            if (i + 1 < n_tiles) {
+                alive = bar_wait_all(full(k % NST), k / NST & 1, gave_up);
+                // the product before this one has read the weights that lie there
+                if (alive && i > 0) alive = bar_wait_all(o_full(0), (i - 1) & 1, gave_up);
+                if (!alive) break;
+                tc_fence_after();
+                if (leader) {
+                    qk(0, k % NST, buf ^ 1);
+                    tc_commit(s_full(buf ^ 1));
+                    tc_commit(empty(k % NST));
+                }
+                __syncwarp();
+            }
+            alive = bar_wait_both(full(v % NST), v / NST & 1, p_full(buf), i >> 1 & 1, gave_up);
+            if (!alive) break;
+            tc_fence_after();
+            if (leader) {
+                pv(0, v % NST, buf, i > 0);
+                tc_commit(o_full(0));
+                tc_commit(empty(v % NST));
+            }
+            __syncwarp();
+        }
         int stage = 1 % NST, phase = 0;  // of the next tile to be read
-        for (int i = 0; i < n_tiles && alive; ++i) {
+        for (int i = 0; n_q == 2 && i < n_tiles && alive; ++i) {
             const bool more = i + 1 < n_tiles;
             const int vs = stage, vp = phase;
             if (++stage == NST) stage = 0, phase ^= 1;
@@ -480,7 +512,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 if (!alive) break;
                 tc_fence_after();
                 if (leader) {
-                    pv(q, vs, i > 0);
+                    pv(q, vs, q, i > 0);
                     tc_commit(o_full(q));
                     if (q == n_q - 1) tc_commit(empty(vs));
                 }
@@ -491,7 +523,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                                    : bar_wait_all(o_full(q), i & 1, gave_up);
                     if (!alive) break;
                     if (leader) {
-                        qk(q, ks);
+                        qk(q, ks, q);
                         tc_commit(s_full(q));
                         if (q == n_q - 1) tc_commit(empty(ks));
                     }
@@ -505,7 +537,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         const int q = warp >> 2;
         const int r = q * kRowTile + (warp & 3) * 32 + lane;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_at = tmem + q * 128 + lanes, o_at = tmem + kO + q * DP + lanes;
+        const uint32_t o_at = tmem + kO + q * DP + lanes;
         const bool any = q * kRowTile + (warp & 3) * 32 < n_rows;  // a row of this warp counts
         if (q < n_q) {
             const int row = min(r0 + r, rows - 1);
@@ -514,7 +546,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             float m = kNegInf, l = 0.f;  // m: the maximum in use
             bool alive = true;
             for (int i = 0; i < n_tiles; ++i) {
-                alive = bar_wait_warp(s_full(q), i & 1, gave_up);
+                const int buf = n_q == 1 ? i & 1 : q;
+                const uint32_t s_at = tmem + buf * 128 + lanes;
+                alive = bar_wait_warp(s_full(buf), (n_q == 1 ? i >> 1 : i) & 1, gave_up);
                 if (!alive) break;
                 tc_fence_after();
                 if (any) {
@@ -594,7 +628,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             for (int e = 0; e < 16; ++e) on |= (c + e < seen ? 1u : 0u) << e;
                             if (bad)
                                 for (int e = 0; e < 16; ++e)
-                                    if (!s_ok[i & 3][c + e]) on &= ~(1u << e);
+                                    if (!s_ok[i % kOks][c + e]) on &= ~(1u << e);
 #pragma unroll
                             for (int e = 0; e < 16; ++e) {
                                 const float v = __uint_as_float(x[e]) * (turned ? p.scale_log2 : 1.f);
@@ -630,7 +664,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 }
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) bar_arrive(p_full(q));
+                if (lane == 0) bar_arrive(p_full(buf));
             }
             if (alive) {
                 alive = bar_wait_warp(o_full(q), (n_tiles - 1) & 1, gave_up);

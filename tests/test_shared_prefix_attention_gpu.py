@@ -316,6 +316,31 @@ def test_bad_pages_and_lengths_are_reported(scb, ref):
     c.check(ref, out, lse)
 
 
+@pytest.mark.parametrize("d,n,page", [(64, 30, 16), (64, 60, 16), (64, 60, 4), (128, 30, 16), (128, 60, 16)])
+def test_bad_pages_among_many_tiles(scb, ref, d, n, page):
+    """Every other tile of a long own cache has a bad page of its own; one and two row tiles."""
+    c = Case(33, torch.bfloat16, [n, n], [2000, 1600], 8, 2, d, 300, 2048, page)
+    for b in range(2):
+        for tile in range(0, 16, 2):
+            c.table[b, (tile * 128 + 8 * (tile + b)) // page] = -1 if tile & 2 else 10 ** 8
+    scb.paged_status(DEV)
+    for _ in range(5):
+        out, lse = c.run(scb)
+    assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_PAGE_ID
+    c.check(ref, out, lse)
+
+
+@pytest.mark.parametrize("prefix,n,d", [(1, 30, 128), (128, 24, 64), (129, 32, 128), (1500, 31, 64), (5000, 25, 128)])
+def test_one_row_tile(scb, ref, prefix, n, d):
+    """Up to 128 rows of a sequence: token tiles take turns."""
+    for lens in ([n, n + 3, 500], [700, n, 129]):
+        c = Case(34, torch.float16, [n, n, n - 2], lens, 8, 2, d, prefix, 700)
+        c.kp.mul_(torch.linspace(0.2, 4, prefix, device=DEV).to(torch.float16)[:, None, None])
+        c.check(ref, *c.run(scb))
+    c = Case(35, torch.bfloat16, [1] * 30, [5] * 30, 8, 2, d, prefix, 8)  # a decode of up to 128 rows
+    c.check(ref, *c.run(scb))
+
+
 def test_strided_queries_and_outputs(scb, ref):
     c = Case(21, torch.float16, [2, 5], [30, 6], 6, 2, 64, 44, 30)
     qkv = torch.zeros((7, 10, 64), dtype=torch.float16, device=DEV)
