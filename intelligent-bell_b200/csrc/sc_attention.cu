@@ -9,8 +9,8 @@
 // prefix token is loaded once for 16 or 32 rows instead of once per sequence.
 //
 // Three kernels write parts, by the rows that one KV head has in common (plan_split):
-//   attend_tiles (sc_attention_tile.cu)    64 rows and more over the prefix, 96 and more of one
-//                                          sequence over prefix and own cache: tensor memory;
+//   attend_tiles (sc_attention_tile.cu)    64 rows and more over the prefix, 32 to 96 and more of
+//                                          one sequence over prefix and own cache: tensor memory;
 //   attend_stream (sc_attention_stream.cu) fewer: HBM bounds it;
 //   attend_rows (here)                     what tensor maps cannot say: pages that no box of 8 rows
 //                                          divides, expanded strides, more than 8,192 sequences.
@@ -563,7 +563,8 @@ constexpr int kTileRows = 256, kTileTokens = 128, kStepTokens = 64;
 constexpr int kMinTileRows = 64;   // fewer rows: the copies bound both kernels
 constexpr int kTailParts = 16;     // of a unit in the last round, at most
 constexpr int kMaxFused = 1024;    // sequences: every block counts their units
-constexpr int kMinFusedRows = 96;  // fewer rows a sequence: packing the batch's rows wins
+constexpr int kMinFusedRows = 32;  // of a sequence and KV head: fewer leave a row tile nearly empty
+constexpr int kAllFusedRows = 96;  // from here on packing the batch's rows never won
 
 // Parts of the token axis for attend_tiles: the number that ends soonest, in units of one step
 // (256 rows x 128 tokens, about 2 us), counting whole rounds of 148 blocks, a block's start and
@@ -580,12 +581,29 @@ int32_t plan_parts(double blocks, int64_t steps, double rows, int32_t D) {
     return best;
 }
 
+// Whether attend_tiles takes each sequence's rows over prefix and own cache (a row tile each, mostly
+// empty with few rows), or the batch's rows packed over the prefix and attend_stream the caches (whose
+// parts go through memory): whichever is estimated to end first, in us.  Measured (fused, packed), 8 KV
+// heads of 128: 16 sequences of 64 rows behind 4,096 with 500 own 62, 103; 4 behind 8,192 with 300 39, 62;
+// 32 of 40 rows behind 1,000 with 1,000 69, 165; 64 of 32 rows behind 4,096 with 500 212, 141; 16 of 40
+// rows of 64 behind 4,099 with 700 64, 51.
+bool fuse(int64_t rows_p, int64_t rows_c, int32_t B, int32_t Hkv, int32_t D, int32_t P, int32_t cap) {
+    if (rows_c < kMinFusedRows || rows_c >= kAllFusedRows) return rows_c >= kAllFusedRows;
+    const double units = static_cast<double>(B) * Hkv;
+    const double steps_p = (P + kTileTokens - 1) / kTileTokens, steps_c = (cap + kTileTokens - 1) / kTileTokens;
+    const double fused = 12.0 + units * (steps_p + steps_c) * 1.5 / kSms;
+    const double prefix = static_cast<double>((rows_p + kTileRows - 1) / kTileRows) * Hkv * steps_p * 2.3;
+    const double caches = units * ((rows_c + 31) / 32) * ((cap + kStepTokens - 1) / kStepTokens) * 2.6;
+    const double packed = 24.0 + (prefix + caches / (D <= 64 ? 2 : 1)) / kSms;
+    return fused < packed;
+}
+
 int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int32_t nq, int32_t P,
                    int32_t cap, int32_t page, Split* out) {
     const int64_t G = Hq / Hkv;
     const int64_t rows_p = N * G, rows_c = cap ? nq * G : 0;
     Split s{};
-    s.fused = D <= 128 && cap && rows_c >= kMinFusedRows && B <= kMaxFused;
+    s.fused = D <= 128 && cap && B <= kMaxFused && fuse(rows_p, rows_c, B, Hkv, D, P, cap);
     s.tile_p = !s.fused && D <= 128 && P && rows_p >= kMinTileRows;
     const double rows = static_cast<double>(N) * Hq;
     if (s.fused) {
