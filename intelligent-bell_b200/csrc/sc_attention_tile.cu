@@ -21,6 +21,7 @@
 #include <math.h>
 
 #include "sc_tensor.cuh"
+#include "sc_tile_waits.h"
 
 namespace sc {
 namespace {
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         const float f = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
                         l *= f;
-                        if (i > 0) {
+                        if (i > 0) {  // the scores are there, so phase i - 2 is over: i - 1 is the open one
                             alive = bar_wait_warp(o_full(q), (i - 1) & 1, gave_up);
                             if (!alive) return;
                             tc_fence_after();
@@ -662,11 +663,16 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     }
                     tmem_wait_st();
                 }
+                const int o_phase = phase_before_weights(n_q, i, n_tiles);
+                if (o_phase >= 0) {
+                    alive = bar_wait_warp(o_full(q), o_phase & 1, gave_up);
+                    if (!alive) break;
+                }
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) bar_arrive(p_full(buf));
             }
-            if (alive) {
+            if (alive) {  // phase n_tiles - 2 is over (phase_before_weights): this is the open one
                 alive = bar_wait_warp(o_full(q), (n_tiles - 1) & 1, gave_up);
             }
             if (alive && any) {
