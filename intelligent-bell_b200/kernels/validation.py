@@ -129,18 +129,41 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return lo, lo + (last + 1) * t.element_size()
 
 
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors are known to share no byte.
+
+    Their extents do not meet, or their elements lie in different parts of some period: modulo a stride
+    of theirs, of which every longer stride is a multiple, each covers one run of bytes (keys and values,
+    or the heads of q and k, side by side in one buffer).
+    """
+    alo, ahi = _extent(a)
+    blo, bhi = _extent(b)
+    if alo >= bhi or blo >= ahi:
+        return True
+    steps = [[s * t.element_size() for n, s in zip(t.shape, t.stride()) if n > 1] for t in (a, b)]
+    sizes = [[n for n in t.shape if n > 1] for t in (a, b)]
+    for period in {s for x in steps for s in x if s > 0}:
+        runs = []
+        for t, step, size in zip((a, b), steps, sizes):
+            run = t.element_size()
+            for n, s in zip(size, step):
+                if s % period:
+                    run += (n - 1) * s if s < period else period
+            runs.append(run)
+        off = (blo - alo) % period
+        if runs[0] <= off and off + runs[1] <= period:
+            return True
+    return False
+
+
 def require_apart(name: str, out: torch.Tensor, *others: torch.Tensor | None) -> None:
-    """``out`` names each of its elements once and reaches into none of ``others``."""
+    """``out`` names each of its elements once and none of ``others``'."""
     if 0 in out.stride():
         for n, s in zip(out.shape, out.stride()):
             if s == 0 and n > 1:
                 raise ValueError(f"{name} must not be an expanded tensor (strides {tuple(out.stride())})")
-    lo, hi = _extent(out)
     for t in others:
-        if t is None:
-            continue
-        a, b = _extent(t)
-        if lo < b and a < hi and t.device == out.device:
+        if t is not None and t.device == out.device and not _apart(out, t):
             raise ValueError(f"{name} must not overlap an input or another output")
 
 
