@@ -49,9 +49,9 @@ def evict_tokens(
         scores: float32 ``[B, Hkv, S]``, as :func:`accumulate_attention_weights` gives them.
         cache_lens: ``[B]`` tokens in use (default: all).
         k_out, v_out: ``[B, budget, Hkv, D]``, and ``scores_out`` float32 ``[B, Hkv, budget]``.  An
-            output may be its input's first ``budget`` tokens: then that one moves in place.  Rows
-            behind a sequence's new length are left as they were (in outputs allocated here:
-            zeros).
+            output may be its input's first ``budget`` tokens: then that one moves in place, and no
+            other input may reach into it (one tensor as keys and values).  Rows behind a
+            sequence's new length are left as they were (in outputs allocated here: zeros).
 
     Returns :class:`Evicted`.
     """
@@ -85,8 +85,8 @@ def evict_tokens(
     in_place = False
     inputs = (k_cache, v_cache, scores)
     outs: list[torch.Tensor] = []
-    for name, src, out in (("k_out", k_cache, k_out), ("v_out", v_cache, v_out),
-                           ("scores_out", scores, scores_out)):
+    for role, (name, src, out) in enumerate((("k_out", k_cache, k_out), ("v_out", v_cache, v_out),
+                                             ("scores_out", scores, scores_out))):
         if out is None:
             if name == "scores_out":
                 out = fresh((b, h, budget), dtype=torch.float32, device=dev)
@@ -103,8 +103,8 @@ def evict_tokens(
             if budget > s:
                 raise ValueError(f"{name} in place cannot hold more than its {s} tokens")
             in_place = True
-            require_apart(name, out, *outs, *(x for x in inputs if x is not src and x is not k_cache
-                                              and x is not v_cache))
+            # keys, values and scores move in blocks of their own, in no order among them
+            require_apart(name, out, *outs, *inputs[:role], *inputs[role + 1:])
         else:
             require_apart(name, out, *outs, *inputs)
         outs.append(out)

@@ -63,3 +63,44 @@ def test_no_pair_that_shares_an_element_is_called_apart(validation):
             claimed += 1
             assert not elements(views[0]) & elements(views[1])
     assert claimed > 400
+
+
+@pytest.fixture
+def stand_in(scb, monkeypatch):
+    """Calls on CPU tensors that pass every check end here; the names of those that did."""
+    reached = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda *args: reached.append(name) or 0
+
+    monkeypatch.setattr(scb._lib, "load", lambda: Library())
+    monkeypatch.setattr(scb._lib, "on_device", lambda dev: contextlib.nullcontext())
+    monkeypatch.setattr(scb._lib, "stream_handle", lambda dev: None)
+    for name in ("evict", "rotary", "attention"):
+        module = importlib.import_module(f"{scb.__name__}.kernels.{name}")
+        monkeypatch.setattr(module, "require_cuda", lambda t: None)
+        if hasattr(module, "_status_word"):
+            monkeypatch.setattr(module, "_status_word", lambda dev: torch.zeros(1, dtype=torch.int32))
+    return reached
+
+
+def test_eviction_in_place_over_the_other_cache_is_refused(scb, stand_in):
+    x, scores = torch.zeros((2, 50, 3, 64), dtype=torch.float16), torch.zeros((2, 3, 50))
+    for v in (x, x.view(x.shape)):
+        with pytest.raises(ValueError, match="k_out must not overlap"):
+            scb.evict_tokens(x, v, scores, 20, k_out=x[:, :20])
+        with pytest.raises(ValueError, match="v_out must not overlap"):
+            scb.evict_tokens(x, v, scores, 20, v_out=v[:, :20])
+        with pytest.raises(ValueError, match="overlap"):
+            scb.evict_tokens(x, v, scores, 20, k_out=x[:, :20], v_out=v[:, :20])
+    longer = torch.zeros((2, 51, 3, 64), dtype=torch.float16)  # values one token behind the keys
+    with pytest.raises(ValueError, match="k_out must not overlap"):
+        scb.evict_tokens(longer[:, :50], longer[:, 1:], scores, 20, k_out=longer[:, :20])
+    assert not stand_in
+    scb.evict_tokens(x, x, scores, 20)  # nothing in place: one tensor may be both
+    kv = torch.zeros((2, 50, 2, 3, 64), dtype=torch.float16)
+    k, v = kv[:, :, 0], kv[:, :, 1]
+    scb.evict_tokens(k, v, scores, 20, k_out=k[:, :20], v_out=v[:, :20], scores_out=scores[..., :20])
+    scb.evict_tokens(k, v, scores, 20, k_out=k[:, :20])
+    assert len(stand_in) == 3
