@@ -193,8 +193,8 @@ def apply_rotary(
         interleaved: pairs are neighbours (2i, 2i + 1) instead of (i, i + rotary_dim / 2).
         scaling: a :class:`RopeScaling`; None: unscaled.
         inverse: undo the rotation (and the scaling's factor) instead.
-        q_out, k_out: outputs of the inputs' shape and dtype, any strides (a cache's next slots,
-            or the input itself); new contiguous tensors by default.
+        q_out, k_out: outputs of the inputs' shape and dtype, any strides (a cache's next slots, or
+            the input itself, apart from the other input); new contiguous tensors by default.
 
     Angles are kept to 2^-33 of a turn at any position below 2^31; products are in float32 and
     rounded once.  Returns ``q_out``, or ``(q_out, k_out)`` when keys are given.
@@ -222,10 +222,10 @@ def apply_rotary(
             if out.dtype != x.dtype:
                 raise TypeError(f"{name} must be {x.dtype}, got {out.dtype}")
             if same_view(out, x):
-                require_apart(name, out)
+                require_apart(name, out, other)
             else:
                 require_apart(name, out, x, other)
-    if q_out is not None and k_out is not None and not (same_view(qo, q) and same_view(ko, k)):
+    if q_out is not None and k_out is not None:
         require_apart("k_out", ko, qo)
 
     start, pos_ptr, pos64, ps = 0, None, 0, (0, 0)

@@ -104,3 +104,22 @@ def test_eviction_in_place_over_the_other_cache_is_refused(scb, stand_in):
     scb.evict_tokens(k, v, scores, 20, k_out=k[:, :20], v_out=v[:, :20], scores_out=scores[..., :20])
     scb.evict_tokens(k, v, scores, 20, k_out=k[:, :20])
     assert len(stand_in) == 3
+
+
+def test_rotation_in_place_over_the_other_input_is_refused(scb, stand_in):
+    x = torch.zeros((6, 4, 64), dtype=torch.float16)
+    for kw in (dict(q_out=x), dict(k_out=x), dict(q_out=x, k_out=x)):
+        with pytest.raises(ValueError, match="overlap"):
+            scb.apply_rotary(x, x, 0, **kw)
+    qkv = torch.zeros((6, 8, 64), dtype=torch.float16)
+    q, k = qkv[:, :4], qkv[:, 4:6]
+    for both in (qkv[:, 3:5], qkv[:, :6]):  # keys that reach into the queries
+        with pytest.raises(ValueError, match="q_out must not overlap"):
+            scb.apply_rotary(q, both, 0, q_out=q)
+    assert not stand_in
+    scb.apply_rotary(x, x, 0)
+    for kw in (dict(q_out=q), dict(k_out=k), dict(q_out=q, k_out=k), dict(q_out=torch.zeros_like(q), k_out=k)):
+        scb.apply_rotary(q, k, 0, **kw)
+    wide = qkv[None].expand(1, 6, 8, 64).transpose(1, 2)  # the model layout
+    scb.apply_rotary(wide[:, :4], wide[:, 4:6], 0, q_out=wide[:, :4], k_out=wide[:, 4:6])
+    assert len(stand_in) == 6
