@@ -129,6 +129,11 @@ class SpecDynamicCache:
         return (self._k[layer_idx][:, :, start:start + n_tokens],
                 self._v[layer_idx][:, :, start:start + n_tokens])
 
+    def views_with(self, layer_idx: int, n_tokens: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """The layer as it will be once the next ``n_tokens`` are committed."""
+        end = self._len[layer_idx] + n_tokens
+        return self._k[layer_idx][:, :, :end], self._v[layer_idx][:, :, :end]
+
     def commit(self, layer_idx: int, n_tokens: int) -> None:
         self._len[layer_idx] += int(n_tokens)
 

@@ -92,15 +92,16 @@ class SharedPrefixCache:
                      k_out=k_slot)
         v_slot.copy_(v)
         start = self.own.get_seq_length(layer_idx)
-        self.own.commit(layer_idx, n)
-        self._seen[layer_idx] += n
-        k_own, v_own = (x.transpose(1, 2) for x in self.own[layer_idx])
+        k_own, v_own = (x.transpose(1, 2) for x in self.own.views_with(layer_idx, n))
         k_pre, v_pre = self.prefix_views(layer_idx)
         turned = turned.view(b * n, hq, d)
         out, lse = shared_prefix_attention(turned, k_pre, v_pre, k_own, v_own, scale=scale)
         if self.track_weights:
             scores = self._room_for_scores(layer_idx, start, start + n, h, k.device)
             accumulate_attention_weights(turned, k_own, lse, scores, scale=scale)
+        # nothing was refused: the step's tokens are the cache's
+        self.own.commit(layer_idx, n)
+        self._seen[layer_idx] += n
         return out.view(b, n, hq, d).transpose(1, 2)
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_recent: int = 0) -> None:

@@ -1,0 +1,100 @@
+"""What SharedPrefixCache keeps of its steps, on the CPU: lengths, positions and weights, with the
+operators replaced by plain ones."""
+
+from __future__ import annotations
+
+import importlib
+
+import pytest
+import torch
+
+BATCH, HEADS, KV_HEADS, DIM = 2, 4, 2, 8
+
+
+@pytest.fixture
+def steps(scb, monkeypatch):
+    """The module with plain operators; ``steps.positions`` lists the first position of each rotation and
+    ``steps.refuse`` names the operator that refuses its next call."""
+    module = importlib.import_module(scb.__name__ + ".serving.shared_prefix")
+    kv_injector = importlib.import_module(scb.__name__ + ".serving.kv_injector")
+
+    class Steps:
+        positions: list[int] = []
+        refuse: str | None = None
+        SharedPrefixCache, SpecDynamicCache = module.SharedPrefixCache, module.SpecDynamicCache
+
+    s = Steps()
+    s.positions = []
+
+    def maybe_refuse(name):
+        if s.refuse == name:
+            s.refuse = None
+            raise ValueError(f"{name} refused")
+
+    def rotary(q, k, position, *, q_out, k_out, **_):
+        maybe_refuse("rotary")
+        s.positions.append(position)
+        q_out.copy_(q)
+        k_out.copy_(k + position)  # a key that tells where it was turned
+
+    def attention(q, k_prefix, v_prefix, k, v, **_):
+        maybe_refuse("attention")
+        n = q.shape[0] // k.shape[0]
+        seen = torch.arange(k.shape[1]) <= k.shape[1] - n + torch.arange(n)[:, None]       # [n, S]
+        x = torch.einsum("bnhd,bshd->bnhs", q.view(-1, n, *q.shape[1:]),
+                         k.repeat_interleave(HEADS // KV_HEADS, 2)).masked_fill(~seen[:, None], -torch.inf)
+        return q.clone(), torch.logsumexp(x, -1).reshape(-1, HEADS)
+
+    def weights(q, k, lse, scores, cache_lens=None, *, scale=None, out=None):
+        maybe_refuse("weights")
+        n = q.shape[0] // k.shape[0]
+        seen = torch.arange(k.shape[1]) <= k.shape[1] - n + torch.arange(n)[:, None]
+        x = torch.einsum("bnhd,bshd->bnhs", q.view(-1, n, *q.shape[1:]), k.repeat_interleave(HEADS // KV_HEADS, 2))
+        w = torch.exp(x - lse.view(-1, n, HEADS, 1)).masked_fill(~seen[:, None], 0.0).sum(1)
+        got = scores + w.view(w.shape[0], KV_HEADS, -1, w.shape[-1]).sum(2)
+        return (scores if out is None else out).copy_(got)
+
+    def evict(k, v, scores, budget, *, keep_first, keep_recent, k_out, v_out, scores_out):
+        for x in (k, v):  # any tokens do: the last ones
+            x[:, :budget] = x[:, -budget:].clone()
+        scores[..., :budget] = scores[..., -budget:].clone()
+
+    monkeypatch.setattr(module, "apply_rotary", rotary)
+    monkeypatch.setattr(module, "shared_prefix_attention", attention)
+    monkeypatch.setattr(module, "accumulate_attention_weights", weights)
+    monkeypatch.setattr(kv_injector, "evict_tokens", evict)
+    return s
+
+
+def prefix(steps, n=3):
+    cache = steps.SpecDynamicCache()
+    x = torch.zeros((1, KV_HEADS, n, DIM))
+    for layer in range(2):
+        cache.update(x, x, layer)
+    return cache
+
+
+def step(n, seed):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn((BATCH, HEADS, n, DIM), generator=g),
+            *(torch.randn((BATCH, KV_HEADS, n, DIM), generator=g) for _ in range(2)))
+
+
+@pytest.mark.parametrize("operator", ["rotary", "attention", "weights"])
+def test_a_refused_step_leaves_nothing_behind(steps, operator):
+    cache = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    twin = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    for i, n in enumerate((4, 1, 3)):
+        if i:
+            before = cache.own[0][0].clone(), cache.own[0][1].clone(), cache.scores(0).clone()
+            steps.refuse = operator
+            with pytest.raises(ValueError, match="refused"):
+                cache.attend(0, *step(n, 50))
+            assert cache.get_seq_length(0) == twin.get_seq_length(0)
+            assert cache.next_position(0) == twin.next_position(0)
+            assert all(torch.equal(a, b) for a, b in zip(before, (*cache.own[0], cache.scores(0))))
+        for c in (cache, twin):
+            c.attend(0, *step(n, i))
+    assert cache.get_seq_length(0) == 3 + 8 and cache.next_position(0) == 11
+    assert all(torch.equal(a, b) for a, b in zip(cache.own[0], twin.own[0]))
+    assert torch.equal(cache.scores(0), twin.scores(0))
