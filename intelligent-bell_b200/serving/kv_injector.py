@@ -35,6 +35,7 @@ class SpecDynamicCache:
         self._k: list[torch.Tensor | None] = []
         self._v: list[torch.Tensor | None] = []
         self._len: list[int] = []
+        self._evicted: list[int] = []  # tokens that evict has dropped since the layer was last empty
         self._default_capacity = int(capacity)
 
     # -- reference interface ----------------------------------------------------------------
@@ -75,6 +76,8 @@ class SpecDynamicCache:
         for i in range(len(self._len)):
             if self._k[i] is not None and self._len[i] > max_seq_len:
                 self._len[i] = max(0, int(max_seq_len))
+                if self._len[i] == 0:
+                    self._evicted[i] = 0
 
     def to_legacy_cache(self) -> tuple[tuple[torch.Tensor, torch.Tensor], ...]:
         return tuple(self[i] for i in range(len(self._k)) if self._k[i] is not None)
@@ -94,6 +97,7 @@ class SpecDynamicCache:
             self._k.append(None)
             self._v.append(None)
             self._len.append(0)
+            self._evicted.append(0)
         buf = self._k[layer_idx]
         need = self._len[layer_idx] + int(extra_tokens)
         if buf is not None:
@@ -153,7 +157,13 @@ class SpecDynamicCache:
         out = evict_tokens(k, v, scores, m, keep_first=keep_first, keep_recent=keep_recent,
                            k_out=k[:, :m], v_out=v[:, :m], scores_out=scores[..., :m])
         self._len[layer_idx] = m
+        self._evicted[layer_idx] += n - m
         return out
+
+    def evicted_tokens(self, layer_idx: int = 0) -> int:
+        """Tokens of each head that :meth:`evict` has dropped: with the layer's length, how many it was
+        given and did not truncate."""
+        return self._evicted[layer_idx] if layer_idx < len(self._evicted) else 0
 
     def _append(self, layer_idx: int, like: torch.Tensor, t: int):
         b, h, _, d = like.shape

@@ -41,7 +41,6 @@ class SharedPrefixCache:
         self.interleaved, self.scaling = bool(interleaved), scaling
         self.track_weights = bool(track_weights)
         self._scores: list[torch.Tensor | None] = []
-        self._seen: list[int] = []  # own tokens so far, evicted ones included
 
     def prefix_views(self, layer_idx: int) -> tuple[torch.Tensor, torch.Tensor] | tuple[None, None]:
         """Token-major ``[P, H, D]`` views of the prefix layer (None, None: it has none)."""
@@ -57,9 +56,9 @@ class SharedPrefixCache:
         return self.prefix.get_seq_length(layer_idx) + self.own.get_seq_length(layer_idx)
 
     def next_position(self, layer_idx: int = 0) -> int:
-        """Position of the layer's next token: behind the prefix and every own token so far."""
-        seen = self._seen[layer_idx] if layer_idx < len(self._seen) else 0
-        return self.prefix.get_seq_length(layer_idx) + seen
+        """Position of the layer's next token: behind the prefix and every own token so far, evicted
+        ones included, truncated ones not."""
+        return self.get_seq_length(layer_idx) + self.own.evicted_tokens(layer_idx)
 
     def scores(self, layer_idx: int) -> torch.Tensor:
         """float32 ``[B, H, own length]`` accumulated weights of the layer's own tokens."""
@@ -81,8 +80,7 @@ class SharedPrefixCache:
         if v.dtype != k.dtype or v.device != k.device:
             raise ValueError(f"v is {v.dtype} on {v.device}, k {k.dtype} on {k.device}")
         h = k.shape[1]
-        while len(self._seen) <= layer_idx:
-            self._seen.append(0)
+        while len(self._scores) <= layer_idx:
             self._scores.append(None)
         self.own.reserve(layer_idx, n, batch=b, heads=h, head_dim=d, dtype=k.dtype, device=k.device)
         k_slot, v_slot = self.own.append_slots(layer_idx, n)
@@ -101,7 +99,6 @@ class SharedPrefixCache:
             accumulate_attention_weights(turned, k_own, lse, scores, scale=scale)
         # nothing was refused: the step's tokens are the cache's
         self.own.commit(layer_idx, n)
-        self._seen[layer_idx] += n
         return out.view(b, n, hq, d).transpose(1, 2)
 
     def evict(self, budget: int, *, keep_first: int = 0, keep_recent: int = 0) -> None:

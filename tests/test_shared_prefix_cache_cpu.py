@@ -98,3 +98,25 @@ def test_a_refused_step_leaves_nothing_behind(steps, operator):
     assert cache.get_seq_length(0) == 3 + 8 and cache.next_position(0) == 11
     assert all(torch.equal(a, b) for a, b in zip(cache.own[0], twin.own[0]))
     assert torch.equal(cache.scores(0), twin.scores(0))
+
+
+def test_positions_follow_truncation_and_eviction(steps):
+    cache = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    for layer in range(2):
+        cache.attend(layer, *step(10, 1))
+        cache.attend(layer, *step(5, 2))
+    cache.own.truncate(12)  # three of the five are rejected
+    assert cache.next_position(0) == cache.next_position(1) == 3 + 12
+    cache.attend(0, *step(1, 3))
+    assert steps.positions[-1] == 15
+    cache.evict(8)
+    assert cache.own.get_seq_length(0) == 8 and cache.own.evicted_tokens(0) == 5 and cache.next_position(0) == 16
+    assert cache.own.evicted_tokens(1) == 4 and cache.next_position(1) == 15
+    cache.attend(0, *step(4, 4))
+    assert steps.positions[-1] == 16
+    cache.own.truncate(9)
+    assert cache.next_position(0) == 17 and cache.next_position(1) == 15
+    cache.own.truncate(0)  # all over again
+    assert cache.next_position(0) == cache.next_position(1) == 3 and cache.own.evicted_tokens(0) == 0
+    cache.attend(1, *step(2, 5))
+    assert steps.positions[-1] == 3 and cache.own.evicted_tokens(7) == 0
