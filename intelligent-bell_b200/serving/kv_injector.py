@@ -79,6 +79,10 @@ class SpecDynamicCache:
                 if self._len[i] == 0:
                     self._evicted[i] = 0
 
+    def truncate_layer(self, layer_idx: int, max_seq_len: int) -> None:
+        """:meth:`truncate` of one layer; what was evicted from it stays counted."""
+        self._len[layer_idx] = min(self._len[layer_idx], max(0, int(max_seq_len)))
+
     def to_legacy_cache(self) -> tuple[tuple[torch.Tensor, torch.Tensor], ...]:
         return tuple(self[i] for i in range(len(self._k)) if self._k[i] is not None)
 

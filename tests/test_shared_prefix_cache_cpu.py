@@ -37,20 +37,22 @@ def steps(scb, monkeypatch):
         q_out.copy_(q)
         k_out.copy_(k + position)  # a key that tells where it was turned
 
+    def products(q, k, n):  # in 64 bits, so that only the scores' own float32 rounds
+        return torch.einsum("bnhd,bshd->bnhs", q.view(-1, n, *q.shape[1:]).double(),
+                            k.repeat_interleave(HEADS // KV_HEADS, 2).double())
+
     def attention(q, k_prefix, v_prefix, k, v, **_):
         maybe_refuse("attention")
         n = q.shape[0] // k.shape[0]
         seen = torch.arange(k.shape[1]) <= k.shape[1] - n + torch.arange(n)[:, None]       # [n, S]
-        x = torch.einsum("bnhd,bshd->bnhs", q.view(-1, n, *q.shape[1:]),
-                         k.repeat_interleave(HEADS // KV_HEADS, 2)).masked_fill(~seen[:, None], -torch.inf)
+        x = products(q, k, n).masked_fill(~seen[:, None], -torch.inf)
         return q.clone(), torch.logsumexp(x, -1).reshape(-1, HEADS)
 
     def weights(q, k, lse, scores, cache_lens=None, *, scale=None, out=None):
         maybe_refuse("weights")
         n = q.shape[0] // k.shape[0]
         seen = torch.arange(k.shape[1]) <= k.shape[1] - n + torch.arange(n)[:, None]
-        x = torch.einsum("bnhd,bshd->bnhs", q.view(-1, n, *q.shape[1:]), k.repeat_interleave(HEADS // KV_HEADS, 2))
-        w = torch.exp(x - lse.view(-1, n, HEADS, 1)).masked_fill(~seen[:, None], 0.0).sum(1)
+        w = torch.exp(products(q, k, n) - lse.view(-1, n, HEADS, 1)).masked_fill(~seen[:, None], 0.0).sum(1)
         got = scores + w.view(w.shape[0], KV_HEADS, -1, w.shape[-1]).sum(2)
         return (scores if out is None else out).copy_(got)
 
@@ -120,3 +122,72 @@ def test_positions_follow_truncation_and_eviction(steps):
     assert cache.next_position(0) == cache.next_position(1) == 3 and cache.own.evicted_tokens(0) == 0
     cache.attend(1, *step(2, 5))
     assert steps.positions[-1] == 3 and cache.own.evicted_tokens(7) == 0
+
+
+@pytest.mark.parametrize("accepted", [0, 1, 3, 4])
+def test_a_rejected_draft_is_taken_back(steps, accepted):
+    """As if only the accepted tokens had been given: lengths, positions, keys and weights."""
+    cache = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    twin = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    draft = step(5, 9)
+    for layer in range(2):
+        for c in (cache, twin):
+            c.attend(layer, *step(6, 1))
+        cache.attend(layer, *draft)
+        if accepted:
+            twin.attend(layer, *(x[:, :, :accepted] for x in draft))
+    if accepted == 3:
+        cache.truncate(3 + 6 + 4)  # in two goes
+    cache.truncate(3 + 6 + accepted)
+    for n, seed in ((1, 3), (2, 4)):
+        for layer in range(2):
+            assert cache.get_seq_length(layer) == twin.get_seq_length(layer)
+            assert cache.next_position(layer) == twin.next_position(layer)
+            assert all(torch.equal(a, b) for a, b in zip(cache.own[layer], twin.own[layer]))
+            # four steps at most, each rounded once to float32 on either side: 4 x 2 x 2^-24 = 4.8e-7
+            assert torch.allclose(cache.scores(layer), twin.scores(layer), rtol=1e-6, atol=0)
+            for c in (cache, twin):
+                c.attend(layer, *step(n, seed))
+
+
+def test_what_cannot_be_taken_back_is_refused(steps):
+    cache = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    cache.attend(0, *step(4, 1))
+    cache.attend(0, *step(3, 2))
+    cache.attend(1, *step(70, 3))
+    before = cache.scores(0).clone(), cache.scores(1).clone()
+    for bad in (2, 3 + 3, 3 + 5):  # into the prefix, behind layer 0's last step, into layer 1's long one
+        with pytest.raises(ValueError, match="cut|part"):
+            cache.truncate(bad)
+        assert cache.get_seq_length(0) == 10 and cache.get_seq_length(1) == 73
+        assert torch.equal(cache.scores(0), before[0]) and torch.equal(cache.scores(1), before[1])
+    cache.truncate(73)
+    steps.refuse = "weights"
+    with pytest.raises(ValueError, match="refused"):  # a refused step between makes no difference
+        cache.attend(0, *step(40, 5))
+    cache.evict(4, keep_first=0, keep_recent=0)
+    with pytest.raises(ValueError, match="cut back to 4"):
+        cache.truncate(3 + 3)
+    cache.attend(0, *step(3, 6))
+    cache.attend(1, *step(3, 6))
+    cache.truncate(3 + 5)
+    assert cache.own.get_seq_length(0) == cache.own.get_seq_length(1) == 5
+    assert cache.next_position(0) == 3 + 7 + 1 and cache.next_position(1) == 3 + 70 + 1
+    plain = steps.SharedPrefixCache(prefix(steps), BATCH)  # no weights: any length
+    plain.attend(0, *step(4, 1))
+    plain.attend(0, *step(3, 2))
+    plain.truncate(3 + 2)
+    assert plain.next_position(0) == 5 and plain.get_seq_length(0) == 5
+
+
+def test_a_refused_step_does_not_spoil_the_way_back(steps):
+    cache = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    twin = steps.SharedPrefixCache(prefix(steps), BATCH, track_weights=True)
+    for c in (cache, twin):
+        c.attend(0, *step(6, 1))
+    cache.attend(0, *step(5, 2))
+    steps.refuse = "weights"
+    with pytest.raises(ValueError, match="refused"):
+        cache.attend(0, *step(60, 5))  # its scores need more room than there was
+    cache.truncate(3 + 6)
+    assert torch.equal(cache.scores(0), twin.scores(0)) and cache.next_position(0) == 9
