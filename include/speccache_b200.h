@@ -387,8 +387,10 @@ SC_API int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_heads, i
  *               page_table, page_size = cache_len
  *  cache_lens   device int32 [batch], tokens in use (the queries' own among them); NULL: all
  *  page_table   device int32, row stride page_table_stride
- *  cu_q_lens    device int32 [batch + 1], each sequence's first token; NULL: max_q_len each.
- *               Rows before the first sequence and behind the last are left as they were.
+ *  cu_q_lens    device int32 [batch + 1], each sequence's first token; NULL: max_q_len each.  A
+ *               sequence whose starts decrease, lie outside those of the first and the last or
+ *               are more than max_q_len apart has no rows (SC_STATUS_BAD_SEQ_LEN).  Rows of no
+ *               sequence are left as they were, of two (starts that decrease) undefined.
  *  lse          float32 [n_tokens, q_heads], natural logarithm, contiguous; may be NULL
  *  workspace    of sc_shared_prefix_attention_workspace bytes, 16-byte aligned, for this call
  *               alone until its work has completed

@@ -418,12 +418,14 @@ template <typename T, int W>
 __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ AttnParams p) {
     __shared__ float4 s_o[kWarps][64];
     __shared__ float s_sum[kWarps];
-    wait_for_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kWarps + warp : blockIdx.x;
     const int64_t all_rows = static_cast<int64_t>(p.N) * p.Hq;
-    if (row >= static_cast<int64_t>(used_tokens(p)) * p.Hq) return;
-    if (p.cu_q != nullptr && row < static_cast<int64_t>(p.cu_q[0]) * p.Hq) return;  // of no sequence
+    // Rows of no sequence stay as they are: nobody has written their own caches' parts.
+    const bool counts = row < all_rows && in_sequence(p, static_cast<int>(row / p.Hq));
+    if (p.cap == 0 && blockIdx.x == 0 && warp == 0) report_sequences(p);  // no kernel before it looked at them
+    wait_for_previous();
+    if (!counts) return;
     const int parts = p.n_pp + p.n_cp;
     const int each = (parts + W - 1) / W, i0 = W == 1 ? 0 : warp * each, i1 = min(parts, i0 + each);
     float m = kNegInf;
@@ -633,7 +635,7 @@ int32_t plan_split(int32_t N, int32_t B, int32_t Hq, int32_t Hkv, int32_t D, int
                     if (best < 0. || cost < best) best = cost, s.n_pp = n, s.sms_left = left;
                 }
             }
-            s.direct = s.n_pp == 1 && !cap;
+            s.direct = s.n_pp == 1 && !B;  // with sequences, join_parts knows whose rows count
             s.units_tile = size_product(s.n_pp, s.tiles_p, Hkv);
         }
         const int64_t rows_most = !P || s.tile_p ? rows_c : rows_p > rows_c ? rows_p : rows_c;

@@ -84,16 +84,8 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
 
     // A sequence's tokens of q and length; the kernel's first block reports what is wrong with them.
     auto sequence = [&](int b, int& tok0, int& n, int& len) {
-        tok0 = b * p.nq;
-        n = p.nq;
         len = p.cap;
-        bool fine = true;
-        if (p.cu_q != nullptr) {
-            const int a = p.cu_q[b], e = p.cu_q[b + 1];
-            fine = a >= 0 && e >= a && e <= p.N && e - a <= p.nq;
-            tok0 = fine ? a : 0;
-            n = fine ? e - a : 0;
-        }
+        bool fine = sequence_of(p, b, tok0, n);
         if (p.cache_lens != nullptr) {
             len = p.cache_lens[b];
             if (len < 0 || len > p.cap) {

@@ -62,11 +62,8 @@ struct Round {
     int units, full, rem, parts;  // units before the last round, in it, and parts of each there
 };
 __device__ __forceinline__ int units_of(const AttnParams& p, int b) {
-    int n = p.nq;
-    if (p.cu_q != nullptr) {
-        const int a = p.cu_q[b], e = p.cu_q[b + 1];
-        n = a >= 0 && e >= a && e <= p.N && e - a <= p.nq ? e - a : 0;
-    }
+    int tok0, n;
+    sequence_of(p, b, tok0, n);
     return (n * p.G + 2 * kRowTile - 1) / (2 * kRowTile);
 }
 __device__ __forceinline__ Round rounds(const TileParams& tp) {
@@ -160,6 +157,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     int tok0 = 0, n_tok, len = 0;
     let_next_start();
     if (tp.per_seq) {
+        // Sequences of no rows have no block that would report what is wrong with them.
+        if (blockIdx.x == 0 && warp == 10) report_sequences(p);
         const Round r = rounds(tp);
         int u = blockIdx.x;
         splits = 1;
@@ -185,7 +184,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
         h = u / tp.tiles;
         n_tok = used_tokens(p);
     }
-    const bool direct = splits == 1 && (tp.per_seq || p.n_pp + p.n_cp == 1);
+    const bool direct = splits == 1 && (tp.per_seq || (p.n_pp == 1 && p.B == 0));
     const int rows = n_tok * p.G;
     const int r0 = rt * 2 * kRowTile;
     if (r0 >= rows) {

@@ -47,16 +47,8 @@ __global__ void __launch_bounds__(kWThreads) add_weights(const __grid_constant__
     const int h = u % p.Hkv, b = u / p.Hkv;
 
     int tok0, n_tok;
-    if (p.cu_q == nullptr) {
-        tok0 = b * p.nq;
-        n_tok = p.nq;
-    } else {
-        const int a = p.cu_q[b], e = p.cu_q[b + 1];
-        const bool fine = a >= 0 && e >= a && e <= p.N && e - a <= p.nq;
-        if (!fine && threadIdx.x == 0) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
-        tok0 = fine ? a : 0;
-        n_tok = fine ? e - a : 0;
-    }
+    if (!sequence_of(p.cu_q, p.B, p.N, p.nq, b, tok0, n_tok) && threadIdx.x == 0)
+        atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
     int len = p.S;
     if (p.cache_lens != nullptr) {
         len = p.cache_lens[b];

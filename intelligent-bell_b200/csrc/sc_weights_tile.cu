@@ -79,16 +79,7 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
         const int len = p.cache_lens[b];
         return len < 0 || len > p.S ? 0 : len;
     };
-    auto tokens_of = [&](int b, int& tok0, int& n) {
-        tok0 = b * p.nq;
-        n = p.nq;
-        if (p.cu_q != nullptr) {
-            const int a = p.cu_q[b], e = p.cu_q[b + 1];
-            const bool fine = a >= 0 && e >= a && e <= p.N && e - a <= p.nq;
-            tok0 = fine ? a : 0;
-            n = fine ? e - a : 0;
-        }
-    };
+    auto tokens_of = [&](int b, int& tok0, int& n) { return sequence_of(p.cu_q, p.B, p.N, p.nq, b, tok0, n); };
 
     if (warp == 8) {
         // Units of 256 tokens in use, per sequence.
@@ -103,10 +94,8 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                 if (blockIdx.x == 0 && p.cache_lens != nullptr &&
                     (p.cache_lens[b] < 0 || p.cache_lens[b] > p.S))
                     atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
-                if (blockIdx.x == 0 && p.cu_q != nullptr) {
-                    const int a = p.cu_q[b], e = p.cu_q[b + 1];
-                    if (a < 0 || e < a || e > p.N || e - a > p.nq) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
-                }
+                int tok0, n_tok;
+                if (blockIdx.x == 0 && !tokens_of(b, tok0, n_tok)) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
             }
             int v = n;
 #pragma unroll

@@ -222,8 +222,10 @@ def shared_prefix_attention(
         cache_lens: ``[B]`` tokens in use, the queries' own among them (default: all).  Query j of
             a sequence's n sees its cache's tokens ``t <= len - n + j``.
         q_lens: ``[B]`` host query counts; or ``cu_q_lens`` int32 ``[B + 1]`` starts on the device
-            with ``max_q_len``.  Default: N / B each.  Rows before the first sequence and behind the
-            last are left as they were (in outputs allocated here: undefined).
+            with ``max_q_len``.  Default: N / B each.  A sequence whose device starts decrease, lie
+            outside those of the first and the last or are more than ``max_q_len`` apart has no rows
+            (reported by :func:`paged_status`).  Rows of no sequence are left as they were (in
+            outputs allocated here: undefined).
         page_table: int32 ``[B, max_pages]``.  A bad id's tokens count as masked, a bad device
             length as 0, both reported by :func:`paged_status`.
         scale: of the scores, default ``D ** -0.5``.

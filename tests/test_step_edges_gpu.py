@@ -65,3 +65,62 @@ def test_a_rejected_draft_leaves_the_accepted_tokens_weights(scb):
     assert bits_equal(cache.scores(0), before) and cache.next_position(0) == 110
     cache.attend(0, q[:, :, :1], k[:, :, :1], v[:, :, :1])
     assert bits_equal(cache.own[0][0][:, :, 20], keys[:, :, 20])
+
+
+STARTS = [  # token starts, tokens a sequence at most
+    ([0, 5, 2, 3], 3), ([0, 2, 4, 30], 4), ([2, 4, 3, 6], 3), ([-1, 2, 3, 5], 4), ([0, 3, 6, 4], 3),
+    ([0, 1, 7, 8], 3), ([4, 4, 4, 4], 2), ([6, 1, 2, 3], 3), ([0, 2, 5, -1], 3), ([1, 3, 9, 9], 9)]
+
+
+@pytest.mark.parametrize("page", [0, 16, 5])  # tensor maps twice, and copies without them
+@pytest.mark.parametrize("scale,hq", [(1, 4), (12, 8), (1, 64), (40, 8)])  # streamed, tiles, one and two row tiles
+@pytest.mark.parametrize("cap", [80, 0])
+def test_rows_of_no_sequence_are_left_alone(scb, ref, scale, hq, page, cap):
+    """Starts that decrease, leave the range of the first and the last or lie too far apart give no rows; the
+    other sequences' rows are right, whatever the plan."""
+    if cap == 0 and page:
+        pytest.skip("no pages without tokens")
+    hk, d, p = 2, 64, 70
+    n = 10 * scale
+    q, kp, vp = rand(1, n, hq, d), rand(2, p, hk, d), rand(3, p, hk, d)
+    table = None
+    if page:
+        per = cap // page
+        kc, vc = rand(4, 3 * per, page, hk, d), rand(5, 3 * per, page, hk, d)
+        table = torch.arange(3 * per, dtype=torch.int32, device=DEV).view(3, per)
+        dense = [x.view(3, cap, hk, d) for x in (kc, vc)]
+    else:
+        kc, vc = rand(4, 3, cap, hk, d), rand(5, 3, cap, hk, d)
+        dense = [kc, vc]
+    lens = [min(cap, x) for x in (80, 33, 61)]
+    for starts, most in STARTS:
+        starts, most = [x * scale for x in starts], most * scale
+        first, last = max(starts[0], 0), min(max(starts[-1], 0), n)
+        fine = [b for b in range(3)
+                if first <= starts[b] <= starts[b + 1] <= last and starts[b + 1] - starts[b] <= most]
+        scb.paged_status(DEV)
+        # a larger call before it leaves its parts in the memory that the workspace comes from
+        scb.shared_prefix_attention(q, kp, vp, kc, vc, lens, page_table=table, q_lens=[n - 2, 1, 1])
+        out = torch.full_like(q, 5.0)
+        _, lse = scb.shared_prefix_attention(q, kp, vp, kc, vc, torch.tensor(lens, dtype=torch.int32, device=DEV),
+                                             page_table=table, max_q_len=most, out=out,
+                                             cu_q_lens=torch.tensor(starts, dtype=torch.int32, device=DEV))
+        assert scb.paged_status(DEV) == (0 if len(fine) == 3 else scb._lib.SC_STATUS_BAD_SEQ_LEN)
+        claims = torch.zeros(n, dtype=torch.int32)
+        for b in fine:
+            claims[starts[b]:starts[b + 1]] += 1
+        for b in fine:
+            a, e = starts[b], starts[b + 1]
+            once = claims[a:e] == 1  # rows that two sequences claim are undefined
+            if a == e:
+                continue
+            want, wlse, absum, size = ref.attention(*(x.cpu() for x in (q[a:e], kp, vp, dense[0][b:b + 1],
+                                                                        dense[1][b:b + 1])), [lens[b]], [e - a])
+            # weights and outputs rounded to 2^-11 each, scores off by (64 + 4) 2^-23 of their products' sum
+            ds = (d + 4) * 2.0 ** -23 * size
+            tol = (2.0 ** -11 + 2 * ds + 2.0 ** -20 + 2 * (p + cap + 32) * 2.0 ** -23) * absum + 2.0 ** -11 * want.abs()
+            err = ((out[a:e].cpu().double() - want).abs() - tol)[once]
+            assert float(err.max()) <= 2.0 ** -25, (starts, b)
+            err = ((lse[a:e].cpu().double() - wlse).abs() - 2.0 ** -22 * wlse.abs())[once]
+            assert float(err.max()) <= ds + 200 * 2.0 ** -23, (starts, b)
+        assert bool((out.cpu()[claims == 0] == 5).all()), starts
