@@ -85,7 +85,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
     } else {
         part = u % p.n_cp;
         b = u / p.n_cp;
-        sequence_tokens(p, b, tok0, n_tok);
+        sequence_tokens(p, Starts(p), b, tok0, n_tok);
     }
     const int rows = n_tok * p.G;
     const int r0 = rt * MR;
@@ -422,8 +422,12 @@ __global__ void __launch_bounds__(kThreads) join_parts(const __grid_constant__ A
     const int64_t row = W == 1 ? static_cast<int64_t>(blockIdx.x) * kWarps + warp : blockIdx.x;
     const int64_t all_rows = static_cast<int64_t>(p.N) * p.Hq;
     // Rows of no sequence stay as they are: nobody has written their own caches' parts.
-    const bool counts = row < all_rows && in_sequence(p, static_cast<int>(row / p.Hq));
-    if (p.cap == 0 && blockIdx.x == 0 && warp == 0) report_sequences(p);  // no kernel before it looked at them
+    bool counts = row < all_rows;
+    if (p.cu_q != nullptr) {
+        counts = counts && in_sequence(p.cu_q, p.B, p.N, p.nq, static_cast<int>(static_cast<uint32_t>(row) / p.Hq));
+        if (p.cap == 0 && blockIdx.x == 0 && warp == 0 && p.status)  // no kernel before looked at the sequences
+            report_sequences(p.cu_q, p.B, p.N, p.nq, nullptr, 0, p.status);
+    }
     wait_for_previous();
     if (!counts) return;
     const int parts = p.n_pp + p.n_cp;

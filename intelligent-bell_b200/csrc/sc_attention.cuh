@@ -41,65 +41,67 @@ struct AttnParams {
 
 constexpr float kNegInf = -__builtin_huge_valf();
 
-// Tokens that sequences may have: those from the first start to the last one.
-__device__ __forceinline__ int used_tokens(const int32_t* cu_q, int B, int N) {
-    if (cu_q == nullptr) return N;
-    const int e = cu_q[B];
-    return e < 0 ? 0 : min(e, N);
-}
-__device__ __forceinline__ int used_tokens(const AttnParams& p) { return used_tokens(p.cu_q, p.B, p.N); }
-
-// Tokens of sequence b: its first one and how many.  A sequence whose starts decrease, leave the range of
-// the first and the last one or are more than nq apart has none (false), and its rows of the output
-// are left alone.
-__device__ __forceinline__ bool sequence_of(const int32_t* cu_q, int B, int N, int nq, int b, int& tok0, int& n) {
-    if (cu_q == nullptr) {
+// Where sequences begin in q.  A sequence whose starts decrease, leave the range of the first and the last
+// one or are more than nq apart has no tokens (`of` is false), and its rows of the output are left alone.
+struct Starts {
+    const int32_t* cu;  // [B + 1], or null: nq each
+    int first, last;    // tokens that sequences may have
+    int nq;
+    __device__ __forceinline__ Starts(const int32_t* cu_q, int B, int N, int most)
+        : cu(cu_q), first(0), last(N), nq(most) {
+        if (cu_q != nullptr) {
+            first = max(cu_q[0], 0);
+            last = max(min(cu_q[B], N), 0);
+        }
+    }
+    __device__ __forceinline__ explicit Starts(const AttnParams& p) : Starts(p.cu_q, p.B, p.N, p.nq) {}
+    __device__ __forceinline__ bool of(int b, int& tok0, int& n) const {
         tok0 = b * nq;
         n = nq;
-        return true;
+        if (cu == nullptr) return true;
+        const int a = cu[b], e = cu[b + 1];
+        const bool fine = a >= first && e >= a && e <= last && e - a <= nq;
+        tok0 = fine ? a : 0;
+        n = fine ? e - a : 0;
+        return fine;
     }
-    const int a = cu_q[b], e = cu_q[b + 1];
-    const bool fine = a >= max(cu_q[0], 0) && e >= a && e <= used_tokens(cu_q, B, N) && e - a <= nq;
-    tok0 = fine ? a : 0;
-    n = fine ? e - a : 0;
-    return fine;
-}
-__device__ __forceinline__ bool sequence_of(const AttnParams& p, int b, int& tok0, int& n) {
-    return sequence_of(p.cu_q, p.B, p.N, p.nq, b, tok0, n);
-}
-__device__ __forceinline__ void sequence_tokens(const AttnParams& p, int b, int& tok0, int& n) {
-    if (!sequence_of(p, b, tok0, n) && threadIdx.x == 0 && p.status) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
+};
+__device__ __forceinline__ int used_tokens(const AttnParams& p) { return Starts(p).last; }
+__device__ __forceinline__ void sequence_tokens(const AttnParams& p, const Starts& starts, int b, int& tok0, int& n) {
+    if (!starts.of(b, tok0, n) && threadIdx.x == 0 && p.status) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
 }
 
-// What is wrong with any sequence that device starts give, by one warp.
-__device__ __forceinline__ void report_sequences(const AttnParams& p) {
-    if (p.cu_q == nullptr || p.status == nullptr) return;
-    for (int b = threadIdx.x & 31; b < p.B; b += 32) {
+// What is wrong with any sequence that device starts give, by one warp.  (Out of line, like in_sequence:
+// few calls need it, and what lies between a kernel's instructions costs their fetches.)
+static __device__ __noinline__ void report_sequences(const int32_t* cu_q, int B, int N, int nq, const int32_t* cache_lens,
+                                                     int cap, int32_t* status) {
+    const Starts starts(cu_q, B, N, nq);
+    for (int b = threadIdx.x & 31; b < B; b += 32) {
         int tok0, n;
-        bool fine = sequence_of(p, b, tok0, n);
-        if (p.cap && p.cache_lens != nullptr) fine = fine && p.cache_lens[b] >= 0 && p.cache_lens[b] <= p.cap;
-        if (!fine) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
+        bool fine = starts.of(b, tok0, n);
+        if (cache_lens != nullptr) fine = fine && cache_lens[b] >= 0 && cache_lens[b] <= cap;
+        if (!fine) atomicOr(status, SC_STATUS_BAD_SEQ_LEN);
     }
 }
 
 // Whether a token is some sequence's, for a whole warp.  Between starts that do not decrease a search
 // finds its sequence; where that one is not fine, the others are asked in turn.
-__device__ __forceinline__ bool in_sequence(const AttnParams& p, int tok) {
-    if (p.cu_q == nullptr) return tok < p.N;
-    if (tok < p.cu_q[0] || tok >= used_tokens(p)) return false;
+static __device__ __noinline__ bool in_sequence(const int32_t* cu_q, int B, int N, int nq, int tok) {
+    const Starts starts(cu_q, B, N, nq);
+    if (tok < starts.first || tok >= starts.last) return false;
     const int lane = threadIdx.x & 31;
-    int lo = 0, hi = p.B;  // cu_q[lo] <= tok < cu_q[hi]
+    int lo = 0, hi = B;  // cu_q[lo] <= tok < cu_q[hi]
     while (hi - lo > 1) {
         const int step = (hi - lo + 31) / 32, i = lo + (lane + 1) * step;
-        const uint32_t upto = __ballot_sync(0xffffffffu, i < hi && p.cu_q[i] <= tok);
+        const uint32_t upto = __ballot_sync(0xffffffffu, i < hi && cu_q[i] <= tok);
         const int k = 32 - __clz(upto);  // the last of them, if any
         hi = min(hi, lo + (k + 1) * step);
         lo += k * step;
     }
     int tok0, n;
-    if (sequence_of(p, lo, tok0, n)) return true;
-    for (int b0 = 0; b0 < p.B; b0 += 32) {
-        const bool in = b0 + lane < p.B && sequence_of(p, b0 + lane, tok0, n) && tok >= tok0 && tok < tok0 + n;
+    if (starts.of(lo, tok0, n)) return true;
+    for (int b0 = 0; b0 < B; b0 += 32) {
+        const bool in = b0 + lane < B && starts.of(b0 + lane, tok0, n) && tok >= tok0 && tok < tok0 + n;
         if (__any_sync(0xffffffffu, in)) return true;
     }
     return false;

@@ -82,10 +82,11 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     auto q_empty = [&](int s) { return bars + 8u * (2 * NST + QB + s); };
     volatile int* gave_up = &s_gave_up;
 
+    const Starts starts(p);
     // A sequence's tokens of q and length; the kernel's first block reports what is wrong with them.
     auto sequence = [&](int b, int& tok0, int& n, int& len) {
         len = p.cap;
-        bool fine = sequence_of(p, b, tok0, n);
+        bool fine = starts.of(b, tok0, n);
         if (p.cache_lens != nullptr) {
             len = p.cache_lens[b];
             if (len < 0 || len > p.cap) {
@@ -128,7 +129,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
     __syncthreads();
 
     // This block's run of steps.
-    const int rows_p = used_tokens(p) * p.G;
+    const int rows_p = starts.last * p.G;
     const int steps_p = sp.with_prefix ? (p.P + kStep - 1) / kStep : 0;
     const int64_t prefix_steps = static_cast<int64_t>(p.Hkv) * ((rows_p + MR - 1) / MR) * steps_p;
     int64_t cache_steps = 0;  // of one head, then of all
@@ -163,7 +164,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
         x.pre = g < prefix_steps;
         if (x.pre) {
             x.b = 0;
-            x.tok0 = 0, x.n_tok = used_tokens(p), x.len = p.P;
+            x.tok0 = 0, x.n_tok = starts.last, x.len = p.P;
             x.tiles = (rows_p + MR - 1) / MR;
             x.steps = steps_p;
             const int tile = static_cast<int>(g / steps_p);

@@ -61,20 +61,20 @@ __device__ __forceinline__ uint32_t tile_chunk(int r, int c) {
 struct Round {
     int units, full, rem, parts;  // units before the last round, in it, and parts of each there
 };
-__device__ __forceinline__ int units_of(const AttnParams& p, int b) {
+__device__ __forceinline__ int units_of(const AttnParams& p, const Starts& starts, int b) {
     int tok0, n;
-    sequence_of(p, b, tok0, n);
+    starts.of(b, tok0, n);
     return (n * p.G + 2 * kRowTile - 1) / (2 * kRowTile);
 }
-__device__ __forceinline__ Round rounds(const TileParams& tp) {
+__device__ __forceinline__ Round rounds(const TileParams& tp, const Starts& starts) {
     const AttnParams& p = tp.a;
     const int lane = threadIdx.x & 31;
     int n = 0;
     if (p.cu_q == nullptr)
-        n = p.B * units_of(p, 0);
+        n = p.B * units_of(p, starts, 0);
     else
         for (int b0 = 0; b0 < p.B; b0 += 32)
-            n += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? units_of(p, b0 + lane) : 0);
+            n += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? units_of(p, starts, b0 + lane) : 0);
     Round r;
     r.units = n * p.Hkv;
     r.full = r.units / tp.sms * tp.sms;
@@ -83,16 +83,16 @@ __device__ __forceinline__ Round rounds(const TileParams& tp) {
     return r;
 }
 // Unit u as sequence, head and row tile; units of a sequence lie together.
-__device__ __forceinline__ void locate(const AttnParams& p, int u, int& b, int& h, int& rt) {
+__device__ __forceinline__ void locate(const AttnParams& p, const Starts& starts, int u, int& b, int& h, int& rt) {
     const int lane = threadIdx.x & 31;
     int in = u, own = 0;
     if (p.cu_q == nullptr) {
-        own = units_of(p, 0);
+        own = units_of(p, starts, 0);
         b = u / (own * p.Hkv);
         in = u - b * own * p.Hkv;
     } else {
         for (int b0 = 0;; b0 += 32) {
-            const int n = b0 + lane < p.B ? units_of(p, b0 + lane) : 0;
+            const int n = b0 + lane < p.B ? units_of(p, starts, b0 + lane) : 0;
             int upto = n;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -158,8 +158,10 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
     let_next_start();
     if (tp.per_seq) {
         // Sequences of no rows have no block that would report what is wrong with them.
-        if (blockIdx.x == 0 && warp == 10) report_sequences(p);
-        const Round r = rounds(tp);
+        if (blockIdx.x == 0 && warp == 10 && p.cu_q != nullptr && p.status)
+            report_sequences(p.cu_q, p.B, p.N, p.nq, p.cap ? p.cache_lens : nullptr, p.cap, p.status);
+        const Starts starts(p);
+        const Round r = rounds(tp, starts);
         int u = blockIdx.x;
         splits = 1;
         if (u >= r.full) {
@@ -172,8 +174,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
             split = slot % splits;
             u = r.full + slot / splits;
         }
-        locate(p, u, b, h, rt);
-        sequence_tokens(p, b, tok0, n_tok);
+        locate(p, starts, u, b, h, rt);
+        sequence_tokens(p, starts, b, tok0, n_tok);
         len = p.cap ? cache_length(p, b) : 0;
     } else {
         int u = blockIdx.x;
@@ -758,7 +760,8 @@ constexpr int kTailLoads = 8;
 template <typename T>
 __global__ void __launch_bounds__(128) join_tail(const __grid_constant__ TileParams tp) {
     const AttnParams& p = tp.a;
-    const Round rd = rounds(tp);
+    const Starts starts(p);
+    const Round rd = rounds(tp, starts);
     constexpr int kGroups = 2 * kRowTile / kTailRows;  // of a unit's rows
     const int lane = threadIdx.x & 31;
     wait_for_previous();
@@ -766,8 +769,8 @@ __global__ void __launch_bounds__(128) join_tail(const __grid_constant__ TilePar
     for (int g = blockIdx.x; g < rd.rem * kGroups; g += gridDim.x) {
         const int unit = g / kGroups, first = (g - unit * kGroups) * kTailRows;
         int b, h, rt, tok0, n_tok;
-        locate(p, rd.full + unit, b, h, rt);
-        sequence_tokens(p, b, tok0, n_tok);
+        locate(p, starts, rd.full + unit, b, h, rt);
+        sequence_tokens(p, starts, b, tok0, n_tok);
         for (int r = first + (threadIdx.x >> 5); r < first + kTailRows; r += 4) {
             const int row = rt * 2 * kRowTile + r;
             if (row >= n_tok * p.G) break;

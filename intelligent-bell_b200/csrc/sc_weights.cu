@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kWThreads) add_weights(const __grid_constant__
     const int h = u % p.Hkv, b = u / p.Hkv;
 
     int tok0, n_tok;
-    if (!sequence_of(p.cu_q, p.B, p.N, p.nq, b, tok0, n_tok) && threadIdx.x == 0)
+    if (!Starts(p.cu_q, p.B, p.N, p.nq).of(b, tok0, n_tok) && threadIdx.x == 0)
         atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
     int len = p.S;
     if (p.cache_lens != nullptr) {

@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
         const int len = p.cache_lens[b];
         return len < 0 || len > p.S ? 0 : len;
     };
-    auto tokens_of = [&](int b, int& tok0, int& n) { return sequence_of(p.cu_q, p.B, p.N, p.nq, b, tok0, n); };
+    const Starts starts(p.cu_q, p.B, p.N, p.nq);
+    auto tokens_of = [&](int b, int& tok0, int& n) { return starts.of(b, tok0, n); };
 
     if (warp == 8) {
         // Units of 256 tokens in use, per sequence.
@@ -94,8 +95,8 @@ __global__ void __launch_bounds__(kThreadsW, 1) weigh_tiles(const __grid_constan
                 if (blockIdx.x == 0 && p.cache_lens != nullptr &&
                     (p.cache_lens[b] < 0 || p.cache_lens[b] > p.S))
                     atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
-                int tok0, n_tok;
-                if (blockIdx.x == 0 && !tokens_of(b, tok0, n_tok)) atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
+                if (int tok0, n_tok; blockIdx.x == 0 && !tokens_of(b, tok0, n_tok))
+                    atomicOr(p.status, SC_STATUS_BAD_SEQ_LEN);
             }
             int v = n;
 #pragma unroll

@@ -129,17 +129,13 @@ def _extent(t: torch.Tensor) -> tuple[int, int]:
     return lo, lo + (last + 1) * t.element_size()
 
 
-def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two tensors are known to share no byte.
+def _side_by_side(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors whose extents meet share no byte all the same.
 
-    Their extents do not meet, or their elements lie in different parts of some period: modulo a stride
-    of theirs, of which every longer stride is a multiple, each covers one run of bytes (keys and values,
-    or the heads of q and k, side by side in one buffer).
+    Their elements lie in different parts of some period: modulo a stride of theirs, of which every
+    longer stride is a multiple, each covers one run of bytes (keys and values, or the heads of q and
+    k, side by side in one buffer).
     """
-    alo, ahi = _extent(a)
-    blo, bhi = _extent(b)
-    if alo >= bhi or blo >= ahi:
-        return True
     steps = [[s * t.element_size() for n, s in zip(t.shape, t.stride()) if n > 1] for t in (a, b)]
     sizes = [[n for n in t.shape if n > 1] for t in (a, b)]
     for period in {s for x in steps for s in x if s > 0}:
@@ -150,7 +146,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
                 if s % period:
                     run += (n - 1) * s if s < period else period
             runs.append(run)
-        off = (blo - alo) % period
+        off = (b.data_ptr() - a.data_ptr()) % period
         if runs[0] <= off and off + runs[1] <= period:
             return True
     return False
@@ -162,8 +158,12 @@ def require_apart(name: str, out: torch.Tensor, *others: torch.Tensor | None) ->
         for n, s in zip(out.shape, out.stride()):
             if s == 0 and n > 1:
                 raise ValueError(f"{name} must not be an expanded tensor (strides {tuple(out.stride())})")
+    lo, hi = _extent(out)
     for t in others:
-        if t is not None and t.device == out.device and not _apart(out, t):
+        if t is None:
+            continue
+        a, b = _extent(t)
+        if lo < b and a < hi and t.device == out.device and not _side_by_side(out, t):
             raise ValueError(f"{name} must not overlap an input or another output")
 
 
