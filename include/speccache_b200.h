@@ -92,6 +92,12 @@ SC_API int32_t sc_abi_version(void);
 SC_API int32_t sc_preload_kernels(void);
 
 /*
+ * The current device's own status word (zero when the library is loaded), for callers that keep none.
+ * Nothing is allocated, cleared or enqueued, so a call may be part of a stream capture.
+ */
+SC_API int32_t sc_status_word(int32_t** word);
+
+/*
  * cos/sin tables for relative RoPE shifts.
  * Replaces compute_rope_cos_sin_delta (speccache/kernels/reference.py:122-165).
  *

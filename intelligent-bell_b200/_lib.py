@@ -55,6 +55,7 @@ _SIGNATURES = {
     "sc_last_error": (ctypes.c_char_p, []),
     "sc_abi_version": (_i32, []),
     "sc_preload_kernels": (_i32, []),
+    "sc_status_word": (_i32, [_vp]),
     "sc_rope_cos_sin_delta": (_i32, [_vp, _i64, _i32, _f64, _vp, _vp, _vp, _i32, _vp]),
     "sc_dequant_rope_kv": (_i32, [_i32, _i64, _i32, _i32,
                                   _vp, _vp, _vp, _vp,   # k_quant, kq_strides, k_scale, ks_strides

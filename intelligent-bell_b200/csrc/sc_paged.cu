@@ -485,6 +485,26 @@ int32_t launch_scatter_pieces(const void* src, int64_t src_pitch, void* dst, int
 
 }  // namespace sc
 
+namespace sc {
+namespace {
+__device__ int32_t status_word;  // zero when the module is loaded
+}
+}  // namespace sc
+
+extern "C" int32_t sc_status_word(int32_t** word) {
+    if (!word) return sc::set_error(SC_ERR_INVALID_ARGUMENT, "null pointer argument");
+    // Loading the module is no part of a graph that this thread may be capturing.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return sc::cuda_error(e, "the status word");
+    void* at = nullptr;
+    e = cudaGetSymbolAddress(&at, sc::status_word);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) return sc::cuda_error(e, "the status word");
+    *word = static_cast<int32_t*>(at);
+    return sc::ok();
+}
+
 extern "C" int32_t sc_restore_paged(int32_t n_requests, int32_t max_pages, int32_t page_size,
                                     int32_t n_heads, int32_t head_dim, int64_t n_pool_pages,
                                     const int8_t* pool_kq, const void* pool_ks,

@@ -13,6 +13,8 @@ reported through a per-device status word, read with :func:`paged_status`.
 
 from __future__ import annotations
 
+import ctypes
+
 import torch
 
 from .. import _lib
@@ -22,11 +24,23 @@ from .validation import require_cuda
 _STATUS: dict[int, torch.Tensor] = {}
 
 
+class _Word:
+    """An int32 in device memory, for torch to view."""
+
+    def __init__(self, address: int) -> None:
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (address, False), "version": 3}
+
+
 def _status_word(device: torch.device) -> torch.Tensor:
+    """The device's status word: the library's own, since the first call may be inside a capture, whose
+    replays would clear a tensor that torch makes there."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
     w = _STATUS.get(idx)
     if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+        dev, at = torch.device("cuda", idx), ctypes.c_void_p()
+        with _lib.on_device(dev):
+            _lib.check(_lib.load().sc_status_word(ctypes.byref(at)), "sc_status_word")
+            w = torch.as_tensor(_Word(at.value), device=dev)
         _STATUS[idx] = w
     return w
 

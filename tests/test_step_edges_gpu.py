@@ -124,3 +124,36 @@ def test_rows_of_no_sequence_are_left_alone(scb, ref, scale, hq, page, cap):
             err = ((lse[a:e].cpu().double() - wlse).abs() - 2.0 ** -22 * wlse.abs())[once]
             assert float(err.max()) <= ds + 200 * 2.0 ** -23, (starts, b)
         assert bool((out.cpu()[claims == 0] == 5).all()), starts
+
+
+def test_a_status_word_made_inside_a_capture_keeps_its_bits(scb):
+    """The first call on a device may be a captured one: a replay reports and does not clear."""
+    import importlib
+
+    paged = importlib.import_module(scb.__name__ + ".kernels.paged")
+    q, k, v = rand(1, 3, 4, 64), rand(2, 3, 20, 2, 64), rand(3, 3, 20, 2, 64)
+    lens = torch.tensor([5, 20, 9], dtype=torch.int32, device=DEV)
+    scb.shared_prefix_attention(q, None, None, k, v, lens)
+    torch.cuda.synchronize()
+    kept = paged._STATUS.pop(DEV.index)
+    try:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            scb.shared_prefix_attention(q, None, None, k, v, lens)
+        graph.replay()
+        assert scb.paged_status(DEV, reset=False) == 0
+        lens[1] = 21
+        graph.replay()
+        lens[1] = 20
+        graph.replay()
+        assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_SEQ_LEN
+        graph.replay()
+        assert scb.paged_status(DEV) == 0
+        del graph
+        torch.cuda.empty_cache()
+        lens[1] = -1
+        scb.shared_prefix_attention(q, None, None, k, v, lens)
+        assert scb.paged_status(DEV) == scb._lib.SC_STATUS_BAD_SEQ_LEN
+    finally:
+        torch.cuda.synchronize()
+        paged._STATUS[DEV.index] = kept
