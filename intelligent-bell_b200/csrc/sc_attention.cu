@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
                     }
                 }
             }
-            const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+            const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>, mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
 #pragma unroll
             for (int n = 0; n < TK / 8; ++n)
 #pragma unroll
@@ -316,24 +316,16 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
                 take_out_odd<T>(vt + chunk_at<DP>(c / CPR, c % CPR), tt + c / CPR, s_odd + c % CPR * 8, DP, &s_any_odd);
             __syncwarp();
         }
-        // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
-        // rounding error goes in as a second product, since this kernel waits for memory and
-        // the products are free.
+        // o += P V, the weights in two pieces: this kernel waits for memory and the products are free.
 #pragma unroll
         for (int kk = 0; kk < TK / 16; ++kk) {
             uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = s[mt][2 * kk + (e >> 1)][2 * (e & 1)];
-                    const float y = s[mt][2 * kk + (e >> 1)][2 * (e & 1) + 1];
-                    hi[mt][e] = pack2<T>(x, y);
-                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                        const float2 r = unpack2<T>(hi[mt][e]);
-                        lo[mt][e] = pack2<T>(x - r.x, y - r.y);
-                    }
-                }
+                for (int e = 0; e < 4; ++e)
+                    two_pieces<T>(s[mt][2 * kk + (e >> 1)][2 * (e & 1)], s[mt][2 * kk + (e >> 1)][2 * (e & 1) + 1],
+                                  hi[mt][e], lo[mt][e]);
 #pragma unroll
             for (int n = 0; n < DP / 16; ++n) {
                 uint32_t vb[4];
@@ -343,10 +335,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
                 for (int mt = 0; mt < MT; ++mt) {
                     mma16816<T>(o[mt][2 * n], hi[mt], vb[0], vb[1]);
                     mma16816<T>(o[mt][2 * n + 1], hi[mt], vb[2], vb[3]);
-                    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                        mma16816<T>(o[mt][2 * n], lo[mt], vb[0], vb[1]);
-                        mma16816<T>(o[mt][2 * n + 1], lo[mt], vb[2], vb[3]);
-                    }
+                    mma16816<T>(o[mt][2 * n], lo[mt], vb[0], vb[1]);
+                    mma16816<T>(o[mt][2 * n + 1], lo[mt], vb[2], vb[3]);
                 }
             }
         }
@@ -375,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             float all = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_m[w][r]);
-            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - all);
+            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - all) * kOnePiece;
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n)
                 *reinterpret_cast<float2*>(s_o + (warp * MR + r) * DP + n * 8 + (lane & 3) * 2) =
@@ -406,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - all));
         const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
         const int64_t at = part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
-        p.part_ml[at] = make_float2(all, sum);
+        p.part_ml[at] = make_float2(all - kLift<T>, sum);
         if (odd) add_odd(p.part_o + at * p.D, p.D, s_odd, DP, min(t1, see + j + 1));
     }
 }

@@ -191,6 +191,30 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
     return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
+// ---- weights as 16-bit pieces ----
+// Where memory bounds a kernel, a weight x >= 0 goes into its product with V as hi + lo, 2^-16 (bfloat16)
+// or 2^-20 (float16) of x off.  hi is x rounded down and lo the rest plus 2^-12 x, so that lo is above
+// zero wherever x is: an infinite value times either piece is that infinity, and their sum too (with a lo
+// of zero or below it would be NaN).  Sums are 1 + 2^-12 too large, which kOnePiece takes back.
+constexpr float kOnePiece = 1.f / (1.f + 0x1p-12f);
+// float16 begins at 2^-24, so its weights are lifted: 2^15 for the largest, whose sums and maxima (15
+// lower) stay float32.
+template <typename T>
+constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
+template <typename T>
+__device__ __forceinline__ void two_pieces(float x, float y, uint32_t& hi, uint32_t& lo) {
+    float2 r;
+    if constexpr (std::is_same<T, __half>::value) {
+        asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(y), "f"(x));
+        r = unpack2<T>(hi);
+    } else {
+        const uint32_t a = __float_as_uint(x), b = __float_as_uint(y);
+        hi = __byte_perm(a, b, 0x7632);
+        r = make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u));
+    }
+    lo = pack2<T>(fmaf(x, 1.f + 0x1p-12f, -r.x), fmaf(y, 1.f + 0x1p-12f, -r.y));
+}
+
 // The tensor-core kernel (sc_attention_tile.cu), over the prefix for all rows together in `splits`
 // parts, or (per_seq) over the prefix and then each sequence's own cache for the sequence's rows,
 // output included: rounds of `sms` units, the last one's split into up to `splits` parts.

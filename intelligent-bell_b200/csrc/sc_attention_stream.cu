@@ -421,23 +421,21 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                             }
                         }
                     }
-                    const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+                    const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>,
+                                           mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[0][e] = exp2_fast(s[0][e] - base[e & 1]);
                         l[0][e & 1] += s[0][e];
                     }
-                    // O^T += V^T P^T: the weights turned within the warp; for bfloat16 their rounding error
-                    // as a second product.
+                    // O^T += V^T P^T: the weights' two pieces, turned within the warp
                     uint32_t hi[2], lo[2];
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
-                        const uint32_t w = pack2<T>(s[0][2 * e], s[0][2 * e + 1]);
+                        uint32_t w, r;
+                        two_pieces<T>(s[0][2 * e], s[0][2 * e + 1], w, r);
                         hi[e] = turn8x8(w);
-                        if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                            const float2 r = unpack2<T>(w);
-                            lo[e] = turn8x8(pack2<T>(s[0][2 * e] - r.x, s[0][2 * e + 1] - r.y));
-                        }
+                        lo[e] = turn8x8(r);
                     }
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
@@ -445,7 +443,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                         ldmatrix4_t(a, vt + kv_chunk<DP>(warp * 16 + (lane & 7) + ((lane >> 4) << 3),
                                                          k * 2 + ((lane >> 3) & 1)));
                         mma16816<T>(o[0][k], a, hi[0], hi[1]);
-                        if constexpr (std::is_same<T, __nv_bfloat16>::value) mma16816<T>(o[0][k], a, lo[0], lo[1]);
+                        mma16816<T>(o[0][k], a, lo[0], lo[1]);
                     }
                 } else {
                     float s[MT][2][4];
@@ -508,7 +506,8 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                                 }
                             }
                         }
-                        const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0], mx[1] == kNegInf ? 0.f : mx[1]};
+                        const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>,
+                                               mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -518,20 +517,14 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                                 l[mt][e >> 1] += w;
                             }
                     }
-                    // o += P V.  The weights go in as 16 bits; for bfloat16 (8 significant bits) their
-                    // rounding error goes in as a second product: the copies, not the products, bound this.
+                    // o += P V, the weights in two pieces: the copies, not the products, bound this.
                     uint32_t hi[MT][4], lo[MT][4];
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const float a = s[mt][e >> 1][2 * (e & 1)], b = s[mt][e >> 1][2 * (e & 1) + 1];
-                            hi[mt][e] = pack2<T>(a, b);
-                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                                const float2 r = unpack2<T>(hi[mt][e]);
-                                lo[mt][e] = pack2<T>(a - r.x, b - r.y);
-                            }
-                        }
+                        for (int e = 0; e < 4; ++e)
+                            two_pieces<T>(s[mt][e >> 1][2 * (e & 1)], s[mt][e >> 1][2 * (e & 1) + 1], hi[mt][e],
+                                          lo[mt][e]);
 #pragma unroll
                     for (int k = 0; k < DP / 16; ++k) {
                         uint32_t vb[4];
@@ -541,10 +534,8 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                         for (int mt = 0; mt < MT; ++mt) {
                             mma16816<T>(o[mt][2 * k], hi[mt], vb[0], vb[1]);
                             mma16816<T>(o[mt][2 * k + 1], hi[mt], vb[2], vb[3]);
-                            if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-                                mma16816<T>(o[mt][2 * k], lo[mt], vb[0], vb[1]);
-                                mma16816<T>(o[mt][2 * k + 1], lo[mt], vb[2], vb[3]);
-                            }
+                            mma16816<T>(o[mt][2 * k], lo[mt], vb[0], vb[1]);
+                            mma16816<T>(o[mt][2 * k + 1], lo[mt], vb[2], vb[3]);
                         }
                     }
                 }
@@ -588,7 +579,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                 float top = s_m[0][r];
 #pragma unroll
                 for (int w = 1; w < kSWarps; ++w) top = fmaxf(top, s_m[w][r]);
-                const float f = m[0][e] == kNegInf ? 0.f : exp2_fast(m[0][e] - top);
+                const float f = m[0][e] == kNegInf ? 0.f : exp2_fast(m[0][e] - top) * kOnePiece;
 #pragma unroll
                 for (int k = 0; k < OK; ++k) {
                     o[0][k][e] *= f;
@@ -637,7 +628,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             float top = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kSWarps; ++w) top = fmaxf(top, s_m[w][r]);
-            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - top);
+            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - top) * kOnePiece;
 #pragma unroll
             for (int k = 0; k < DP / 8; ++k) {
                 o[mt][k][2 * e] *= f;
@@ -688,7 +679,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                 sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - top));
             const int jq = static_cast<int>(fdiv(r0 + r, p.div_G));
             const int64_t row = static_cast<int64_t>(x.tok0 + jq) * p.Hq + x.h * p.G + r0 + r - jq * p.G;
-            p.part_ml[part * all_rows + row] = make_float2(top, sum);
+            p.part_ml[part * all_rows + row] = make_float2(top - kLift<T>, sum);
             if (odd) add_odd(p.part_o + (part * all_rows + row) * p.D, p.D, s_odd, DP, min(x.len, see + jq + 1));
             if (last)  // parts that this row tile does not have
                 for (int k = part + 1; k < parts_end; ++k) p.part_ml[k * all_rows + row] = make_float2(kNegInf, 0.f);

@@ -157,3 +157,60 @@ def test_a_status_word_made_inside_a_capture_keeps_its_bits(scb):
     finally:
         torch.cuda.synchronize()
         paged._STATUS[DEV.index] = kept
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hk,d,page", [
+    (1, 8, 2, 128, 0), (1, 8, 2, 64, 16), (3, 8, 2, 64, 0), (3, 8, 1, 256, 0), (9, 8, 2, 128, 0),  # streamed
+    (2, 8, 2, 64, 5), (9, 8, 2, 64, 5),                        # copies without tensor maps
+    (1, 64, 2, 128, 0), (30, 8, 2, 64, 0), (70, 8, 2, 128, 16)])  # tiles
+def test_infinite_values_that_every_row_sees(scb, ref, dtype, n, hq, hk, d, page):
+    """The sum is that infinity (both signs: not a number), wherever the token lies and whichever kernel
+    takes it."""
+    b, p, cap = 3, 300, 240
+    q, kp, vp = rand(1, b * n, hq, d, dtype=dtype), rand(2, p, hk, d, dtype=dtype), rand(3, p, hk, d, dtype=dtype)
+    table = None
+    if page:
+        kc, vc = (rand(i, b * cap // page, page, hk, d, dtype=dtype) for i in (4, 5))
+        table = torch.arange(b * cap // page, dtype=torch.int32, device=DEV).view(b, -1)
+    else:
+        kc, vc = (rand(i, b, cap, hk, d, dtype=dtype) for i in (4, 5))
+    lens = [240, 77, 200]
+    flat = vc.view(b, cap, hk, d)
+    for t, column, value in ((0, 0, "inf"), (17, 1, "-inf"), (130, 2, "inf"), (299, 3, "inf"), (64, 4, "inf"),
+                             (200, 4, "-inf"), (255, 5, "-inf"), (5, 6, "inf")):
+        vp[t, :, column] = float(value)
+    for t, column, value in ((0, 8, "inf"), (3, 9, "-inf"), (2, 10, "inf"), (5, 10, "-inf"), (4, 6, "inf")):
+        flat[:, t, :, column] = float(value)
+    out, _ = scb.shared_prefix_attention(q, kp, vp, kc, vc, lens, page_table=table)
+    want, _, _, _ = ref.attention(*(x.cpu() for x in (q, kp, vp, kc, vc)), lens, [n] * b,
+                                  page_table=None if table is None else table.cpu())
+    got = out.cpu().double()
+    odd = ~torch.isfinite(want)
+    assert int(odd.sum()) >= 10 * b * n * hq and bool((torch.isfinite(got) == ~odd).all())
+    same = (got == want) | (torch.isnan(got) & torch.isnan(want))
+    assert bool(same[odd].all()), f"{int((odd & ~same).sum())} of {int(odd.sum())}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hk,d,page", [(1, 8, 2, 128, 0), (1, 4, 2, 64, 16), (3, 8, 1, 256, 0), (9, 4, 2, 64, 0),
+                                            (3, 8, 2, 128, 5)])
+def test_weights_keep_more_bits_than_the_type(scb, ref, dtype, n, hq, hk, d, page):
+    """Streamed weights go into the product in two pieces: 2^-16 off instead of half a step of the type.
+    Outputs are rounded once; scores are off by (d + 4) 2^-23 of their products' sum."""
+    b, p, cap = 2, 60 if n > 1 else 30, 160  # fewer than 64 rows of a KV head: no tiles
+    q, kp, vp = rand(1, b * n, hq, d, dtype=dtype), rand(2, p, hk, d, dtype=dtype), rand(3, p, hk, d, dtype=dtype)
+    table = None
+    if page:
+        kc, vc = (rand(i, b * cap // page, page, hk, d, dtype=dtype) for i in (4, 5))
+        table = torch.arange(b * cap // page, dtype=torch.int32, device=DEV).view(b, -1)
+    else:
+        kc, vc = (rand(i, b, cap, hk, d, dtype=dtype) for i in (4, 5))
+    out, _ = scb.shared_prefix_attention(q, kp, vp, kc, vc, page_table=table)
+    want, _, absum, size = ref.attention(*(x.cpu() for x in (q, kp, vp, kc, vc)), [cap] * b, [n] * b,
+                                         page_table=None if table is None else table.cpu())
+    ds = (d + 4) * 2.0 ** -23 * size
+    tol = (2.0 ** -16 + 2 * ds + 2.0 ** -20 + 2 * (p + cap + 32) * 2.0 ** -23) * absum
+    tol += torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -26
+    err = (out.cpu().double() - want).abs()
+    assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()}"
