@@ -7,8 +7,9 @@
 //   P = 2^(s - m)     one thread a row: no shuffles; written over S as 16 bits,
 //   O += P V          A operand from tensor memory, fp32 accumulators in tensor memory.
 // Two row tiles take turns: while the tensor cores work on one, eight warps turn the other's
-// scores into weights.  (With one row tile, two token tiles' scores do.)  The running maximum that scales O is only raised when a score passes it
-// by 2^8, so O is rarely rescaled (weights up to 2^8 and their fp32 sums lose nothing).
+// scores into weights.  (With one row tile, two token tiles' scores do.)  The running maximum that scales
+// O is only raised when a score passes it by 2^8 (float16: 2^6), so O is rarely rescaled; weights above
+// one and their fp32 sums lose nothing.
 //
 // Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies, warp 11 issues
 // the products.  Tiles come by TMA (4-D tensor maps of prefix, caches or page pool; a page's piece
@@ -30,7 +31,14 @@ constexpr int kTThreads = 384;
 constexpr int kLoadWarps = 3;
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
-constexpr float kRaise = 8.f;  // log2: how far a score may pass the maximum in use
+// log2: how far a score may pass the maximum in use, and by how much weights are lifted.  float16 ends at
+// 2^16 and begins at 2^-24, so that lifted its weights count down to 2^-34 of the largest (as they are,
+// 2^17 tokens 2^25 below the largest would be lost: 2^-8 of the sum); bfloat16 has room on both sides.
+// 24 sequences of float16 behind 32,768: 47.3 us, 2^4 and 2^11 49.2 (O is rescaled more often), 2^8 and 2^7 47.1.
+template <typename T>
+constexpr float kRaise = std::is_same<T, __half>::value ? 6.f : 8.f;
+template <typename T>
+constexpr float kLiftTile = std::is_same<T, __half>::value ? 9.f : 0.f;
 
 template <int DP>
 struct TileShape {
@@ -560,9 +568,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     const int seen = (pre ? p.P : own_limit) - t0;  // columns below it count
                     const bool bad = !pre && *reinterpret_cast<volatile int*>(&s_any_bad) != 0;
                     const bool masked = __any_sync(0xffffffffu, seen < kTokTile) || bad;
-                    // A score above the maximum in use by 2^8 raises it, and O with it.
+                    // A score above the maximum in use by kRaise raises it, and O with it.
                     auto raised = [&](float top) {
-                        const bool raise = top > m + kRaise || (m == kNegInf && top > m);
+                        const bool raise = top > m + kRaise<T> || (m == kNegInf && top > m);
                         if (!__any_sync(0xffffffffu, raise)) return;
                         const float f = raise ? exp2_fast(m - top) : 1.f;
                         if (raise) m = top;
@@ -594,7 +602,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             t4[(e >> 1) & 3] = max3(t4[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
                         raised(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2);
                         if (!alive) break;
-                        const float base = m == kNegInf ? 0.f : m;
+                        const float base = m == kNegInf ? 0.f : m - kLiftTile<T>;
                         const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
                         float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
@@ -647,7 +655,7 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         }
                         raised(top * mul);
                         if (!alive) break;
-                        const float base = m == kNegInf ? 0.f : m;
+                        const float base = m == kNegInf ? 0.f : m - kLiftTile<T>;
 #pragma unroll 1
                         for (int c = 0; c < kTokTile; c += 16) {
                             uint32_t x[16], w[8];
@@ -684,9 +692,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 if (*reinterpret_cast<volatile int*>(&s_any_odd)) add_odd_tmem<DP>(o_at, s_odd, own_limit);
                 if (mine) {
                     if (!direct)
-                        p.part_ml[part_at(r)] = make_float2(m, l);
+                        p.part_ml[part_at(r)] = make_float2(m - kLiftTile<T>, l);
                     else if (p.lse)
-                        p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l)) * 0.6931471805599453f;
+                        p.lse[at] = l == 0.f ? kNegInf : (m - kLiftTile<T> + log2f(l)) * 0.6931471805599453f;
                 }
                 // 128 bytes of each of the warp's 32 rows at a time, turned in shared memory (where the
                 // warp's queries were) so that a store covers whole lines: a lane's 16 bytes in 32 rows

@@ -3,6 +3,8 @@ capture, values that are not finite and weights far below a row's largest."""
 
 from __future__ import annotations
 
+import math
+
 import pytest
 import torch
 
@@ -214,3 +216,35 @@ def test_weights_keep_more_bits_than_the_type(scb, ref, dtype, n, hq, hk, d, pag
     tol += torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -26
     err = (out.cpu().double() - want).abs()
     assert bool((err <= tol).all()), f"{int((err > tol).sum())} of {err.numel()}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hk", [(1, 8, 2), (2, 16, 2), (1, 256, 2), (40, 8, 2), (100, 8, 2)])  # streams, tiles
+@pytest.mark.parametrize("nats", [12.0, 17.0, 19.0])
+@pytest.mark.parametrize("first", [True, False])
+def test_many_weights_far_below_the_largest(scb, dtype, n, hq, hk, nats, first):
+    """One token takes nearly all of the weight and 6,000 others e^-nats of it each: what they add, in a column
+    that is zero for the first, keeps its bits."""
+    b, p, cap, d = 2, 6000, n + 3, 64
+    q = torch.zeros((b * n, hq, d), dtype=dtype, device=DEV)
+    q[..., 0] = nats
+    kp = torch.zeros((p, hk, d), dtype=dtype, device=DEV)
+    vp = torch.ones_like(kp)
+    at = 0 if first else p - 1
+    kp[at, :, 0] = 1.0
+    vp[at, :, :32] = 0.0
+    kc = torch.zeros((b, cap, hk, d), dtype=dtype, device=DEV)
+    kc[..., 0] = -20.0  # own tokens: e^(-21 nats) and less, nothing
+    out, lse = scb.shared_prefix_attention(q, kp, vp, kc, kc, scale=1.0)
+    w = math.exp(-nats)
+    rest, total = (p - 1) * w, 1 + (p - 1) * w
+    want = torch.full((d,), 1.0, dtype=torch.float64)
+    want[:32] = rest / total
+    # A weight is off by half a step of the type (float16: or 2^-34, its lifted end) and the output once more,
+    # which float16 holds in steps of 2^-24 below 2^-14; the exponentials and sums by 2^-21 + p 2^-23.
+    u = torch.finfo(dtype).eps / 2
+    tol = (2 * u + 2.0 ** -21 + p * 2.0 ** -23) * want + 2.0 ** -25
+    tol += p * 2.0 ** -34 if dtype == torch.float16 else 0.0
+    err = (out.cpu().double() - want).abs().amax((0, 1))
+    assert bool((err <= tol).all()), f"{err[0].item():.3g} of {rest:.3g} (most {tol[0].item():.3g})"
+    assert float((lse.cpu().double() - nats - math.log(total)).abs().max()) <= 2.0 ** -20 * nats + p * 2.0 ** -23
