@@ -9,6 +9,7 @@ working.  One additive extension: ``out`` may be bfloat16 as well as float16.
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 OUT_DTYPES = (torch.float16, torch.bfloat16)
 
@@ -116,6 +117,10 @@ def require_no_grad(what: str, *tensors: torch.Tensor | None) -> None:
             if t is not None and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad() "
                                    "or on detached tensors")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # inside a forward-mode level
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{what} has no forward-mode derivative: call it on tensors without tangents")
 
 
 def _extent(t: torch.Tensor) -> tuple[int, int]:
