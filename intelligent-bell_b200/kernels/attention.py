@@ -16,7 +16,7 @@ import torch
 
 from .. import _lib
 from .paged import _status_word
-from .staging import Plans, step_arguments
+from .staging import Plans, integers, step_arguments
 from .validation import require_apart, require_cuda, require_no_grad, same_view
 
 _DTYPES = (torch.float16, torch.bfloat16)
@@ -96,7 +96,7 @@ def _sequence_starts(n: int, batch: int, q_lens, cu_q_lens, max_q_len):
         cu = [0]
         for x in lens:
             cu.append(cu[-1] + x)
-        return torch.tensor(cu, dtype=torch.int32), max(lens)
+        return torch.tensor(cu, dtype=torch.int32), max(lens, default=0)
     if cu_q_lens is not None:
         if not isinstance(cu_q_lens, torch.Tensor) or cu_q_lens.dtype != torch.int32 or \
                 cu_q_lens.shape != (batch + 1,):
@@ -106,6 +106,8 @@ def _sequence_starts(n: int, batch: int, q_lens, cu_q_lens, max_q_len):
         if not 0 <= int(max_q_len) <= n:
             raise ValueError(f"max_q_len must lie in [0, {n}], got {max_q_len}")
         return cu_q_lens.contiguous(), int(max_q_len)
+    if n == 0 and batch == 0:
+        return None, 0
     if batch == 0 or n % batch:
         raise ValueError(f"{n} tokens are not the same number for each of {batch} sequences; give q_lens")
     return None, n // batch
@@ -116,8 +118,7 @@ def _lengths(name: str, lens, batch: int, most: int):
     if lens is None or (isinstance(lens, torch.Tensor) and lens.is_cuda and lens.dtype == torch.int32 and
                         lens.shape == (batch,) and lens.stride(0) == 1):
         return lens
-    if not isinstance(lens, torch.Tensor):
-        lens = torch.as_tensor(lens)
+    lens = integers(lens)
     if lens.dtype not in (torch.int32, torch.int64):
         raise TypeError(f"{name} must be integers, got {lens.dtype}")
     if lens.shape != (batch,):
@@ -250,7 +251,9 @@ def shared_prefix_attention(
     batch, cap, page, n_pages, table, lens = 0, 0, 1, 0, None, None
     if k_cache is not None:
         if page_table is not None:
-            table = page_table if isinstance(page_table, torch.Tensor) else torch.as_tensor(page_table)
+            table = integers(page_table)
+            if table.dtype not in (torch.int32, torch.int64):
+                raise TypeError(f"page_table must be integers, got {table.dtype}")
             if table.ndim != 2:
                 raise ValueError(f"page_table must be [B, max_pages], got {tuple(table.shape)}")
             if table.dtype != torch.int32:

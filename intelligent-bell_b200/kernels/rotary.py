@@ -18,7 +18,7 @@ import torch
 
 from .. import _lib
 from .restore import DEFAULT_THETA
-from .staging import Plans, step_arguments
+from .staging import Plans, integers, step_arguments
 from .validation import require_apart, require_cuda, require_no_grad, same_view
 
 _DTYPES = (torch.float16, torch.bfloat16, torch.float32)
@@ -232,8 +232,7 @@ def apply_rotary(
     if isinstance(positions, int):
         start = positions
     else:
-        if not isinstance(positions, torch.Tensor):
-            positions = torch.as_tensor(positions)
+        positions = integers(positions)
         if positions.dtype not in (torch.int32, torch.int64):
             raise TypeError(f"positions must be int32 or int64, got {positions.dtype}")
         if positions.shape != (t,) and positions.shape != (b, t):

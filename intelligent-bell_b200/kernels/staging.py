@@ -26,6 +26,14 @@ def host_array(x, dtype: torch.dtype) -> torch.Tensor:
     return t.contiguous()
 
 
+def integers(x) -> torch.Tensor:
+    """A tensor, or host numbers as one; of none at all torch would make floats."""
+    if isinstance(x, torch.Tensor):
+        return x
+    t = torch.as_tensor(x)
+    return t if t.numel() else t.to(torch.int32)
+
+
 def to_device(tensors: list[torch.Tensor], device: torch.device) -> list[torch.Tensor]:
     """Device versions of ``tensors`` (contiguous, already of their final dtype).
 
