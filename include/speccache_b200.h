@@ -358,8 +358,9 @@ SC_API int32_t sc_pipeline_destroy(sc_pipeline* p);
  *   (y1, y2) = factor * (x1 cos a - x2 sin a, x2 cos a + x1 sin a)
  * over pairs (x[i], x[i + R/2]), or (x[2i], x[2i + 1]) with `interleaved`; elements from
  * R = rotary_dim on are copied.  `inverse` turns by -a and divides by factor.  Angles are kept
- * as 64-bit fractions of a turn (at most 2^-33 of a turn off for positions below 2^31), products
- * in fp32, one rounding.
+ * as 64-bit fractions of a turn; they are off by at most 2^-26 of a turn (their conversion to fp32)
+ * and 2^-54 of a turn a position (the 53 bits of inv_freq / 2 pi): 2^-22 of a turn in all below
+ * position 2^31.  Products in fp32, one rounding.
  *
  *  q, k       [batch, tokens, heads, head_dim]; strides {batch, token, head, dim}; k may be NULL
  *  dtype      SC_DTYPE_F16, _BF16 or _F32 of all four tensors

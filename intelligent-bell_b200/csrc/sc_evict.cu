@@ -20,7 +20,8 @@
 // HBM bounds both: every kept row is read and written once.
 //
 // Measured: 128 rows of up to 8,192 tokens to 2,048, selection 11 us and move 49, as long as a plain
-// copy of the kept rows; 8 rows of 131,072 to 16,384, 20.5 and 26.
+// copy of the kept rows; 8 rows of 131,072 to 16,384, 20.5 and 26.  In place the latter's move takes 345:
+// 72 blocks of 128 threads, each 128 rounds that wait for one another.
 #include <cooperative_groups.h>
 
 #include "sc_common.cuh"
@@ -35,7 +36,7 @@ constexpr int kSelWarps = kSelThreads / 32;
 constexpr int kBins = 2048;
 constexpr int kMaxCluster = 16;
 constexpr int kMaxKeys = 32;  // a thread
-constexpr int kMaxTokens = 393216;
+constexpr int kMaxTokens = 393216;  // as documented; the registers of 16 blocks would hold 524,288 keys
 
 struct SelectParams {
     const float* scores;
@@ -436,9 +437,9 @@ extern "C" int32_t sc_evict_tokens(int32_t batch, int32_t n_heads, int64_t cache
     sp.budget = static_cast<int32_t>(budget);
     sp.first = static_cast<int32_t>(keep_first), sp.recent = static_cast<int32_t>(keep_recent);
     sp.status = status;
-    // A cluster where there are fewer rows than SMs, down to 16 keys a thread (8 rows of 131,072:
-    // 26.7 us; 8 keys and twice the blocks 29.0, 32 keys 43.4), or where one block cannot hold a
-    // row's keys.
+    // A cluster where there are fewer rows than SMs, down to 16 keys a thread (8 rows of 131,072 to
+    // 16,384, move included: 47.2 us; 8 keys and twice the blocks 61.0, 32 keys 57.4), or where one
+    // block cannot hold a row's keys.
     int ranks = 1;
     auto per_thread = [&] { return (cache_len + ranks * kSelThreads - 1) / (ranks * kSelThreads); };
     while (ranks < kMaxCluster && (per_thread() > kMaxKeys || (rows * ranks * 2 <= 148 && per_thread() > 16)))

@@ -11,15 +11,16 @@
 // Angles.  p * f_i in fp32 is off by up to 2^-24 p f_i radians, 0.03 at p = 10^6, so the angle
 // is kept as a fraction of a turn in 64-bit fixed point: the host gives F_i = f_i / (2 pi) *
 // 2^64 and the product p * F_i modulo 2^64 IS the fraction (whole turns fall off the top),
-// exact but for the rounding of F_i.  The top bits, as a signed number in [-1, 1) of half
-// turns, go to sincospif, which then needs no range reduction.
+// exact but for F_i, which has a double's 53 bits (f_i <= 1: 2^-55 of a turn off, 2^-24 at p = 2^31).
+// It goes as a signed fp32 number in [-1, 1) of half turns, 2^-25 of one off, to sincospif, which
+// then needs no range reduction.
 //
 // What bounds it: HBM (two 16-bit values read and written for 3 multiplications).  A block
 // loads the slices of its rows first, then tabulates its tokens' cosines and sines in shared
 // memory while they are in flight (64 per token at R = 128, used by every head of q and k), then
-// turns and stores.  32 + 8 heads of 128 for 8,192 tokens: 36.3 us, a plain copy of the same bytes
-// 32.7.  Blocks of 128 threads with two items each in flight (one or four: 39.2 and 39.6 us for
-// 35.5; 512 threads: 51.9).
+// turns and stores.  32 + 8 heads of 128 for 8,192 tokens: 36.5 us, a plain copy of the same bytes
+// 32.7.  Blocks of 128 threads with two items each in flight (one 36.9, four 36.8 us; blocks of 512
+// threads 51.6).
 #include <math.h>
 
 #include "sc_common.cuh"

@@ -196,8 +196,8 @@ def apply_rotary(
         q_out, k_out: outputs of the inputs' shape and dtype, any strides (a cache's next slots, or
             the input itself, apart from the other input); new contiguous tensors by default.
 
-    Angles are kept to 2^-33 of a turn at any position below 2^31; products are in float32 and
-    rounded once.  Returns ``q_out``, or ``(q_out, k_out)`` when keys are given.
+    Angles are off by at most 2^-26 of a turn (their conversion to float32) and 2^-54 of a turn a
+    position (the frequency's 53 bits); products are in float32 and rounded once.  Returns ``q_out``, or ``(q_out, k_out)`` when keys are given.
     """
     require_cuda(q)
     require_no_grad("apply_rotary", q, k, q_out, k_out)
