@@ -365,7 +365,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             float all = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kWarps; ++w) all = fmaxf(all, s_m[w][r]);
-            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - all) * kOnePiece;
+            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - all) * kOnePiece<T>;
 #pragma unroll
             for (int n = 0; n < DP / 8; ++n)
                 *reinterpret_cast<float2*>(s_o + (warp * MR + r) * DP + n * 8 + (lane & 3) * 2) =
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - all));
         const int j = static_cast<int>(fdiv(r0 + r, p.div_G));
         const int64_t at = part_row + static_cast<int64_t>(tok0 + j) * p.Hq + h * p.G + r0 + r - j * p.G;
-        p.part_ml[at] = make_float2(all - kLift<T>, sum);
+        p.part_ml[at] = make_float2(all, sum * kUnlift<T>);
         if (odd) add_odd(p.part_o + at * p.D, p.D, s_odd, DP, min(t1, see + j + 1));
     }
 }

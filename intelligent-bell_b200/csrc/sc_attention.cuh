@@ -195,12 +195,15 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 // Where memory bounds a kernel, a weight x >= 0 goes into its product with V as hi + lo, 2^-16 (bfloat16)
 // or 2^-20 (float16) of x off.  hi is x rounded down and lo the rest plus 2^-12 x, so that lo is above
 // zero wherever x is: an infinite value times either piece is that infinity, and their sum too (with a lo
-// of zero or below it would be NaN).  Sums are 1 + 2^-12 too large, which kOnePiece takes back.
-constexpr float kOnePiece = 1.f / (1.f + 0x1p-12f);
-// float16 begins at 2^-24, so its weights are lifted: 2^15 for the largest, whose sums and maxima (15
-// lower) stay float32.
+// of zero or below it would be NaN).  float16 begins at 2^-24, so its weights are lifted: 2^15 for the
+// largest.  A part's sums of weights (kUnlift) and of values (kUnlift, and the 2^-12 taken back) go out
+// without either, so that its lse keeps its bits.
 template <typename T>
 constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
+template <typename T>
+constexpr float kUnlift = std::is_same<T, __half>::value ? 0x1p-15f : 1.f;
+template <typename T>
+constexpr float kOnePiece = kUnlift<T> / (1.f + 0x1p-12f);
 template <typename T>
 __device__ __forceinline__ void two_pieces(float x, float y, uint32_t& hi, uint32_t& lo) {
     float2 r;

@@ -579,7 +579,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                 float top = s_m[0][r];
 #pragma unroll
                 for (int w = 1; w < kSWarps; ++w) top = fmaxf(top, s_m[w][r]);
-                const float f = m[0][e] == kNegInf ? 0.f : exp2_fast(m[0][e] - top) * kOnePiece;
+                const float f = m[0][e] == kNegInf ? 0.f : exp2_fast(m[0][e] - top) * kOnePiece<T>;
 #pragma unroll
                 for (int k = 0; k < OK; ++k) {
                     o[0][k][e] *= f;
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
             float top = s_m[0][r];
 #pragma unroll
             for (int w = 1; w < kSWarps; ++w) top = fmaxf(top, s_m[w][r]);
-            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - top) * kOnePiece;
+            const float f = m[mt][e] == kNegInf ? 0.f : exp2_fast(m[mt][e] - top) * kOnePiece<T>;
 #pragma unroll
             for (int k = 0; k < DP / 8; ++k) {
                 o[mt][k][2 * e] *= f;
@@ -679,7 +679,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                 sum += s_l[w][r] * (s_m[w][r] == kNegInf ? 0.f : exp2_fast(s_m[w][r] - top));
             const int jq = static_cast<int>(fdiv(r0 + r, p.div_G));
             const int64_t row = static_cast<int64_t>(x.tok0 + jq) * p.Hq + x.h * p.G + r0 + r - jq * p.G;
-            p.part_ml[part * all_rows + row] = make_float2(top - kLift<T>, sum);
+            p.part_ml[part * all_rows + row] = make_float2(top, sum * kUnlift<T>);
             if (odd) add_odd(p.part_o + (part * all_rows + row) * p.D, p.D, s_odd, DP, min(x.len, see + jq + 1));
             if (last)  // parts that this row tile does not have
                 for (int k = part + 1; k < parts_end; ++k) p.part_ml[k * all_rows + row] = make_float2(kNegInf, 0.f);

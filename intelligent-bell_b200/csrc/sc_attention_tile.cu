@@ -41,6 +41,8 @@ template <typename T>
 constexpr float kRaise = std::is_same<T, __half>::value ? 6.f : 8.f;
 template <typename T>
 constexpr float kLiftTile = std::is_same<T, __half>::value ? 9.f : 0.f;
+template <typename T>
+constexpr float kUnliftTile = std::is_same<T, __half>::value ? 0x1p-9f : 1.f;  // of what goes out as a part or lse
 
 template <int DP>
 struct TileShape {
@@ -694,9 +696,9 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                 if (*reinterpret_cast<volatile int*>(&s_any_odd)) add_odd_tmem<DP>(o_at, s_odd, own_limit);
                 if (mine) {
                     if (!direct)
-                        p.part_ml[part_at(r)] = make_float2(m - kLiftTile<T>, l);
+                        p.part_ml[part_at(r)] = make_float2(m, l * kUnliftTile<T>);
                     else if (p.lse)
-                        p.lse[at] = l == 0.f ? kNegInf : (m - kLiftTile<T> + log2f(l)) * 0.6931471805599453f;
+                        p.lse[at] = l == 0.f ? kNegInf : (m + log2f(l * kUnliftTile<T>)) * 0.6931471805599453f;
                 }
                 // 128 bytes of each of the warp's 32 rows at a time, turned in shared memory (where the
                 // warp's queries were) so that a store covers whole lines: a lane's 16 bytes in 32 rows
@@ -716,6 +718,11 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                     tmem_ld32(o_at + c, o);
                     if (direct) tmem_ld32(o_at + c + 32, o + 32);
                     tmem_wait_ld();
+                    if constexpr (kUnliftTile<T> != 1.f) {
+                        if (!direct)
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * kUnliftTile<T>);
+                    }
                     if (direct) {
 #pragma unroll
                         for (int e = 0; e < 32; ++e)

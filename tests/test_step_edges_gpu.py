@@ -248,3 +248,21 @@ def test_many_weights_far_below_the_largest(scb, dtype, n, hq, hk, nats, first):
     err = (out.cpu().double() - want).abs().amax((0, 1))
     assert bool((err <= tol).all()), f"{err[0].item():.3g} of {rest:.3g} (most {tol[0].item():.3g})"
     assert float((lse.cpu().double() - nats - math.log(total)).abs().max()) <= 2.0 ** -20 * nats + p * 2.0 ** -23
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hk", [(1, 8, 2), (2, 16, 2), (1, 256, 2), (40, 8, 2), (100, 8, 2)])  # streams, tiles
+def test_lse_keeps_its_bits(scb, dtype, n, hq, hk):
+    """Equal scores of zero over up to 300 tokens: lse is ln of their number to 2^-22 of it and 2^-21, whatever
+    weights are lifted by."""
+    b, d = 2, 64
+    q = torch.zeros((b * n, hq, d), dtype=dtype, device=DEV)
+    kv = torch.ones((b, n + 20, hk, d), dtype=dtype, device=DEV)
+    for p in (1, 3, 130, 200):
+        kp = torch.ones((p, hk, d), dtype=dtype, device=DEV)
+        out, lse = scb.shared_prefix_attention(q, kp, kp, kv, kv)
+        seen = p + 21 + torch.arange(n, dtype=torch.float64).repeat(b)[:, None].expand(-1, hq)
+        # sums of ones are exact; log2 and its product with ln 2 are off by 2^-23 of a value below 2^3 each
+        assert float((lse.cpu().double() - torch.log(seen)).abs().max()) <= 2.0 ** -21 + 2.0 ** -22 * math.log(p + 21 + n)
+        # the weights' one rounding is a factor of both sums; the output's is half a step
+        assert float((out.double() - 1).abs().max()) <= torch.finfo(dtype).eps / 2 + 2.0 ** -15
