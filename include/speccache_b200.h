@@ -383,7 +383,7 @@ SC_API int32_t sc_rope_apply(int32_t batch, int64_t n_tokens, int32_t q_heads, i
  * of the sequence's own cache, the tokens t <= len - n + j (query j of n), so the newest query
  * sees all of it.  A row that sees nothing gives zeros and a log-sum-exp of -infinity.
  * What a row does not see never reaches it, NaN and infinities included; an infinite value that it
- * sees gives an infinity or NaN.
+ * sees gives that infinity (NaN with the other one, or where its weight is too small for the type).
  *
  *  q, out       [n_tokens, q_heads, head_dim], the sequences' tokens one after another; strides
  *               {token, head}; unit stride along head_dim in every tensor
