@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
             for (int n = 0; n < TK / 8; ++n)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    float x = s[mt][n][e] * p.scale_log2;
+                    float x = __fmul_rn(s[mt][n][e], p.scale_log2);  // as the maximum has it, not fused below
                     if (mask) {
                         const int t = tt + n * 8 + (lane & 3) * 2 + (e & 1);
                         bool seen = t < lim[mt][e >> 1];
@@ -301,7 +301,8 @@ __global__ void __launch_bounds__(kThreads) attend_rows(const __grid_constant__ 
                     }
                 }
             }
-            const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>, mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
+            const float base[2] = {mx[0] == kNegInf ? 0.f : lifted<T>(mx[0], kLift<T>),
+                                   mx[1] == kNegInf ? 0.f : lifted<T>(mx[1], kLift<T>)};
 #pragma unroll
             for (int n = 0; n < TK / 8; ++n)
 #pragma unroll

@@ -195,15 +195,23 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 // Where memory bounds a kernel, a weight x >= 0 goes into its product with V as hi + lo, 2^-16 (bfloat16)
 // or 2^-20 (float16) of x off.  hi is x rounded down and lo the rest plus 2^-12 x, so that lo is above
 // zero wherever x is: an infinite value times either piece is that infinity, and their sum too (with a lo
-// of zero or below it would be NaN).  float16 begins at 2^-24, so its weights are lifted: 2^15 for the
-// largest.  A part's sums of weights (kUnlift) and of values (kUnlift, and the 2^-12 taken back) go out
+// of zero or below it would be NaN).  float16 begins at 2^-24, so its weights are lifted: 2^16 for the
+// largest, of which hi is float16's largest number and lo the rest.  A part's sums of weights (kUnlift) and of values (kUnlift, and the 2^-12 taken back) go out
 // without either, so that its lse keeps its bits.
 template <typename T>
-constexpr float kLift = std::is_same<T, __half>::value ? 15.f : 0.f;
+constexpr float kLift = std::is_same<T, __half>::value ? 16.f : 0.f;
 template <typename T>
-constexpr float kUnlift = std::is_same<T, __half>::value ? 0x1p-15f : 1.f;
+constexpr float kUnlift = std::is_same<T, __half>::value ? 0x1p-16f : 1.f;
 template <typename T>
 constexpr float kOnePiece = kUnlift<T> / (1.f + 0x1p-12f);
+// What weights are taken from for a maximum m: it less the lift, or m itself where it is so large that the
+// difference rounds to more.  (A lift of 2^k is exact up to maxima of 2^(24 + k).)
+template <typename T>
+__device__ __forceinline__ float lifted(float m, float lift) {
+    if constexpr (!std::is_same<T, __half>::value) return m;
+    const float base = m - lift;
+    return m - base <= lift + 0.5f ? base : m;
+}
 template <typename T>
 __device__ __forceinline__ void two_pieces(float x, float y, uint32_t& hi, uint32_t& lo) {
     float2 r;

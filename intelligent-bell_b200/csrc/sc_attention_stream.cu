@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                     float mx[2] = {m[0][0], m[0][1]};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        float v = (s[0][e] + s[1][e]) * p.scale_log2;
+                        float v = __fmul_rn(s[0][e] + s[1][e], p.scale_log2);  // as the maximum has it, not fused below
                         if (mask) {
                             const int t = tt + (lane >> 2) + (e >> 1) * 8;
                             bool seen = t < lim[0][e & 1];
@@ -421,8 +421,8 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                             }
                         }
                     }
-                    const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>,
-                                           mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
+                    const float base[2] = {mx[0] == kNegInf ? 0.f : lifted<T>(mx[0], kLift<T>),
+                                           mx[1] == kNegInf ? 0.f : lifted<T>(mx[1], kLift<T>)};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         s[0][e] = exp2_fast(s[0][e] - base[e & 1]);
@@ -478,7 +478,7 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                         for (int k = 0; k < 2; ++k)
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
-                                float v = s[mt][k][e] * p.scale_log2;
+                                float v = __fmul_rn(s[mt][k][e], p.scale_log2);
                                 if (mask) {
                                     const int t = tt + k * 8 + (lane & 3) * 2 + (e & 1);
                                     bool seen = t < lim[mt][e >> 1];
@@ -506,8 +506,8 @@ __global__ void __launch_bounds__(kSThreads, StreamShape<DP, MT>::kBlocks) atten
                                 }
                             }
                         }
-                        const float base[2] = {mx[0] == kNegInf ? 0.f : mx[0] - kLift<T>,
-                                               mx[1] == kNegInf ? 0.f : mx[1] - kLift<T>};
+                        const float base[2] = {mx[0] == kNegInf ? 0.f : lifted<T>(mx[0], kLift<T>),
+                                               mx[1] == kNegInf ? 0.f : lifted<T>(mx[1], kLift<T>)};
 #pragma unroll
                         for (int k = 0; k < 2; ++k)
 #pragma unroll

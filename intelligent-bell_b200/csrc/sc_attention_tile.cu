@@ -10,7 +10,7 @@
 //   O += P V          A operand from tensor memory, fp32 accumulators in tensor memory.
 // Two row tiles take turns: while the tensor cores work on one, eight warps turn the other's
 // scores into weights.  (With one row tile, two token tiles' scores do.)  The running maximum that scales
-// O is only raised when a score passes it by 2^8 (float16: 2^6), so O is rarely rescaled; weights above
+// O is only raised when a score passes it by 2^8 (float16: 2^7), so O is rarely rescaled; weights above
 // one and their fp32 sums lose nothing.
 //
 // Roles: warps 0-3 and 4-7 the softmax of row tile 0 and 1, warps 8-10 the copies, warp 11 issues
@@ -34,15 +34,16 @@ constexpr int kLoadWarps = 3;
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
 // log2: how far a score may pass the maximum in use, and by how much weights are lifted.  float16 ends at
-// 2^16 and begins at 2^-24, so that lifted its weights count down to 2^-34 of the largest (as they are,
+// 2^16 and begins at 2^-24, so that lifted its weights count down to 2^-33 of the largest (as they are,
 // 2^17 tokens 2^25 below the largest would be lost: 2^-8 of the sum); bfloat16 has room on both sides.
-// 24 sequences of float16 behind 32,768: 47.3 us, 2^4 and 2^11 49.2 (O is rescaled more often), 2^8 and 2^7 47.1.
+// 24 sequences of float16 behind 32,768: 47 us, with 2^4 and 2^11 49 (O is rescaled more often).
 template <typename T>
-constexpr float kRaise = std::is_same<T, __half>::value ? 6.f : 8.f;
+constexpr float kRaise = std::is_same<T, __half>::value ? 7.f : 8.f;
 template <typename T>
-constexpr float kLiftTile = std::is_same<T, __half>::value ? 9.f : 0.f;
+constexpr float kLiftTile = std::is_same<T, __half>::value ? 8.f : 0.f;
+constexpr float kFar = 4194304.f;  // 2^22: scores of such a maximum are 1/4 off from their exact product
 template <typename T>
-constexpr float kUnliftTile = std::is_same<T, __half>::value ? 0x1p-9f : 1.f;  // of what goes out as a part or lse
+constexpr float kUnliftTile = std::is_same<T, __half>::value ? 0x1p-8f : 1.f;  // of what goes out as a part or lse
 
 template <int DP>
 struct TileShape {
@@ -594,7 +595,8 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             }
                         }
                     };
-                    if (!masked && p.scale_log2 > 0.f) {
+                    bool quick = !masked && p.scale_log2 > 0.f;
+                    if (quick) {
                         // All scores in registers, one pass.
                         uint32_t x[128];
 #pragma unroll
@@ -606,30 +608,35 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                             t4[(e >> 1) & 3] = max3(t4[(e >> 1) & 3], __uint_as_float(x[e]), __uint_as_float(x[e + 1]));
                         raised(fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * p.scale_log2);
                         if (!alive) break;
-                        const float base = m == kNegInf ? 0.f : m - kLiftTile<T>;
-                        const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
-                        float2 sum = make_float2(0.f, 0.f), sum2 = sum;
+                        // The fused product below is off from the maximum by its rounding, which must not count.
+                        quick = !__any_sync(0xffffffffu, fabsf(m) >= kFar);
+                        if (quick) {
+                            const float base = m == kNegInf ? 0.f : lifted<T>(m, kLiftTile<T>);
+                            const float2 mul2 = make_float2(p.scale_log2, p.scale_log2), sub2 = make_float2(-base, -base);
+                            float2 sum = make_float2(0.f, 0.f), sum2 = sum;
 #pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            uint32_t w[16];
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t w[16];
 #pragma unroll
-                            for (int e = 0; e < 16; ++e) {
-                                float2 v = make_float2(__uint_as_float(x[c * 32 + 2 * e]),
-                                                       __uint_as_float(x[c * 32 + 2 * e + 1]));
-                                v = __ffma2_rn(v, mul2, sub2);
-                                v.x = exp2_fast(v.x);
-                                v.y = exp2_fast(v.y);
-                                if (e & 1)
-                                    sum2 = __fadd2_rn(sum2, v);
-                                else
-                                    sum = __fadd2_rn(sum, v);
-                                w[e] = pack2<T>(v.x, v.y);
+                                for (int e = 0; e < 16; ++e) {
+                                    float2 v = make_float2(__uint_as_float(x[c * 32 + 2 * e]),
+                                                           __uint_as_float(x[c * 32 + 2 * e + 1]));
+                                    v = __ffma2_rn(v, mul2, sub2);
+                                    v.x = exp2_fast(v.x);
+                                    v.y = exp2_fast(v.y);
+                                    if (e & 1)
+                                        sum2 = __fadd2_rn(sum2, v);
+                                    else
+                                        sum = __fadd2_rn(sum, v);
+                                    w[e] = pack2<T>(v.x, v.y);
+                                }
+                                tmem_st16(s_at + c * 16, w);
                             }
-                            tmem_st16(s_at + c * 16, w);
+                            l += (sum.x + sum.y) + (sum2.x + sum2.y);
                         }
-                        l += (sum.x + sum.y) + (sum2.x + sum2.y);
-                    } else {
-                        // A tile's end, a mask, or a scale that turns the order: the few of these take short
+                    }
+                    if (!quick) {
+                        // A tile's end, a mask, a scale that turns the order, far scores: the few of these take short
                         // loops, which leave the others' instructions together (eight prompts of up to
                         // 512 tokens behind 8,192: 459 us, this way 452).
                         const bool turned = p.scale_log2 <= 0.f;
@@ -659,15 +666,15 @@ __global__ void __launch_bounds__(kTThreads, 1) attend_tiles(const __grid_consta
                         }
                         raised(top * mul);
                         if (!alive) break;
-                        const float base = m == kNegInf ? 0.f : m - kLiftTile<T>;
+                        const float base = m == kNegInf ? 0.f : lifted<T>(m, kLiftTile<T>);
 #pragma unroll 1
                         for (int c = 0; c < kTokTile; c += 16) {
                             uint32_t x[16], w[8];
                             scores(c, x);
 #pragma unroll
                             for (int e = 0; e < 8; ++e) {
-                                const float v0 = exp2_fast(fmaf(__uint_as_float(x[2 * e]), mul, -base));
-                                const float v1 = exp2_fast(fmaf(__uint_as_float(x[2 * e + 1]), mul, -base));
+                                const float v0 = exp2_fast(__fsub_rn(__fmul_rn(__uint_as_float(x[2 * e]), mul), base));
+                                const float v1 = exp2_fast(__fsub_rn(__fmul_rn(__uint_as_float(x[2 * e + 1]), mul), base));
                                 l += v0 + v1;
                                 w[e] = pack2<T>(v0, v1);
                             }

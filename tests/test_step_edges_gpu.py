@@ -240,11 +240,12 @@ def test_many_weights_far_below_the_largest(scb, dtype, n, hq, hk, nats, first):
     rest, total = (p - 1) * w, 1 + (p - 1) * w
     want = torch.full((d,), 1.0, dtype=torch.float64)
     want[:32] = rest / total
-    # A weight is off by half a step of the type (float16: or 2^-34, its lifted end) and the output once more,
+    # A weight is off by half a step of the type (float16: or 2^-33, half a step of its end
+    # lifted by 2^8) and the output once more,
     # which float16 holds in steps of 2^-24 below 2^-14; the exponentials and sums by 2^-21 + p 2^-23.
     u = torch.finfo(dtype).eps / 2
     tol = (2 * u + 2.0 ** -21 + p * 2.0 ** -23) * want + 2.0 ** -25
-    tol += p * 2.0 ** -34 if dtype == torch.float16 else 0.0
+    tol += p * 2.0 ** -33 if dtype == torch.float16 else 0.0
     err = (out.cpu().double() - want).abs().amax((0, 1))
     assert bool((err <= tol).all()), f"{err[0].item():.3g} of {rest:.3g} (most {tol[0].item():.3g})"
     assert float((lse.cpu().double() - nats - math.log(total)).abs().max()) <= 2.0 ** -20 * nats + p * 2.0 ** -23
@@ -266,3 +267,39 @@ def test_lse_keeps_its_bits(scb, dtype, n, hq, hk):
         assert float((lse.cpu().double() - torch.log(seen)).abs().max()) <= 2.0 ** -21 + 2.0 ** -22 * math.log(p + 21 + n)
         # the weights' one rounding is a factor of both sums; the output's is half a step
         assert float((out.double() - 1).abs().max()) <= torch.finfo(dtype).eps / 2 + 2.0 ** -15
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("n,hq,hk,page", [(1, 8, 2, 0), (2, 16, 2, 0), (2, 16, 2, 5), (1, 256, 2, 0), (40, 8, 2, 0),
+                                          (100, 8, 2, 0)])  # streams, copies without tensor maps, tiles
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_far_beyond_the_weights_range(scb, dtype, n, hq, hk, page, sign):
+    """Scores of up to 2^29: the largest one's value and nothing else, in float16 as in bfloat16."""
+    b, p, d, cap = 2, 301, 64, n + 20
+    q = torch.zeros((b * n, hq, d), dtype=dtype, device=DEV)
+    q[..., 0] = 59968.0
+    kp = torch.zeros((p, hk, d), dtype=dtype, device=DEV)
+    kp[..., 0] = (sign * (48000.0 - 32.0 * torch.arange(p, device=DEV))).to(dtype)[:, None]
+    best = 260  # a token above all others: twice the largest, or half the smallest
+    kp[best, :, 0] = 65024.0 if sign > 0 else -16000.0
+    vp = (torch.arange(p * d, device=DEV).view(p, 1, d) % 7).expand(p, hk, d).to(dtype).contiguous()
+    shape = (b * cap // page, page, hk, d) if page else (b, cap, hk, d)
+    if page:
+        cap = cap // page * page
+        shape = (b * cap // page, page, hk, d)
+    kc = torch.zeros(shape, dtype=dtype, device=DEV)
+    kc[..., 0] = -65024.0 if sign < 0 else 1000.0
+    table = torch.arange(b * cap // page, dtype=torch.int32, device=DEV).view(b, -1) if page else None
+    out, lse = scb.shared_prefix_attention(q, kp, vp, kc, kc, page_table=table)
+    # the largest weight is a power of two, so nothing is rounded
+    assert torch.equal(out, vp[best].repeat_interleave(hq // hk, 0).expand_as(out).to(dtype))
+    want = float(q[0, 0, 0]) * float(kp[best, 0, 0]) / 8
+    assert float((lse.double() - want).abs().max()) <= 2.0 ** -21 * abs(want)
+    # scores of 2^24, 2 apart in units of log2: the parts of a split agree on what is largest
+    kp[..., 0] = 0.0
+    kp[5, :, 0], kp[290, :, 0] = 1024.0, 1026.0 if dtype == torch.float16 else 1032.0
+    q[..., 0] = 32768.0 * sign
+    if sign > 0:
+        kc[..., 0] = 0.0
+        out, _ = scb.shared_prefix_attention(q, kp, vp, kc, kc, page_table=table, scale=math.log(2.0) / 2)
+        assert torch.equal(out, vp[290].repeat_interleave(hq // hk, 0).expand_as(out).to(dtype))
